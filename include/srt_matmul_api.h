@@ -431,6 +431,64 @@ cudaError_t srtGruCell(
     void* newHidden, const srtTensorDescriptor* newHiddenDesc,
     cudaStream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * srtGatedRecurrence: a gated linear recurrence over whole sequences, and its backward pass.
+ *
+ * The reference's recurrent cells multiply the previous hidden state by a weight at every step
+ * (Sources/SwiftRTLayers/Recurrent.swift:255-266, 328-337), so a sequence is as many products as it
+ * has steps.  Here the gates depend on the layer's input alone: they are column blocks of ONE product
+ * over all steps, named as in the LSTM cell (Part, Recurrent.swift:173), and what remains of the
+ * recurrence is elementwise.  Per batch item and channel, with s the logistic function,
+ *     f = s(forget_t),   i = input ? s(input_t) : 1 - f
+ *     c_t = f c_{t-1} + i update_t,      hidden_t = output ? c_t s(output_t) : c_t
+ * update, forget, input, output, hidden: [batch x steps x channels], or rank 2 [batch x channels] for one
+ * step (generation); real32F, real16F or real16BF, all of one type, any strides (the column blocks of a
+ * fused product are such views).  input and output may be NULL.
+ * The state c is Float32 whatever the type.  initial (NULL: zero) and last (NULL: not wanted) are
+ * [batch x channels]; last may be initial, which advances a state in place.
+ * lengths (NULL: all steps) points at one int32 per batch item on the device, taken as 0 .. steps: a step
+ * at or behind it leaves the state as it is, its inputs are not read (they may hold anything) and its
+ * hidden value is zero.
+ * states (NULL: not wanted) is Float32 [batch x ceil(steps / 64) x channels] and receives the state before
+ * steps 0, 64, 128, ...: what srtGatedRecurrenceBackward needs.
+ * Outputs must not overlap each other or an input (but last, see above).  One launch on `stream`, no workspace; no
+ * steps: last = initial.  A call without elements launches nothing. */
+#define SRT_GATED_RECURRENCE_CHUNK 64
+cudaError_t srtGatedRecurrence(
+    const void* update, const srtTensorDescriptor* updateDesc,
+    const void* forget, const srtTensorDescriptor* forgetDesc,
+    const void* input, const srtTensorDescriptor* inputDesc,
+    const void* output, const srtTensorDescriptor* outputDesc,
+    const void* initial, const srtTensorDescriptor* initialDesc,
+    const int32_t* lengths,
+    void* hidden, const srtTensorDescriptor* hiddenDesc,
+    void* last, const srtTensorDescriptor* lastDesc,
+    void* states, const srtTensorDescriptor* statesDesc,
+    cudaStream_t stream);
+
+/* Gradients of srtGatedRecurrence.  outGrad is the gradient of hidden, lastGrad (NULL: zero) that of last; update,
+ * forget, input, output and lengths as in the forward call, states as it left them.  dUpdate, dForget, dInput and
+ * dOutput have the type and extents of their tensors (dInput and dOutput are ignored where the gate is NULL), dInitial
+ * (NULL: not wanted) is Float32 [batch x channels].  Gradients at or behind an item's length are zero, and outGrad is
+ * not read there.  A gradient is that of every element of the tensor as described: one of a broadcast (zero-stride)
+ * input is not summed over the repeated elements.  Sums and states are Float32, each gradient is rounded once; the
+ * result does not depend on timing.  One launch, no workspace. */
+cudaError_t srtGatedRecurrenceBackward(
+    const void* outGrad, const srtTensorDescriptor* outGradDesc,
+    const void* lastGrad, const srtTensorDescriptor* lastGradDesc,
+    const void* update, const srtTensorDescriptor* updateDesc,
+    const void* forget, const srtTensorDescriptor* forgetDesc,
+    const void* input, const srtTensorDescriptor* inputDesc,
+    const void* output, const srtTensorDescriptor* outputDesc,
+    const void* states, const srtTensorDescriptor* statesDesc,
+    const int32_t* lengths,
+    void* dUpdate, const srtTensorDescriptor* dUpdateDesc,
+    void* dForget, const srtTensorDescriptor* dForgetDesc,
+    void* dInput, const srtTensorDescriptor* dInputDesc,
+    void* dOutput, const srtTensorDescriptor* dOutputDesc,
+    void* dInitial, const srtTensorDescriptor* dInitialDesc,
+    cudaStream_t stream);
+
 /* ---- several GPUs of one machine, one process per GPU -----------------------------------------
  *
  * The reference has no multi-GPU path: its only data-parallel construct partitions axis 0 of a

@@ -15,3 +15,4 @@ from .sharded import shard_range, sharded_matmul, sharded_matmul_host  # noqa: F
 from .peer import PeerBuffer  # noqa: F401,E402
 from .recurrent import BasicRNNCell, GRUCell, GraphedSequence, LSTMCell, LSTMState, run_sequence, run_sequence_preconcatenated  # noqa: F401,E402
 from .transform import MatrixLayout, leading_dimension, matrix_transform  # noqa: F401,E402
+from .linear_recurrent import STATE_CHUNK, LinearRecurrentCell, gated_recurrence, gated_recurrence_backward  # noqa: F401,E402

@@ -44,7 +44,8 @@ EXPORTS = ["srtMatmul", "srtMatmulBiasActivation", "srtMatmulQueryPlan", "srtMat
            "srtMatmulAllGatherMulticast", "srtMatmulTune", "srtMatmulPlanCacheSave", "srtMatmulPlanCacheLoad", "srtMatmulPlanCacheClear",
            "srtActivationForward", "srtMatmulReleaseWorkspaces", "srtGruCell", "srtShardRange", "srtMatmulSharded",
            "srtMatmulShardedDevices", "srtMatmulSetWaitLimit", "srtLstmCellFused", "srtLstmInterleaveGates", "srtPeerSignal", "srtPeerWait", "srtMulticastAlloc", "srtMulticastFree",
-           "srtMatrixTransform", "srtMatrixLayoutLeadingDimension", "srtMatrixLayoutElementCount"]
+           "srtMatrixTransform", "srtMatrixLayoutLeadingDimension", "srtMatrixLayoutElementCount",
+           "srtGatedRecurrence", "srtGatedRecurrenceBackward"]
 
 if not os.path.exists(SO):
     raise ImportError(
@@ -159,6 +160,11 @@ lib.srtMulticastFree.restype = ctypes.c_int
 lib.srtMulticastFree.argtypes = [_P]
 lib.srtMatmulSetWaitLimit.restype = ctypes.c_int
 lib.srtMatmulSetWaitLimit.argtypes = [ctypes.c_uint64]
+# descriptors are passed by address (Descriptor.address): a call of a single token is bound by its marshalling
+lib.srtGatedRecurrence.restype = ctypes.c_int
+lib.srtGatedRecurrence.argtypes = [_P] * 18
+lib.srtGatedRecurrenceBackward.restype = ctypes.c_int
+lib.srtGatedRecurrenceBackward.argtypes = [_P] * 26
 
 
 def last_error() -> str:

@@ -13,14 +13,13 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 SO = os.path.join(PKG, "libsrt_b200.so")
-SOURCES = [os.path.join(PKG, "csrc", "srt_matmul.cu")]
-HEADERS = [os.path.join(PKG, "csrc", h) for h in ("ptx.cuh", "gemm_tcgen05.cuh", "gemm_simt.cuh", "gemm_splitk.cuh",
-                                                  "dense_backward.cuh", "lstm_cell.cuh")] + [
+SOURCES = [os.path.join(PKG, "csrc", f) for f in ("srt_matmul.cu", "srt_sequence.cu")]
+HEADERS = [os.path.join(PKG, "csrc", h) for h in sorted(os.listdir(os.path.join(PKG, "csrc"))) if h.endswith((".cuh", ".h"))] + [
     os.path.join(ROOT, "include", "srt_matmul_api.h")]
 
 # the explicit -gencode form is required: a bare -arch=sm_100a does not enable tcgen05
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-shared", "-Xcompiler", "-fPIC", "-I" + os.path.join(ROOT, "include")]
+              "-shared", "-Xcompiler", "-fPIC", "--threads", "0", "-I" + os.path.join(ROOT, "include")]
 
 
 def nvcc_path() -> str:

@@ -7,7 +7,6 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
-#include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -20,73 +19,20 @@
 #include "gemm_splitk.cuh"
 #include "gemm_tcgen05.cuh"
 #include "gemm_tf32x3.cuh"
+#include "host_common.h"
 #include "lstm_cell.cuh"
 #include "matrix_transform.cuh"
 
 namespace {
 
 using namespace srt;
+using namespace srt::host;
 
-thread_local char g_error[512] = "";
-std::atomic<uint64_t> g_launches{0};
 std::atomic<uint64_t> g_wait_limit_ns{srt::kDefaultWaitLimitNs};     // srtMatmulSetWaitLimit
 
 struct Tuning {
     std::atomic<int32_t> force_kernel{0}, tile_n{0}, stages{0}, max_ctas{0}, split_k{0};
 } g_tuning;
-
-cudaError_t fail(cudaError_t code, const char* fmt, ...)
-{
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(g_error, sizeof g_error, fmt, ap);
-    va_end(ap);
-    return code;
-}
-
-// ------------------------------------------------------------------ the device of a call
-// Every entry point that takes a stream works on THAT stream's device, whatever device is current
-// on the calling thread: the reference's queues never select a device before they enqueue
-// (Sources/SwiftRTCore/platform/cuda/functions/CudaMath.swift:117-125 launches on `stream` with no
-// device call; nothing calls CudaQueue.selectDevice, cuda/device/CudaQueue.swift:77).  The scope
-// resolves the stream's device, makes it current for the duration of the call when it differs and
-// restores the caller's device afterwards; per-device state (workspaces, kernel attributes, the
-// status word, the static scratch) is keyed by `device`.  The legacy and per-thread default
-// streams belong to whatever device is current.  While a stream is being captured the runtime
-// refuses the device query (and a refused call would invalidate the capture), so a capturing
-// stream is taken to belong to the current device: capture with the stream's device current.
-struct DeviceScope {
-    int device = -1;
-    int previous = -1;
-    cudaError_t status = cudaSuccess;
-    explicit DeviceScope(cudaStream_t stream)
-    {
-        int cur = 0;
-        status = cudaGetDevice(&cur);
-        if (status != cudaSuccess) return;
-        int dev = cur;
-        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-        if (stream != nullptr && stream != cudaStreamLegacy && stream != cudaStreamPerThread &&
-            cudaStreamIsCapturing(stream, &cap) == cudaSuccess && cap == cudaStreamCaptureStatusNone) {
-            status = cudaStreamGetDevice(stream, &dev);
-            if (status != cudaSuccess) {
-                fail(status, "cannot resolve the device of the stream: %s", cudaGetErrorString(status));
-                return;
-            }
-        }
-        device = dev;
-        if (dev != cur) {
-            status = cudaSetDevice(dev);
-            if (status == cudaSuccess) previous = cur;
-        }
-    }
-    ~DeviceScope()
-    {
-        if (previous >= 0) cudaSetDevice(previous);
-    }
-    DeviceScope(const DeviceScope&) = delete;
-    DeviceScope& operator=(const DeviceScope&) = delete;
-};
 
 // ------------------------------------------------------------------ problem description
 struct Problem {
@@ -100,15 +46,6 @@ struct Problem {
     const char* bias; long long bias_stride;
     uint32_t act;
 };
-
-uint32_t elem_size(srtDataType t)
-{
-    switch (t) {
-    case real32F: return 4;
-    case real16F: case real16BF: return 2;
-    default: return 0;
-    }
-}
 
 cudaError_t parse(const void* a, const srtTensorDescriptor* ad, bool ta,
                   const void* b, const srtTensorDescriptor* bd, bool tb,

@@ -1,0 +1,205 @@
+// C ABI of the recurrence over whole sequences: argument checks and launches.  Declarations are in
+// include/srt_matmul_api.h.
+#include "srt_matmul_api.h"
+
+#include <cuda_runtime.h>
+
+#include <cstring>
+
+#include "gated_recurrence.cuh"
+#include "host_common.h"
+
+namespace {
+
+using namespace srt;
+using namespace srt::host;
+
+struct Shape3 { uint64_t B, T, D; };
+
+// rank 3 [batch x steps x channels], or rank 2 [batch x channels] for one step
+cudaError_t shape3(const char* op, const char* what, const srtTensorDescriptor* d, Shape3& s, long long (&strides)[3])
+{
+    if (!d || !d->shape || !d->strides) return fail(cudaErrorInvalidValue, "%s: %s: missing descriptor", op, what);
+    if (d->rank != 2 && d->rank != 3) return fail(cudaErrorInvalidValue, "%s: %s must have rank 3, or rank 2 for one step", op, what);
+    const uint32_t last = d->rank - 1;
+    s.B = d->shape[0];
+    s.T = d->rank == 3 ? d->shape[1] : 1;
+    s.D = d->shape[last];
+    strides[0] = (long long)d->strides[0];
+    strides[1] = d->rank == 3 ? (long long)d->strides[1] : 0;
+    strides[2] = (long long)d->strides[last];
+    return cudaSuccess;
+}
+
+cudaError_t sequence_arg(const char* op, const char* what, const void* ptr, const srtTensorDescriptor* d, srtDataType type, const Shape3& want,
+                         bool written, long long (&strides)[3])
+{
+    Shape3 s;
+    cudaError_t e = shape3(op, what, d, s, strides);
+    if (e != cudaSuccess) return e;
+    if (d->type != type) return fail(cudaErrorInvalidValue, "%s: %s must have the element type of update", op, what);
+    if (s.B != want.B || s.T != want.T || s.D != want.D)
+        return fail(cudaErrorInvalidValue, "%s: %s must be [%llu x %llu x %llu] like update", op, what, (unsigned long long)want.B,
+                    (unsigned long long)want.T, (unsigned long long)want.D);
+    if (!ptr && s.B * s.T * s.D != 0) return fail(cudaErrorInvalidValue, "%s: %s is null", op, what);
+    if (written && ((s.B > 1 && strides[0] == 0) || (s.T > 1 && strides[1] == 0) || (s.D > 1 && strides[2] == 0)))
+        return fail(cudaErrorInvalidValue, "%s: %s must not repeat elements (zero stride)", op, what);
+    return cudaSuccess;
+}
+
+cudaError_t read_arg(const char* op, const char* what, const void* ptr, const srtTensorDescriptor* d, srtDataType type, const Shape3& want, Strided3& out)
+{
+    long long st[3];
+    cudaError_t e = sequence_arg(op, what, ptr, d, type, want, false, st);
+    if (e == cudaSuccess) out = Strided3{ptr, st[0], st[1], st[2]};
+    return e;
+}
+
+cudaError_t write_arg(const char* op, const char* what, void* ptr, const srtTensorDescriptor* d, srtDataType type, const Shape3& want, Strided3W& out)
+{
+    long long st[3];
+    cudaError_t e = sequence_arg(op, what, ptr, d, type, want, true, st);
+    if (e == cudaSuccess) out = Strided3W{ptr, st[0], st[1], st[2]};
+    return e;
+}
+
+// a Float32 state [batch x channels]
+cudaError_t state_arg(const char* op, const char* what, const srtTensorDescriptor* d, const Shape3& want, bool written, long long& sb, long long& sd)
+{
+    if (!d || !d->shape || !d->strides) return fail(cudaErrorInvalidValue, "%s: %s: missing descriptor", op, what);
+    if (d->type != real32F || d->rank != 2 || d->shape[0] != want.B || d->shape[1] != want.D)
+        return fail(cudaErrorInvalidValue, "%s: %s must be Float32 [%llu x %llu]", op, what, (unsigned long long)want.B, (unsigned long long)want.D);
+    sb = (long long)d->strides[0];
+    sd = (long long)d->strides[1];
+    if (written && ((want.B > 1 && sb == 0) || (want.D > 1 && sd == 0)))
+        return fail(cudaErrorInvalidValue, "%s: %s must not repeat elements (zero stride)", op, what);
+    return cudaSuccess;
+}
+
+cudaError_t states_arg(const char* op, const srtTensorDescriptor* d, const Shape3& want, bool written, RecurrenceParams& p)
+{
+    const uint64_t chunks = (want.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
+    if (!d || !d->shape || !d->strides) return fail(cudaErrorInvalidValue, "%s: states: missing descriptor", op);
+    if (d->type != real32F || d->rank != 3 || d->shape[0] != want.B || d->shape[1] != chunks || d->shape[2] != want.D)
+        return fail(cudaErrorInvalidValue, "%s: states must be Float32 [%llu x %llu x %llu]", op, (unsigned long long)want.B,
+                    (unsigned long long)chunks, (unsigned long long)want.D);
+    p.states_b = (long long)d->strides[0];
+    p.states_c = (long long)d->strides[1];
+    p.states_d = (long long)d->strides[2];
+    if (written && ((want.B > 1 && p.states_b == 0) || (chunks > 1 && p.states_c == 0) || (want.D > 1 && p.states_d == 0)))
+        return fail(cudaErrorInvalidValue, "%s: states must not repeat elements (zero stride)", op);
+    return cudaSuccess;
+}
+
+// type and extents of the call, from `update`
+cudaError_t recurrence_shape(const char* op, const srtTensorDescriptor* updateDesc, Shape3& s, RecurrenceParams& p)
+{
+    long long st[3];
+    cudaError_t e = shape3(op, "update", updateDesc, s, st);
+    if (e != cudaSuccess) return e;
+    if (elem_size(updateDesc->type) == 0)
+        return fail(cudaErrorNotSupported, "%s: element type %d is not computed by this library", op, (int)updateDesc->type);
+    if (s.B > 65535 || s.T > 0x7fffffffull || s.D > 0x7fffffffull)
+        return fail(cudaErrorInvalidValue, "%s: dimension exceeds the supported range", op);
+    memset(&p, 0, sizeof p);
+    p.B = (uint32_t)s.B;
+    p.T = (uint32_t)s.T;
+    p.D = (uint32_t)s.D;
+    return cudaSuccess;
+}
+
+template <typename T>
+cudaError_t launch_recurrence(const RecurrenceParams& p, bool backward, cudaStream_t stream)
+{
+    const unsigned long long threads = (unsigned long long)p.B * p.D;
+    const unsigned blocks = (unsigned)((threads + 127) / 128);
+    if (backward) recurrence_steps_backward_kernel<T><<<blocks, 128, 0, stream>>>(p);
+    else          recurrence_steps_kernel<T><<<blocks, 128, 0, stream>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return e;
+}
+
+cudaError_t launch_recurrence_type(srtDataType type, const RecurrenceParams& p, bool backward, cudaStream_t stream)
+{
+    switch (type) {
+    case real32F: return launch_recurrence<float>(p, backward, stream);
+    case real16F: return launch_recurrence<__half>(p, backward, stream);
+    default: return launch_recurrence<__nv_bfloat16>(p, backward, stream);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+cudaError_t srtGatedRecurrence(const void* update, const srtTensorDescriptor* updateDesc, const void* forget, const srtTensorDescriptor* forgetDesc,
+                               const void* input, const srtTensorDescriptor* inputDesc, const void* output, const srtTensorDescriptor* outputDesc,
+                               const void* initial, const srtTensorDescriptor* initialDesc, const int32_t* lengths,
+                               void* hidden, const srtTensorDescriptor* hiddenDesc, void* last, const srtTensorDescriptor* lastDesc,
+                               void* states, const srtTensorDescriptor* statesDesc, cudaStream_t stream)
+{
+    const char* const op = "srtGatedRecurrence";
+    RecurrenceParams p;
+    Shape3 s;
+    cudaError_t e = recurrence_shape(op, updateDesc, s, p);
+    if (e != cudaSuccess) return e;
+    const srtDataType type = updateDesc->type;
+    if ((e = read_arg(op, "update", update, updateDesc, type, s, p.x)) != cudaSuccess) return e;
+    if ((e = read_arg(op, "forget", forget, forgetDesc, type, s, p.f)) != cudaSuccess) return e;
+    if (input && (e = read_arg(op, "input", input, inputDesc, type, s, p.i)) != cudaSuccess) return e;
+    if (output && (e = read_arg(op, "output", output, outputDesc, type, s, p.o)) != cudaSuccess) return e;
+    if ((e = write_arg(op, "hidden", hidden, hiddenDesc, type, s, p.y)) != cudaSuccess) return e;
+    if (initial && (e = state_arg(op, "initial", initialDesc, s, false, p.initial_b, p.initial_d)) != cudaSuccess) return e;
+    if (last && (e = state_arg(op, "last", lastDesc, s, true, p.last_b, p.last_d)) != cudaSuccess) return e;
+    if (states && (e = states_arg(op, statesDesc, s, true, p)) != cudaSuccess) return e;
+    g_error[0] = 0;
+    if (s.B == 0 || s.D == 0 || (s.T == 0 && !last)) return cudaSuccess;
+    p.initial = static_cast<const float*>(initial);
+    p.lengths = lengths;
+    p.last = static_cast<float*>(last);
+    p.states = static_cast<float*>(states);
+    DeviceScope scope(stream);
+    if (scope.status != cudaSuccess) return scope.status;
+    return launch_recurrence_type(type, p, false, stream);
+}
+
+cudaError_t srtGatedRecurrenceBackward(const void* outGrad, const srtTensorDescriptor* outGradDesc, const void* lastGrad, const srtTensorDescriptor* lastGradDesc,
+                                       const void* update, const srtTensorDescriptor* updateDesc, const void* forget, const srtTensorDescriptor* forgetDesc,
+                                       const void* input, const srtTensorDescriptor* inputDesc, const void* output, const srtTensorDescriptor* outputDesc,
+                                       const void* states, const srtTensorDescriptor* statesDesc, const int32_t* lengths,
+                                       void* dUpdate, const srtTensorDescriptor* dUpdateDesc, void* dForget, const srtTensorDescriptor* dForgetDesc,
+                                       void* dInput, const srtTensorDescriptor* dInputDesc, void* dOutput, const srtTensorDescriptor* dOutputDesc,
+                                       void* dInitial, const srtTensorDescriptor* dInitialDesc, cudaStream_t stream)
+{
+    const char* const op = "srtGatedRecurrenceBackward";
+    RecurrenceParams p;
+    Shape3 s;
+    cudaError_t e = recurrence_shape(op, updateDesc, s, p);
+    if (e != cudaSuccess) return e;
+    const srtDataType type = updateDesc->type;
+    if ((e = read_arg(op, "outGrad", outGrad, outGradDesc, type, s, p.dy)) != cudaSuccess) return e;
+    if ((e = read_arg(op, "update", update, updateDesc, type, s, p.x)) != cudaSuccess) return e;
+    if ((e = read_arg(op, "forget", forget, forgetDesc, type, s, p.f)) != cudaSuccess) return e;
+    if (input && (e = read_arg(op, "input", input, inputDesc, type, s, p.i)) != cudaSuccess) return e;
+    if (output && (e = read_arg(op, "output", output, outputDesc, type, s, p.o)) != cudaSuccess) return e;
+    if ((e = write_arg(op, "dUpdate", dUpdate, dUpdateDesc, type, s, p.dx)) != cudaSuccess) return e;
+    if ((e = write_arg(op, "dForget", dForget, dForgetDesc, type, s, p.df)) != cudaSuccess) return e;
+    if (input && (e = write_arg(op, "dInput", dInput, dInputDesc, type, s, p.di)) != cudaSuccess) return e;
+    if (output && (e = write_arg(op, "dOutput", dOutput, dOutputDesc, type, s, p.dout)) != cudaSuccess) return e;
+    if (lastGrad && (e = state_arg(op, "lastGrad", lastGradDesc, s, false, p.dlast_b, p.dlast_d)) != cudaSuccess) return e;
+    if (dInitial && (e = state_arg(op, "dInitial", dInitialDesc, s, true, p.dinitial_b, p.dinitial_d)) != cudaSuccess) return e;
+    if (!states && s.B * s.T * s.D != 0) return fail(cudaErrorInvalidValue, "%s: states is null: the forward pass has to keep them", op);
+    if ((e = states_arg(op, statesDesc, s, false, p)) != cudaSuccess) return e;
+    g_error[0] = 0;
+    if (s.B == 0 || s.D == 0 || (s.T == 0 && !dInitial)) return cudaSuccess;
+    p.dlast = static_cast<const float*>(lastGrad);
+    p.lengths = lengths;
+    p.states = static_cast<float*>(const_cast<void*>(states));
+    p.dinitial = static_cast<float*>(dInitial);
+    DeviceScope scope(stream);
+    if (scope.status != cudaSuccess) return scope.status;
+    return launch_recurrence_type(type, p, true, stream);
+}
+
+}  // extern "C"

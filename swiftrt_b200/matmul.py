@@ -47,13 +47,36 @@ _DESC_CACHE_MAX = 512
 def _descriptor(t: torch.Tensor) -> Descriptor:
     """Descriptor for a tensor's geometry; built once per (shape, strides, dtype) and reused --
     descriptors hold no pointer, so tensors with equal geometry share one."""
-    key = (t.dtype, tuple(t.shape), t.stride())
+    key = (t.dtype, t.shape, t.stride())
     d = _DESC_CACHE.get(key)
     if d is None:
         if len(_DESC_CACHE) >= _DESC_CACHE_MAX:
             _DESC_CACHE.clear()
         d = _DESC_CACHE[key] = Descriptor(t)
     return d
+
+
+def enqueue(fn, device: torch.device, *args) -> None:
+    """Calls `fn(*args, stream)` with torch's current stream of `device`, that device being current (a legacy
+    default stream belongs to whatever device is); raises MatmulError for a non-zero status."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if rc != _lib.cudaSuccess:
+        raise MatmulError(rc, _lib.last_error())
+
+
+def on_one_device(first: torch.Tensor, *others) -> None:
+    """All tensors (None is skipped) on the device of `first`, a CUDA device."""
+    if not first.is_cuda:
+        raise ValueError("device tensors expected")
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on different devices: {device} and {t.device}")
 
 
 class MatmulOp:

@@ -85,7 +85,7 @@ typedef struct {
 
 /* Raw values equal ActivationType (Sources/SwiftRTCore/platform/common/
  * FunctionProperties.swift:44-51).  srtActivationGelu / GeluTanh are additions (the
- * reference enum has no GELU).  clippedRelu and elu take coefficients the Dense layer
+ * reference enum has no GELU); so is srtActivationSilu.  clippedRelu and elu take coefficients the Dense layer
  * never supplies and return cudaErrorNotSupported. */
 typedef enum {
     srtActivationSigmoid     = 0,
@@ -95,7 +95,8 @@ typedef enum {
     srtActivationElu         = 4,
     srtActivationIdentity    = 5,
     srtActivationGelu        = 6,
-    srtActivationGeluTanh    = 7
+    srtActivationGeluTanh    = 7,
+    srtActivationSilu        = 8    /* z s(z); srtMatmulGated and srtMatmulInt4 only, the other entry points return cudaErrorNotSupported */
 } srtActivationType;
 
 /* ---------------------------------------------------------------------------------------
@@ -429,6 +430,56 @@ cudaError_t srtGruCell(
     const void* outputWeight, const srtTensorDescriptor* outputWeightDesc,
     const void* outputBias, const srtTensorDescriptor* outputBiasDesc,
     void* newHidden, const srtTensorDescriptor* newHiddenDesc,
+    cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * srtMatmulGated: out = activation(x . wGate + biasGate) * (x . wUp + biasUp), elementwise product of two Dense
+ * layers over the same input (Dense, Sources/SwiftRTLayers/Dense.swift:21-71, has one), everything behind the two dot
+ * products in fp32 with one final rounding.
+ * x [M x K], wGate and wUp [K x H], out [M x H], biases [H] (each may be NULL); one element type, rank 2, any
+ * strides (a transposed weight is its descriptor's strides).  gate and up [M x H] (both or neither) receive
+ * x . wGate + biasGate and x . wUp + biasUp, rounded once each: what srtMatmulGatedBackward needs.  All activations
+ * but clippedRelu and elu; K = 0 is a sum of no terms.  `out`, gate and up must not overlap anything.
+ * Float16 / BFloat16 views with 16-byte aligned rows run as one launch in which neither product reaches memory.
+ * Others (Float32 among them) run as two products and an elementwise pass over gate and up, which are rounded to the
+ * element type in between; without gate and up that returns cudaErrorNotSupported. */
+cudaError_t srtMatmulGated(
+    const void* x, const srtTensorDescriptor* xDesc,
+    const void* wGate, const srtTensorDescriptor* wGateDesc,
+    const void* wUp, const srtTensorDescriptor* wUpDesc,
+    const void* biasGate, const srtTensorDescriptor* biasGateDesc,
+    const void* biasUp, const srtTensorDescriptor* biasUpDesc,
+    srtActivationType activation,
+    void* gate, const srtTensorDescriptor* gateDesc,
+    void* up, const srtTensorDescriptor* upDesc,
+    void* out, const srtTensorDescriptor* outDesc,
+    cudaStream_t stream);
+
+/* Gradients of srtMatmulGated from gate and up as it left them:
+ *     dGate = outGrad * up * activation'(gate),   dUp = outGrad * activation(gate)          (one rounding each)
+ *     dX = dGate . wGate^T + dUp . wUp^T,   dWGate = x^T . dGate,   dWUp = x^T . dUp
+ *     dBiasGate, dBiasUp = column sums of dGate and dUp (fp32 sums of the unrounded values)
+ * dGate and dUp [M x H] are always written: the products read them, rounded as they are.  dX, dWGate, dWUp, dBiasGate and dBiasUp may be NULL
+ * when not wanted.  dX2 [M x K] is scratch for one of dX's two products and may be NULL where dX is one launch
+ * (Float16 / BFloat16 views with 16-byte aligned rows); where it is needed and NULL the call returns
+ * cudaErrorNotSupported before it launches anything.  With it each of the two products is rounded before their sum is.  Results do not depend on timing.  M, K and H are at least 1.
+ * The weight products may use the library's per-(device, stream) workspace, as srtMatmul does. */
+cudaError_t srtMatmulGatedBackward(
+    const void* outGrad, const srtTensorDescriptor* outGradDesc,
+    const void* x, const srtTensorDescriptor* xDesc,
+    const void* wGate, const srtTensorDescriptor* wGateDesc,
+    const void* wUp, const srtTensorDescriptor* wUpDesc,
+    const void* gate, const srtTensorDescriptor* gateDesc,
+    const void* up, const srtTensorDescriptor* upDesc,
+    srtActivationType activation,
+    void* dGate, const srtTensorDescriptor* dGateDesc,
+    void* dUp, const srtTensorDescriptor* dUpDesc,
+    void* dX, const srtTensorDescriptor* dXDesc,
+    void* dX2, const srtTensorDescriptor* dX2Desc,
+    void* dWGate, const srtTensorDescriptor* dWGateDesc,
+    void* dWUp, const srtTensorDescriptor* dWUpDesc,
+    void* dBiasGate, const srtTensorDescriptor* dBiasGateDesc,
+    void* dBiasUp, const srtTensorDescriptor* dBiasUpDesc,
     cudaStream_t stream);
 
 /* ---------------------------------------------------------------------------------------

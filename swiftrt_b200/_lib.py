@@ -45,7 +45,7 @@ EXPORTS = ["srtMatmul", "srtMatmulBiasActivation", "srtMatmulQueryPlan", "srtMat
            "srtActivationForward", "srtMatmulReleaseWorkspaces", "srtGruCell", "srtShardRange", "srtMatmulSharded",
            "srtMatmulShardedDevices", "srtMatmulSetWaitLimit", "srtLstmCellFused", "srtLstmInterleaveGates", "srtPeerSignal", "srtPeerWait", "srtMulticastAlloc", "srtMulticastFree",
            "srtMatrixTransform", "srtMatrixLayoutLeadingDimension", "srtMatrixLayoutElementCount",
-           "srtGatedRecurrence", "srtGatedRecurrenceBackward"]
+           "srtGatedRecurrence", "srtGatedRecurrenceBackward", "srtMatmulGated", "srtMatmulGatedBackward"]
 
 if not os.path.exists(SO):
     raise ImportError(
@@ -165,6 +165,10 @@ lib.srtGatedRecurrence.restype = ctypes.c_int
 lib.srtGatedRecurrence.argtypes = [_P] * 18
 lib.srtGatedRecurrenceBackward.restype = ctypes.c_int
 lib.srtGatedRecurrenceBackward.argtypes = [_P] * 26
+lib.srtMatmulGated.restype = ctypes.c_int
+lib.srtMatmulGated.argtypes = [_P] * 10 + [ctypes.c_int] + [_P] * 7
+lib.srtMatmulGatedBackward.restype = ctypes.c_int
+lib.srtMatmulGatedBackward.argtypes = [_P] * 12 + [ctypes.c_int] + [_P] * 17
 
 
 def last_error() -> str:

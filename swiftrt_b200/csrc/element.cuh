@@ -8,7 +8,7 @@
 
 namespace srt {
 
-enum : uint32_t { kActSigmoid = 0, kActRelu = 1, kActTanh = 2, kActIdentity = 5, kActGelu = 6, kActGeluTanh = 7 };
+enum : uint32_t { kActSigmoid = 0, kActRelu = 1, kActTanh = 2, kActIdentity = 5, kActGelu = 6, kActGeluTanh = 7, kActSilu = 8 };
 
 __device__ __forceinline__ float apply_activation(uint32_t act, float x)
 {
@@ -21,6 +21,7 @@ __device__ __forceinline__ float apply_activation(uint32_t act, float x)
         float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
         return 0.5f * x * (1.0f + tanhf(u));
     }
+    case kActSilu: return x / (1.0f + expf(-x));
     default: return x;
     }
 }
@@ -45,6 +46,66 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
 {
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// The activation of a gate.  For results of 16 bits the logistic function is exp and a division of a few units of
+// 2^-23 each (three to eight bits below the result's rounding); Float32 takes the exact forms above.
+template <typename T> __device__ __forceinline__ float gate_activation(uint32_t act, float x)
+{
+    if constexpr (sizeof(T) == 2) {
+        switch (act) {
+        case kActSigmoid: return __fdividef(1.0f, 1.0f + __expf(-x));
+        case kActSilu: return x > -80.0f ? __fdividef(x, 1.0f + __expf(-x)) : apply_activation(kActSilu, x);
+        default: break;
+        }
+    }
+    return apply_activation(act, x);
+}
+
+// its slope at the pre-activation value x
+template <typename T> __device__ __forceinline__ float gate_slope(uint32_t act, float x)
+{
+    switch (act) {
+    case kActRelu: return x > 0.0f ? 1.0f : 0.0f;
+    case kActSigmoid: {
+        const float s = gate_activation<T>(kActSigmoid, x);
+        return s * gate_activation<T>(kActSigmoid, -x);
+    }
+    case kActTanh: {
+        const float t = tanhf(x);
+        return 1.0f - t * t;
+    }
+    case kActSilu: {
+        const float s = gate_activation<T>(kActSigmoid, x);
+        return s * (1.0f + x * gate_activation<T>(kActSigmoid, -x));
+    }
+    case kActGelu:
+        return 0.5f * (1.0f + erff(x * 0.70710678118654752440f)) + x * 0.39894228040143267794f * expf(-0.5f * x * x);
+    case kActGeluTanh: {
+        const float t = tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x));
+        return 0.5f * (1.0f + t) + 0.5f * x * (1.0f - t * t) * 0.7978845608028654f * (1.0f + 3.0f * 0.044715f * x * x);
+    }
+    default: return 1.0f;
+    }
+}
+
+// 32 values of one accumulator row; the selector is uniform, so the switch is taken once
+template <typename T> __device__ __forceinline__ void gate_chunk(uint32_t act, float (&v)[32])
+{
+    switch (act) {
+#define SRT_GATE_CASE(A)                                                        \
+    case A:                                                                     \
+        _Pragma("unroll") for (int j = 0; j < 32; ++j) v[j] = gate_activation<T>(A, v[j]); \
+        break
+    SRT_GATE_CASE(kActSilu);
+    SRT_GATE_CASE(kActGelu);
+    SRT_GATE_CASE(kActGeluTanh);
+    SRT_GATE_CASE(kActRelu);
+    SRT_GATE_CASE(kActSigmoid);
+    SRT_GATE_CASE(kActTanh);
+#undef SRT_GATE_CASE
+    default: break;
+    }
 }
 
 }  // namespace srt

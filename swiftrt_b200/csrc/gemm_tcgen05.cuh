@@ -248,6 +248,26 @@ struct NoPeers { uint32_t unused; };
 template <bool GATHER> struct PeerArgOf { using type = NoPeers; };
 template <> struct PeerArgOf<true> { using type = PeerMaps; };
 
+// What one launch of the pair kernel computes.
+//   kPairProduct  op(a) . op(b)
+//   kPairGated    act(a . b + bias) * (a . b2 + bias2): a tile's 256 accumulator columns are the same 128 output
+//                 columns of both products, CTA 0 staging them from b and CTA 1 from b2
+//   kPairSum      a . b + a2 . b2: the reduction runs through the first pair of operands and then through the second
+enum : int { kPairProduct = 0, kPairGated = 1, kPairSum = 2 };
+struct GatedArgs {
+    CUtensorMap b2, gate, up;            // second weight; kept pre-activations (with `keep`)
+    const void* bias2;
+    long long bias2_stride;
+    uint32_t has_bias2, keep;
+};
+struct SumArgs {
+    CUtensorMap a2, b2;
+    uint32_t k_blocks1;                  // k-blocks of the first pair; p.k_blocks counts both
+};
+template <bool GATHER, int MODE> struct PairArgOf { using type = typename PeerArgOf<GATHER>::type; };
+template <> struct PairArgOf<false, kPairGated> { using type = GatedArgs; };
+template <> struct PairArgOf<false, kPairSum> { using type = SumArgs; };
+
 // `rehearsal` (drain_accumulator): run the whole epilogue once on whatever an idle accumulator buffer holds, with
 // every store left out.  The epilogue warps have nothing to do while the first tile is reduced, and the first
 // execution of the epilogue on an SM otherwise waits for its instructions to arrive (about 4000 cycles on the first
@@ -397,6 +417,75 @@ __device__ __forceinline__ void drain_accumulator(const GemmParams& p, const CUt
         // the next box's bias values move to the front (static indices: the array stays in registers)
 #pragma unroll
         for (uint32_t c = 0; c + kLoadsPerBox < TileBias<T, BN, PARTS>::kChunks; ++c) tb.col[c] = tb.col[c + kLoadsPerBox];
+    }
+}
+
+// One 128-byte wide segment of this warp's 32 rows (packed[]: this thread's row) through the staging buffer to a
+// tensor map: the store path of drain_accumulator, for the epilogues with several outputs.
+__device__ __forceinline__ void stage_segment(const CUtensorMap* map, uint32_t staging, uint32_t lane, const uint32_t (&packed)[32], uint32_t col,
+                                              uint32_t row, uint32_t rehearsal)
+{
+    if (lane == 0) bulk_wait_group_read<0>();
+    __syncwarp();
+#pragma unroll
+    for (uint32_t q = 0; q < 8; ++q) {
+        const uint32_t addr = staging + lane * 128 + ((q ^ (lane & 7)) << 4);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};"
+                     ::"r"(addr), "r"(packed[4 * q]), "r"(packed[4 * q + 1]), "r"(packed[4 * q + 2]), "r"(packed[4 * q + 3]) : "memory");
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && !rehearsal) {
+        tma_store_3d(map, staging, static_cast<int32_t>(col), static_cast<int32_t>(row), 0);
+        bulk_commit_group();
+    }
+}
+
+// Epilogue of kPairGated: accumulator columns [0, 128) are the gate's pre-activations of output columns n0 .. n0 + 127,
+// columns [128, 256) the other product's.  Warp `part` (0, 1) of a lane quarter drains 64 output columns:
+// y = act(g + bias) * (u + bias2) in fp32, rounded once; with `keep` g + bias and u + bias2 are stored too (each
+// rounded once, read again from TMEM: holding all three segments in registers would spill).
+template <typename T>
+__device__ __forceinline__ void drain_accumulator_gated(const GemmParams& p, const GatedArgs& x, const CUtensorMap* tmap_out, uint32_t staging,
+                                                        uint32_t part, uint32_t acc, uint32_t quarter, uint32_t lane, uint32_t m0, uint32_t n0,
+                                                        const float (&bias_g)[2], const float (&bias_u)[2], uint32_t rehearsal)
+{
+    const uint32_t col = n0 + part * 64;
+    if (col >= p.N) return;                                     // uniform over the warp
+    const uint32_t src = acc + ((quarter * 32u) << 16) + part * 64;
+    uint32_t packed[32];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        uint32_t g[32], u[32];
+        tmem_ld_32x32(src + h * 32, g);
+        tmem_ld_32x32(src + 128 + h * 32, u);
+        tmem_ld_wait_regs2(g, u);
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(g[j]) + __shfl_sync(0xffffffffu, bias_g[h], j);
+        gate_chunk<T>(p.act, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= __uint_as_float(u[j]) + __shfl_sync(0xffffffffu, bias_u[h], j);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) packed[h * 16 + j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+    }
+    stage_segment(tmap_out, staging, lane, packed, col, m0 + quarter * 32, rehearsal);
+    if (!x.keep) return;
+#pragma unroll
+    for (uint32_t which = 0; which < 2; ++which) {
+        uint32_t a[32], b[32];
+        tmem_ld_32x32(src + which * 128, a);
+        tmem_ld_32x32(src + which * 128 + 32, b);
+        tmem_ld_wait_regs2(a, b);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float* bias = which ? bias_u : bias_g;
+            packed[j] = pack2<T>(__uint_as_float(a[2 * j]) + __shfl_sync(0xffffffffu, bias[0], 2 * j),
+                                 __uint_as_float(a[2 * j + 1]) + __shfl_sync(0xffffffffu, bias[0], 2 * j + 1));
+            packed[16 + j] = pack2<T>(__uint_as_float(b[2 * j]) + __shfl_sync(0xffffffffu, bias[1], 2 * j),
+                                      __uint_as_float(b[2 * j + 1]) + __shfl_sync(0xffffffffu, bias[1], 2 * j + 1));
+        }
+        stage_segment(which ? &x.up : &x.gate, staging, lane, packed, col, m0 + quarter * 32, rehearsal);
     }
 }
 
@@ -700,14 +789,16 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
 //
 // GATHER: the epilogue also stores every tile into the peers' output buffers (product followed
 // by an all-gather of the shards, in one kernel; see drain_accumulator).
-template <typename T, uint32_t BN, bool GATHER = false>
+// MODE: see kPairProduct.
+template <typename T, uint32_t BN, bool GATHER = false, int MODE = kPairProduct>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                          const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_out,
                          const __grid_constant__ GemmParams p,
-                         const __grid_constant__ typename PeerArgOf<GATHER>::type peer_maps)
+                         const __grid_constant__ typename PairArgOf<GATHER, MODE>::type peer_maps)
 {
+    static_assert(MODE != kPairGated || BN == 256, "a gated tile is 128 columns of either product");
     constexpr uint32_t kBHalf = BN / 2;
     constexpr uint32_t kBTileBytes = kBHalf * kRowBytes;
     constexpr uint32_t kStageBytes = kATileBytes + kBTileBytes;
@@ -767,28 +858,49 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
         st_shared_remote_u32(smem_u32(const_cast<uint32_t*>(&abort_flag)), cta_rank ^ 1u, 1u);
         atomicOr(&g_gemm_status, code);
     };
+    // the operands a k-block comes from: tensor maps, k coordinate and this CTA's first row or column of B
+    auto operands = [&](uint32_t kb, uint32_t tile_n0, const CUtensorMap*& ta, const CUtensorMap*& tb, int32_t& k0, uint32_t& n0) {
+        ta = &tmap_a;
+        tb = &tmap_b;
+        n0 = tile_n0 + cta_rank * kBHalf;
+        if constexpr (MODE == kPairGated) {
+            n0 = tile_n0 >> 1;
+            if (cta_rank) tb = &peer_maps.b2;
+        }
+        if constexpr (MODE == kPairSum) {
+            if (kb >= peer_maps.k_blocks1) {
+                kb -= peer_maps.k_blocks1;
+                ta = &peer_maps.a2;
+                tb = &peer_maps.b2;
+            }
+        }
+        k0 = static_cast<int32_t>(kb * p.kb_elems);
+    };
     // the loads of this CTA for k-block iteration j of the pair's work list (every tile has p.k_blocks of them:
     // pair tiles are never split along K); CTA 0 arms the stage's barrier for both CTAs
     auto issue_loads = [&](uint32_t j) {
         const uint32_t t_local = j / p.k_blocks, kb = j - t_local * p.k_blocks, stage = j % stages;
         const TileCoord tc = decode_tile(p, pair_id + t_local * num_pairs, BN);
-        const uint32_t m0 = tc.m0 * 2 + cta_rank * kTileM, n0 = tc.n0 + cta_rank * kBHalf, batch = tc.batch;
+        const uint32_t m0 = tc.m0 * 2 + cta_rank * kTileM, batch = tc.batch;
+        const CUtensorMap *ta, *tb;
+        int32_t k0;
+        uint32_t n0;
+        operands(kb, tc.n0, ta, tb, k0, n0);
         const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
         const uint32_t sa = smem_base + stage * kStageBytes;
         const uint32_t sb = sa + kATileBytes;
-        const int32_t k0 = static_cast<int32_t>(kb * p.kb_elems);
         if (cta_rank == 0) mbar_arrive_expect_tx(smem_u32(&full_bar[stage]), 2 * p.stage_tx_bytes);
         if (!p.a.mn_major) {
-            tma_load_3d_pair(sa, &tmap_a, bar, k0, m0, batch * p.a.batch_mul);
+            tma_load_3d_pair(sa, ta, bar, k0, m0, batch * p.a.batch_mul);
         } else {
             for (uint32_t c = 0; c < p.a.chunks; ++c)
-                tma_load_3d_pair(sa + c * p.a.chunk_bytes, &tmap_a, bar, m0 + c * p.a.chunk_elems, k0, batch * p.a.batch_mul);
+                tma_load_3d_pair(sa + c * p.a.chunk_bytes, ta, bar, m0 + c * p.a.chunk_elems, k0, batch * p.a.batch_mul);
         }
         if (!p.b.mn_major) {
-            tma_load_3d_pair(sb, &tmap_b, bar, k0, n0, batch * p.b.batch_mul);
+            tma_load_3d_pair(sb, tb, bar, k0, n0, batch * p.b.batch_mul);
         } else {
             for (uint32_t c = 0; c < p.b.chunks; ++c)
-                tma_load_3d_pair(sb + c * p.b.chunk_bytes, &tmap_b, bar, n0 + c * p.b.chunk_elems, k0, batch * p.b.batch_mul);
+                tma_load_3d_pair(sb + c * p.b.chunk_bytes, tb, bar, n0 + c * p.b.chunk_elems, k0, batch * p.b.batch_mul);
         }
     };
 
@@ -799,29 +911,31 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
             bool ok = true;
             for (uint32_t tile = pair_id; ok && tile < p.num_tiles; tile += num_pairs) {
                 const TileCoord tc = decode_tile(p, tile, BN);
-                uint32_t batch = tc.batch, m0 = tc.m0, n0 = tc.n0;
+                uint32_t batch = tc.batch, m0 = tc.m0;
                 m0 = m0 * 2 + cta_rank * kTileM;            // decode_tile counts 128-row units; pair tiles are 256 rows
-                n0 += cta_rank * kBHalf;
                 for (uint32_t kb = tc.kb0; kb < tc.kb1; ++kb) {
                     if (!mbar_wait_cluster(smem_u32(&empty_bar[stage]), phase ^ 1, &abort_flag, p.wait_cycles)) { ok = false; break; }
                     // every load of the pair reports to the leader's barrier
                     const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
                     const uint32_t sa = smem_base + stage * kStageBytes;
                     const uint32_t sb = sa + kATileBytes;
-                    const int32_t k0 = static_cast<int32_t>(kb * p.kb_elems);
+                    const CUtensorMap *ta, *tb;
+                    int32_t k0;
+                    uint32_t n0;
+                    operands(kb, tc.n0, ta, tb, k0, n0);
                     if (cta_rank == 0) mbar_arrive_expect_tx(smem_u32(&full_bar[stage]), 2 * p.stage_tx_bytes);
                     if (!p.a.mn_major) {
-                        tma_load_3d_pair(sa, &tmap_a, bar, k0, m0, batch * p.a.batch_mul);
+                        tma_load_3d_pair(sa, ta, bar, k0, m0, batch * p.a.batch_mul);
                     } else {
                         for (uint32_t c = 0; c < p.a.chunks; ++c)
-                            tma_load_3d_pair(sa + c * p.a.chunk_bytes, &tmap_a, bar, m0 + c * p.a.chunk_elems, k0,
+                            tma_load_3d_pair(sa + c * p.a.chunk_bytes, ta, bar, m0 + c * p.a.chunk_elems, k0,
                                              batch * p.a.batch_mul);
                     }
                     if (!p.b.mn_major) {
-                        tma_load_3d_pair(sb, &tmap_b, bar, k0, n0, batch * p.b.batch_mul);
+                        tma_load_3d_pair(sb, tb, bar, k0, n0, batch * p.b.batch_mul);
                     } else {
                         for (uint32_t c = 0; c < p.b.chunks; ++c)
-                            tma_load_3d_pair(sb + c * p.b.chunk_bytes, &tmap_b, bar, n0 + c * p.b.chunk_elems, k0,
+                            tma_load_3d_pair(sb + c * p.b.chunk_bytes, tb, bar, n0 + c * p.b.chunk_elems, k0,
                                              batch * p.b.batch_mul);
                     }
                     ++issued;
@@ -880,12 +994,25 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
             const uint32_t buf = rehearsal ? 1u : (local & 1);
             const uint32_t acc_phase = (local >> 1) & 1;
             TileBias<T, BN, 2> tile_bias = {};
+            float bias_g[2] = {0.0f, 0.0f}, bias_u[2] = {0.0f, 0.0f};
             if (!rehearsal) {
-                load_tile_bias<T, BN, 2>(p, (warp - 2) >> 2, quarter, lane, m0, n0, tile_bias);      // under the reduction
+                if constexpr (MODE == kPairGated) {
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        const uint32_t col = (n0 >> 1) + ((warp - 2) >> 2) * 64 + h * 32 + lane;
+                        if (p.bias_mode && col < p.N) bias_g[h] = to_float<T>(__ldg(static_cast<const T*>(p.bias) + col * p.bias_stride));
+                        if (peer_maps.has_bias2 && col < p.N) bias_u[h] = to_float<T>(__ldg(static_cast<const T*>(peer_maps.bias2) + col * peer_maps.bias2_stride));
+                    }
+                } else {
+                    load_tile_bias<T, BN, 2>(p, (warp - 2) >> 2, quarter, lane, m0, n0, tile_bias);  // under the reduction
+                }
                 if (!mbar_wait_cluster(smem_u32(&tmem_full_bar[buf]), acc_phase, &abort_flag, p.wait_cycles)) { ok = false; break; }
                 tc_fence_after_sync();
             }
-            if constexpr (GATHER)
+            if constexpr (MODE == kPairGated)
+                drain_accumulator_gated<T>(p, peer_maps, &tmap_out, smem_base + stages * kStageBytes + (warp - 2) * 4096, (warp - 2) >> 2,
+                                           tmem_base + buf * BN, quarter, lane, m0, n0 >> 1, bias_g, bias_u, rehearsal);
+            else if constexpr (GATHER)
                 drain_accumulator<T, BN, false, 2, true>(p, &tmap_out, smem_base + stages * kStageBytes + (warp - 2) * 4096,
                                                          (warp - 2) >> 2, tmem_base + buf * BN, quarter, lane, batch, m0, n0,
                                                          tile_bias, 0, &peer_maps);

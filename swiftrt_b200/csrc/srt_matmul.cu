@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "dense_backward.cuh"
+#include "gated_dense.cuh"
 #include "gemm_simt.cuh"
 #include "gemm_splitk.cuh"
 #include "gemm_tcgen05.cuh"
@@ -130,6 +131,8 @@ cudaError_t parse(const void* a, const srtTensorDescriptor* ad, bool ta,
         break;
     case srtActivationClippedRelu: case srtActivationElu:
         return fail(cudaErrorNotSupported, "clippedRelu and elu need coefficients that this entry point does not carry");
+    case srtActivationSilu:
+        return fail(cudaErrorNotSupported, "silu is an activation of the gated and 4-bit products only");
     default:
         return fail(cudaErrorInvalidValue, "unknown activation %d", act);
     }
@@ -649,11 +652,11 @@ cudaError_t launch_split(const CUtensorMap& ma, const CUtensorMap& mb, const CUt
     return cudaGetLastError();
 }
 
-template <typename T, uint32_t BN, bool GATHER = false>
+template <typename T, uint32_t BN, bool GATHER = false, int MODE = kPairProduct>
 cudaError_t launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const GemmParams& gp, uint32_t ctas, size_t smem,
-                        cudaStream_t stream, const typename PeerArgOf<GATHER>::type& peers = typename PeerArgOf<GATHER>::type())
+                        cudaStream_t stream, const typename PairArgOf<GATHER, MODE>::type& peers = typename PairArgOf<GATHER, MODE>::type())
 {
-    auto kernel = gemm_tcgen05_pair_kernel<T, BN, GATHER>;
+    auto kernel = gemm_tcgen05_pair_kernel<T, BN, GATHER, MODE>;
     static std::atomic<uint64_t> attr_done{0};
     static std::atomic<int> cluster_cache[64];           // max co-resident pairs per device, 0 = unknown
     cudaError_t e = ensure_smem_attr(kernel, attr_done, smem);
@@ -1575,6 +1578,219 @@ cudaError_t run_matmul(const void* a, const srtTensorDescriptor* aDesc, bool tra
     return e;
 }
 
+// ------------------------------------------------------------------ srtMatmulGated, srtMatmulGatedBackward: helpers
+
+struct Matrix { const char* p; uint64_t rows, cols; long long m, n; };          // element strides
+
+cudaError_t gated_matrix(const char* op, const char* what, const void* ptr, const srtTensorDescriptor* d, srtDataType type, bool written, Matrix& v)
+{
+    if (!d || !d->shape || !d->strides) return fail(cudaErrorInvalidValue, "%s: %s: missing descriptor", op, what);
+    if (d->rank != 2) return fail(cudaErrorInvalidValue, "%s: %s must have rank 2", op, what);
+    if (d->type != type) return fail(cudaErrorInvalidValue, "%s: %s must have the element type of x", op, what);
+    v = Matrix{static_cast<const char*>(ptr), d->shape[0], d->shape[1], (long long)d->strides[0], (long long)d->strides[1]};
+    if (!ptr && v.rows * v.cols != 0) return fail(cudaErrorInvalidValue, "%s: %s is null", op, what);
+    if (v.rows > 0x7fffffffull || v.cols > 0x7fffffffull) return fail(cudaErrorInvalidValue, "%s: dimension exceeds the supported range", op);
+    if (written && ((v.rows > 1 && v.m == 0) || (v.cols > 1 && v.n == 0)))
+        return fail(cudaErrorInvalidValue, "%s: %s must not repeat elements (zero stride)", op, what);
+    return cudaSuccess;
+}
+
+cudaError_t gated_extent(const char* op, const char* what, const Matrix& v, uint64_t rows, uint64_t cols)
+{
+    if (v.rows == rows && v.cols == cols) return cudaSuccess;
+    return fail(cudaErrorInvalidValue, "%s: %s must be [%llu x %llu], got [%llu x %llu]", op, what, (unsigned long long)rows,
+                (unsigned long long)cols, (unsigned long long)v.rows, (unsigned long long)v.cols);
+}
+
+cudaError_t gated_vector(const char* op, const char* what, const srtTensorDescriptor* d, srtDataType type, uint64_t n, bool written, long long& stride)
+{
+    if (!d || !d->shape || !d->strides || d->rank != 1 || d->shape[0] != n || d->type != type)
+        return fail(cudaErrorInvalidValue, "%s: %s must be rank 1 with %llu elements of x's type", op, what, (unsigned long long)n);
+    stride = (long long)d->strides[0];
+    if (written && n > 1 && stride == 0) return fail(cudaErrorInvalidValue, "%s: %s must not repeat elements (zero stride)", op, what);
+    return cudaSuccess;
+}
+
+cudaError_t gated_activation(const char* op, int act)
+{
+    switch (act) {
+    case srtActivationSigmoid: case srtActivationRelu: case srtActivationTanh: case srtActivationIdentity:
+    case srtActivationGelu: case srtActivationGeluTanh: case srtActivationSilu: return cudaSuccess;
+    case srtActivationClippedRelu: case srtActivationElu:
+        return fail(cudaErrorNotSupported, "%s: clippedRelu and elu need coefficients that this entry point does not carry", op);
+    default: return fail(cudaErrorInvalidValue, "%s: unknown activation %d", op, act);
+    }
+}
+
+cudaError_t gated_type(const char* op, const srtTensorDescriptor* xDesc)
+{
+    if (!xDesc) return fail(cudaErrorInvalidValue, "%s: x: missing descriptor", op);
+    if (elem_size(xDesc->type) == 0) return fail(cudaErrorNotSupported, "%s: element type %d is not computed by this library", op, (int)xDesc->type);
+    return cudaSuccess;
+}
+
+// The descriptor of a Matrix (or of its transpose) for a call of another entry point of this library.
+struct LocalDescriptor {
+    size_t shape[2], strides[2];
+    srtTensorDescriptor d;
+    LocalDescriptor(const Matrix& v, srtDataType type, bool transposed = false)
+    {
+        shape[0] = transposed ? v.cols : v.rows; shape[1] = transposed ? v.rows : v.cols;
+        strides[0] = (size_t)(transposed ? v.n : v.m); strides[1] = (size_t)(transposed ? v.m : v.n);
+        memset(&d, 0, sizeof d);
+        d.type = type; d.rank = 2; d.order = srtOrderRow;
+        d.count = d.spanCount = shape[0] * shape[1];
+        d.shape = shape; d.strides = strides; d.logicalStrides = strides;
+    }
+    LocalDescriptor(const LocalDescriptor&) = delete;
+};
+
+bool rows_ok_for_tma(const Matrix& v, uint32_t elem)        // row-contiguous, 16-byte aligned rows
+{
+    return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && (v.n == 1 || v.cols == 1) && (v.m * (long long)elem) % 16 == 0 &&
+           (v.rows == 1 || v.m >= (long long)v.cols);
+}
+
+// Prepares the pair kernel for a [M x N] result whose operands are a (rows M) and b (rows N), both over K; the caller adds the
+// second operands.  `cols_per_tile`: output columns of a tile (128 for kPairGated).  False: not a product for this kernel.
+bool prepare_pair(srtDataType type, const Matrix& a, const Matrix& b, uint64_t K, const Matrix& out, uint32_t bn, uint32_t cols_per_tile, uint32_t k_blocks,
+                  const DeviceInfo& dev, Problem& Q, TcOperand& ta, TcOperand& tb, Prepared& pr)
+{
+    memset(&Q, 0, sizeof Q);
+    Q.type = type; Q.elem = 2; Q.batch = 1;
+    Q.M = out.rows; Q.N = out.cols; Q.K = K;
+    Q.a = a.p; Q.a_m = a.m; Q.a_k = a.n;
+    Q.b = b.p; Q.b_n = b.m; Q.b_k = b.n;
+    Q.out = const_cast<char*>(out.p); Q.o_m = out.m; Q.o_n = out.n;
+    Q.act = kActIdentity;
+    if (!rows_ok_for_tma(out, 2) || Q.N < 2) return false;
+    ta = classify(Q.a, Q.M, K, 1, Q.a_m, Q.a_k, 0, 2);
+    tb = classify(Q.b, Q.N, K, 1, Q.b_n, Q.b_k, 0, 2);
+    if (!ta.ok || !tb.ok) return false;
+    GemmParams& gp = pr.gp;
+    memset(&gp, 0, sizeof gp);
+    if (encode_operand(&pr.ma, Q, Q.a, ta, Q.M, 0, kTileM, gp.a) != cudaSuccess || encode_operand(&pr.mb, Q, Q.b, tb, Q.N, 0, bn / 2, gp.b) != cudaSuccess)
+        return false;
+    gp.ldo = Q.M == 1 ? (long long)((Q.N + 7) / 8 * 8) : Q.o_m;
+    if (!encode_out_map(&pr.mo, Q, gp.ldo, Q.out)) return false;
+    gp.out_tma = gp.out_vec_ok = 1;
+    gp.M = (uint32_t)Q.M; gp.N = (uint32_t)Q.N; gp.K = (uint32_t)K; gp.batch = 1;
+    gp.tiles_m = (uint32_t)((Q.M + 2 * kTileM - 1) / (2 * kTileM));
+    gp.tiles_n = (uint32_t)((Q.N + cols_per_tile - 1) / cols_per_tile);
+    gp.tiles_per_batch = gp.tiles_total = gp.num_tiles = gp.tiles_m * gp.tiles_n;
+    gp.k_splits = 1;
+    gp.kb_elems = kRowBytes / 2;
+    gp.k_blocks = gp.kb_per_split = k_blocks;
+    gp.group_m = 8;
+    set_tile_walk(gp);
+    const uint32_t pairs = (uint32_t)dev.sms / 2;
+    gp.stages = gp.num_tiles <= pairs ? 6 : 4;              // as the planner chooses for the plain product
+    if (bn == 128) gp.stages = 6;
+    gp.stage_tx_bytes = kATileBytes + bn / 2 * kRowBytes;
+    const uint32_t fmt = type == real16F ? 0u : 1u;
+    gp.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)ta.mn_major << 15) | ((uint32_t)tb.mn_major << 16) | ((bn >> 3) << 17) |
+               ((2 * kTileM >> 4) << 24);
+    gp.out = Q.out;
+    gp.act = kActIdentity;
+    gp.wait_cycles = g_wait_limit_ns.load(std::memory_order_relaxed) * 2;
+    pr.smem = (size_t)gp.stages * gp.stage_tx_bytes + kEpilogueStagingBytes + 1024;
+    pr.ctas = 2 * (gp.num_tiles < pairs ? gp.num_tiles : pairs);
+    return true;
+}
+
+// both projections, the activation and the product in one launch; cudaErrorNotSupported when the views do not suit
+cudaError_t gated_fused(srtDataType type, const Matrix& x, const Matrix& wg, const Matrix& wu, const void* bg, long long bg_n, const void* bu,
+                        long long bu_n, uint32_t act, const Matrix* gate, const Matrix* up, const Matrix& out, const DeviceInfo& dev, cudaStream_t stream)
+{
+    if (type == real32F) return cudaErrorNotSupported;
+    const Matrix wgt = {wg.p, wg.cols, wg.rows, wg.n, wg.m}, wut = {wu.p, wu.cols, wu.rows, wu.n, wu.m};
+    Problem Q;
+    TcOperand ta, tb;
+    std::unique_ptr<Prepared> pr(new Prepared());
+    if (!prepare_pair(type, x, wgt, x.cols, out, 256, 128, (uint32_t)((x.cols + 63) / 64), dev, Q, ta, tb, *pr)) return cudaErrorNotSupported;
+    GatedArgs ga;
+    memset(&ga, 0, sizeof ga);
+    const TcOperand t2 = classify(wut.p, Q.N, Q.K, 1, wut.m, wut.n, 0, 2);
+    OperandParams same;
+    if (!t2.ok || t2.mn_major != tb.mn_major || encode_operand(&ga.b2, Q, wut.p, t2, Q.N, 0, 128, same) != cudaSuccess) return cudaErrorNotSupported;
+    if (gate) {
+        const auto out_map = [&](const Matrix& v, CUtensorMap* map) {
+            return rows_ok_for_tma(v, 2) && encode_out_map(map, Q, Q.M == 1 ? pr->gp.ldo : v.m, const_cast<char*>(v.p));
+        };
+        if (!out_map(*gate, &ga.gate) || !out_map(*up, &ga.up)) return cudaErrorNotSupported;
+        ga.keep = 1;
+    }
+    pr->gp.act = act;
+    pr->gp.bias = bg; pr->gp.bias_stride = bg_n; pr->gp.bias_mode = bg ? 1 : 0;
+    ga.bias2 = bu; ga.bias2_stride = bu_n; ga.has_bias2 = bu ? 1 : 0;
+    const cudaError_t e = type == real16F
+        ? launch_pair<__half, 256, false, kPairGated>(pr->ma, pr->mb, pr->mo, pr->gp, pr->ctas, pr->smem, stream, ga)
+        : launch_pair<__nv_bfloat16, 256, false, kPairGated>(pr->ma, pr->mb, pr->mo, pr->gp, pr->ctas, pr->smem, stream, ga);
+    if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return e;
+}
+
+// out = a1 . b1^T + a2 . b2^T (a [M x K], b [N x K]) in one launch
+cudaError_t sum_fused(srtDataType type, const Matrix& a1, const Matrix& b1, const Matrix& a2, const Matrix& b2, const Matrix& out, const DeviceInfo& dev,
+                      cudaStream_t stream)
+{
+    if (type == real32F) return cudaErrorNotSupported;
+    const uint64_t K = a1.cols;
+    const uint32_t kb = (uint32_t)((K + 63) / 64);
+    const uint32_t bn = out.cols <= 128 ? 128 : 256;
+    Problem Q;
+    TcOperand ta, tb;
+    std::unique_ptr<Prepared> pr(new Prepared());
+    if (!prepare_pair(type, a1, b1, K, out, bn, bn, 2 * kb, dev, Q, ta, tb, *pr)) return cudaErrorNotSupported;
+    SumArgs sa;
+    memset(&sa, 0, sizeof sa);
+    sa.k_blocks1 = kb;
+    const TcOperand ta2 = classify(a2.p, Q.M, K, 1, a2.m, a2.n, 0, 2), tb2 = classify(b2.p, Q.N, K, 1, b2.m, b2.n, 0, 2);
+    OperandParams same;
+    if (!ta2.ok || !tb2.ok || ta2.mn_major != ta.mn_major || tb2.mn_major != tb.mn_major ||
+        encode_operand(&sa.a2, Q, a2.p, ta2, Q.M, 0, kTileM, same) != cudaSuccess || encode_operand(&sa.b2, Q, b2.p, tb2, Q.N, 0, bn / 2, same) != cudaSuccess)
+        return cudaErrorNotSupported;
+    cudaError_t e;
+    if (type == real16F)
+        e = bn == 128 ? launch_pair<__half, 128, false, kPairSum>(pr->ma, pr->mb, pr->mo, pr->gp, pr->ctas, pr->smem, stream, sa)
+                      : launch_pair<__half, 256, false, kPairSum>(pr->ma, pr->mb, pr->mo, pr->gp, pr->ctas, pr->smem, stream, sa);
+    else
+        e = bn == 128 ? launch_pair<__nv_bfloat16, 128, false, kPairSum>(pr->ma, pr->mb, pr->mo, pr->gp, pr->ctas, pr->smem, stream, sa)
+                      : launch_pair<__nv_bfloat16, 256, false, kPairSum>(pr->ma, pr->mb, pr->mo, pr->gp, pr->ctas, pr->smem, stream, sa);
+    if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return e;
+}
+
+template <typename T>
+cudaError_t launch_gate_backward(const GateBackwardParams& gp, bool vec, cudaStream_t stream)
+{
+    constexpr int kVec = 16 / sizeof(T);
+    const bool sums = gp.sum_g || gp.sum_u;
+    const unsigned col_blocks = (gp.N + 8 * (vec ? kVec : 1) - 1) / (8 * (vec ? kVec : 1)), row_groups = (gp.M + 31) / 32;
+    // with sums the CTAs of a column block are one cluster; without, as many row blocks as keep the device busy
+    unsigned rows = 1;
+    if (sums) while (rows < 8 && rows < row_groups) rows *= 2;
+    else {
+        rows = (148u * 8 + col_blocks - 1) / col_blocks;
+        if (rows > row_groups) rows = row_groups;
+    }
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3(col_blocks, rows, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = sums ? rows : 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = vec ? cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, kVec>, gp) : cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, 1>, gp);
+    if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return e;
+}
+
 }  // namespace
 
 // ===================================================================== exported entry points
@@ -2297,6 +2513,171 @@ cudaError_t srtLstmCellFused(const void* input, const srtTensorDescriptor* input
     gp.lstm_cell = cell; gp.lstm_new_cell = newCell; gp.lstm_new_hidden = newHidden;
     gp.lstm_c_m = c_m; gp.lstm_nc_m = nc_m; gp.lstm_nh_m = nh_m;
     return launch_prepared(*pr, stream);
+}
+
+// ------------------------------------------------------------------ srtMatmulGated, srtMatmulGatedBackward
+cudaError_t srtMatmulGated(const void* x, const srtTensorDescriptor* xDesc, const void* wGate, const srtTensorDescriptor* wGateDesc,
+                           const void* wUp, const srtTensorDescriptor* wUpDesc, const void* biasGate, const srtTensorDescriptor* biasGateDesc,
+                           const void* biasUp, const srtTensorDescriptor* biasUpDesc, srtActivationType activation, void* gate,
+                           const srtTensorDescriptor* gateDesc, void* up, const srtTensorDescriptor* upDesc, void* out,
+                           const srtTensorDescriptor* outDesc, cudaStream_t stream)
+{
+    const char* const op = "srtMatmulGated";
+    cudaError_t e = gated_type(op, xDesc);
+    if (e != cudaSuccess) return e;
+    const srtDataType type = xDesc->type;
+    Matrix mx, mg, mu, mo, kg, ku;
+    long long bg_n = 0, bu_n = 0;
+    if ((e = gated_matrix(op, "x", x, xDesc, type, false, mx)) != cudaSuccess || (e = gated_matrix(op, "wGate", wGate, wGateDesc, type, false, mg)) != cudaSuccess ||
+        (e = gated_matrix(op, "wUp", wUp, wUpDesc, type, false, mu)) != cudaSuccess || (e = gated_matrix(op, "out", out, outDesc, type, true, mo)) != cudaSuccess)
+        return e;
+    const uint64_t M = mx.rows, K = mx.cols, H = mg.cols;
+    if ((e = gated_extent(op, "wGate", mg, K, H)) != cudaSuccess || (e = gated_extent(op, "wUp", mu, K, H)) != cudaSuccess ||
+        (e = gated_extent(op, "out", mo, M, H)) != cudaSuccess)
+        return e;
+    if (biasGate && (e = gated_vector(op, "biasGate", biasGateDesc, type, H, false, bg_n)) != cudaSuccess) return e;
+    if (biasUp && (e = gated_vector(op, "biasUp", biasUpDesc, type, H, false, bu_n)) != cudaSuccess) return e;
+    if ((e = gated_activation(op, (int)activation)) != cudaSuccess) return e;
+    if ((gate == nullptr) != (up == nullptr)) return fail(cudaErrorInvalidValue, "%s: gate and up are both given or both null", op);
+    if (gate) {
+        if ((e = gated_matrix(op, "gate", gate, gateDesc, type, true, kg)) != cudaSuccess || (e = gated_matrix(op, "up", up, upDesc, type, true, ku)) != cudaSuccess ||
+            (e = gated_extent(op, "gate", kg, M, H)) != cudaSuccess || (e = gated_extent(op, "up", ku, M, H)) != cudaSuccess)
+            return e;
+    }
+    g_error[0] = 0;
+    if (M == 0 || H == 0) return cudaSuccess;
+    DeviceScope scope(stream);
+    if (scope.status != cudaSuccess) return scope.status;
+    DeviceInfo info;
+    if ((e = device_info(scope.device, info)) != cudaSuccess) return e;
+    if (!info.sm100) return fail(cudaErrorNotSupported, "this library is built for sm_100a devices only");
+    if (K > 0) {
+        e = gated_fused(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, info, stream);
+        if (e != cudaErrorNotSupported) return e;
+    }
+    // two products and an elementwise pass; the pre-activations need a place then
+    if (!gate)
+        return fail(cudaErrorNotSupported, "%s: these tensors (Float32, or views without 16-byte aligned rows) need gate and up to hold the two products", op);
+    e = srtMatmulBiasActivation(x, xDesc, false, wGate, wGateDesc, false, biasGate, biasGateDesc, srtActivationIdentity, gate, gateDesc, stream);
+    if (e != cudaSuccess) return e;
+    e = srtMatmulBiasActivation(x, xDesc, false, wUp, wUpDesc, false, biasUp, biasUpDesc, srtActivationIdentity, up, upDesc, stream);
+    if (e != cudaSuccess) return e;
+    GateForwardParams fp;
+    fp.g = View2{kg.p, kg.m, kg.n}; fp.u = View2{ku.p, ku.m, ku.n};
+    fp.y = View2W{out, mo.m, mo.n};
+    fp.M = (uint32_t)M; fp.N = (uint32_t)H; fp.act = (uint32_t)activation;
+    unsigned long long blocks = (M * H + 255) / 256;
+    if (blocks > 148ull * 16) blocks = 148ull * 16;
+    switch (type) {
+    case real32F: gate_forward_kernel<float><<<(unsigned)blocks, 256, 0, stream>>>(fp); break;
+    case real16F: gate_forward_kernel<__half><<<(unsigned)blocks, 256, 0, stream>>>(fp); break;
+    default: gate_forward_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, stream>>>(fp); break;
+    }
+    e = cudaGetLastError();
+    if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return e;
+}
+
+cudaError_t srtMatmulGatedBackward(const void* outGrad, const srtTensorDescriptor* outGradDesc, const void* x, const srtTensorDescriptor* xDesc,
+                                   const void* wGate, const srtTensorDescriptor* wGateDesc, const void* wUp, const srtTensorDescriptor* wUpDesc,
+                                   const void* gate, const srtTensorDescriptor* gateDesc, const void* up, const srtTensorDescriptor* upDesc,
+                                   srtActivationType activation, void* dGate, const srtTensorDescriptor* dGateDesc, void* dUp,
+                                   const srtTensorDescriptor* dUpDesc, void* dX, const srtTensorDescriptor* dXDesc, void* dX2,
+                                   const srtTensorDescriptor* dX2Desc, void* dWGate, const srtTensorDescriptor* dWGateDesc, void* dWUp,
+                                   const srtTensorDescriptor* dWUpDesc, void* dBiasGate, const srtTensorDescriptor* dBiasGateDesc, void* dBiasUp,
+                                   const srtTensorDescriptor* dBiasUpDesc, cudaStream_t stream)
+{
+    const char* const op = "srtMatmulGatedBackward";
+    cudaError_t e = gated_type(op, xDesc);
+    if (e != cudaSuccess) return e;
+    const srtDataType type = xDesc->type;
+    const uint32_t elem = elem_size(type);
+    Matrix my, mx, mg, mu, kg, ku, dg, du, dx, dx2, dwg, dwu;
+    if ((e = gated_matrix(op, "x", x, xDesc, type, false, mx)) != cudaSuccess || (e = gated_matrix(op, "wGate", wGate, wGateDesc, type, false, mg)) != cudaSuccess)
+        return e;
+    const uint64_t M = mx.rows, K = mx.cols, H = mg.cols;
+    struct Item { const char* name; const void* p; const srtTensorDescriptor* d; Matrix* m; uint64_t r, c; bool written, wanted; };
+    const Item items[] = {{"outGrad", outGrad, outGradDesc, &my, M, H, false, true}, {"wGate", wGate, wGateDesc, &mg, K, H, false, true},
+                          {"wUp", wUp, wUpDesc, &mu, K, H, false, true}, {"gate", gate, gateDesc, &kg, M, H, false, true},
+                          {"up", up, upDesc, &ku, M, H, false, true}, {"dGate", dGate, dGateDesc, &dg, M, H, true, true},
+                          {"dUp", dUp, dUpDesc, &du, M, H, true, true}, {"dX", dX, dXDesc, &dx, M, K, true, dX != nullptr},
+                          {"dX2", dX2, dX2Desc, &dx2, M, K, true, dX2 != nullptr}, {"dWGate", dWGate, dWGateDesc, &dwg, K, H, true, dWGate != nullptr},
+                          {"dWUp", dWUp, dWUpDesc, &dwu, K, H, true, dWUp != nullptr}};
+    for (const Item& i : items) {
+        if (!i.wanted) continue;
+        if ((e = gated_matrix(op, i.name, i.p, i.d, type, i.written, *i.m)) != cudaSuccess || (e = gated_extent(op, i.name, *i.m, i.r, i.c)) != cudaSuccess) return e;
+    }
+    long long sg_n = 0, su_n = 0;
+    if (dBiasGate && (e = gated_vector(op, "dBiasGate", dBiasGateDesc, type, H, true, sg_n)) != cudaSuccess) return e;
+    if (dBiasUp && (e = gated_vector(op, "dBiasUp", dBiasUpDesc, type, H, true, su_n)) != cudaSuccess) return e;
+    if ((e = gated_activation(op, (int)activation)) != cudaSuccess) return e;
+    if (M == 0 || H == 0 || K == 0) return fail(cudaErrorInvalidValue, "%s: tensors without elements have no gradients to compute", op);
+    g_error[0] = 0;
+    DeviceScope scope(stream);
+    if (scope.status != cudaSuccess) return scope.status;
+    DeviceInfo info;
+    if ((e = device_info(scope.device, info)) != cudaSuccess) return e;
+    if (!info.sm100) return fail(cudaErrorNotSupported, "this library is built for sm_100a devices only");
+
+    const Matrix wg = {mg.p, K, H, mg.m, mg.n}, wu = {mu.p, K, H, mu.m, mu.n};
+    // dX = dg . Wg^T + du . Wu^T in one launch when the views suit; else two products and their sum, which takes dX2
+    bool one_launch = false;
+    if (dX) {
+        Problem Q;
+        TcOperand ta, tb;
+        Prepared pr;
+        auto same = [&](const Matrix& p, const Matrix& q, uint64_t rows, uint64_t cols) {
+            const TcOperand s = classify(p.p, rows, cols, 1, p.m, p.n, 0, 2), t = classify(q.p, rows, cols, 1, q.m, q.n, 0, 2);
+            return s.ok && t.ok && s.mn_major == t.mn_major;
+        };
+        one_launch = type != real32F && same(dg, du, M, H) && same(wg, wu, K, H) && prepare_pair(type, dg, wg, H, dx, 256, 256, 1, info, Q, ta, tb, pr);
+        if (!one_launch && !dX2)
+            return fail(cudaErrorNotSupported, "%s: these tensors (Float32, or views without 16-byte aligned rows) need dX2, a second [M x K] tensor, to hold one of dX's two products", op);
+    }
+
+    GateBackwardParams gp;
+    memset(&gp, 0, sizeof gp);
+    gp.dy = View2{my.p, my.m, my.n}; gp.g = View2{kg.p, kg.m, kg.n}; gp.u = View2{ku.p, ku.m, ku.n};
+    gp.dg = View2W{dGate, dg.m, dg.n}; gp.du = View2W{dUp, du.m, du.n};
+    gp.sum_g = dBiasGate; gp.sum_g_n = sg_n; gp.sum_u = dBiasUp; gp.sum_u_n = su_n;
+    gp.M = (uint32_t)M; gp.N = (uint32_t)H; gp.act = (uint32_t)activation;
+    auto vec_ok = [&](const Matrix& v) {
+        return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && v.n == 1 && (v.m * (long long)elem) % 16 == 0;
+    };
+    const bool vec = H % (16 / elem) == 0 && vec_ok(my) && vec_ok(kg) && vec_ok(ku) && vec_ok(dg) && vec_ok(du);
+    e = type == real32F ? launch_gate_backward<float>(gp, vec, stream)
+        : type == real16F ? launch_gate_backward<__half>(gp, vec, stream) : launch_gate_backward<__nv_bfloat16>(gp, vec, stream);
+    if (e != cudaSuccess) return e;
+
+    if (dX && one_launch) {
+        if ((e = sum_fused(type, dg, wg, du, wu, dx, info, stream)) != cudaSuccess) return e;
+    } else if (dX) {
+        const LocalDescriptor d_out(dx, type), d_tmp(dx2, type), d_dg(dg, type), d_du(du, type), d_wg(mg, type), d_wu(mu, type);
+        if ((e = srtMatmul(dGate, &d_dg.d, false, wGate, &d_wg.d, true, dX, &d_out.d, stream)) != cudaSuccess) return e;
+        if ((e = srtMatmul(dUp, &d_du.d, false, wUp, &d_wu.d, true, dX2, &d_tmp.d, stream)) != cudaSuccess) return e;
+        GateForwardParams sp;
+        sp.g = View2{dx.p, dx.m, dx.n}; sp.u = View2{dx2.p, dx2.m, dx2.n}; sp.y = View2W{dX, dx.m, dx.n};
+        sp.M = (uint32_t)M; sp.N = (uint32_t)K; sp.act = kActIdentity;
+        unsigned long long blocks = (M * K + 255) / 256;
+        if (blocks > 148ull * 16) blocks = 148ull * 16;
+        switch (type) {
+        case real32F: add_kernel<float><<<(unsigned)blocks, 256, 0, stream>>>(sp); break;
+        case real16F: add_kernel<__half><<<(unsigned)blocks, 256, 0, stream>>>(sp); break;
+        default: add_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, stream>>>(sp); break;
+        }
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        g_launches.fetch_add(1, std::memory_order_relaxed);
+    }
+    const LocalDescriptor d_x(mx, type);
+    if (dWGate) {
+        const LocalDescriptor d_out(dwg, type), d_dg(dg, type);
+        if ((e = srtMatmul(x, &d_x.d, true, dGate, &d_dg.d, false, dWGate, &d_out.d, stream)) != cudaSuccess) return e;
+    }
+    if (dWUp) {
+        const LocalDescriptor d_out(dwu, type), d_du(du, type);
+        if ((e = srtMatmul(x, &d_x.d, true, dUp, &d_du.d, false, dWUp, &d_out.d, stream)) != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 // ------------------------------------------------------------------ srtRnnCell

@@ -9,7 +9,7 @@ import torch
 
 from . import _lib
 from ._lib import lib
-from .matmul import MatmulError, _descriptor, matmul
+from .matmul import MatmulError, _descriptor, descriptor_args, enqueue, matmul, on_one_device
 from .tensor import ActivationType, order_of
 
 
@@ -96,3 +96,74 @@ class Dense:
         dx = matmul(dz, self.weight, False, True)
         dw = matmul(input, dz, True, False)
         return dx, dw, db
+
+
+class GatedDense:
+    """y = activation(x . weightGate + biasGate) * (x . weightUp + biasUp): two Dense layers over one input and the
+    product of their results, as one launch (srtMatmulGated).  Weights [inputSize x outputSize], biases [outputSize] or
+    None.  Inputs may have any leading dimensions."""
+
+    def __init__(self, weight_gate, weight_up, bias_gate: torch.Tensor | None = None, bias_up: torch.Tensor | None = None,
+                 activation: ActivationType = ActivationType.silu):
+        if tuple(weight_gate.shape) != tuple(weight_up.shape) or len(weight_gate.shape) != 2:
+            raise ValueError("weightGate and weightUp must be matrices of one shape")
+        for bias in (bias_gate, bias_up):
+            if bias is not None and tuple(bias.shape) != (weight_gate.shape[1],):
+                raise ValueError("a bias has one element per column of its weight")
+        self.weight_gate, self.weight_up = weight_gate, weight_up
+        self.bias_gate, self.bias_up = bias_gate, bias_up
+        self.activation = ActivationType(activation)
+
+    def _forward(self, x: torch.Tensor, gate, up) -> torch.Tensor:
+        y = torch.empty((x.shape[0], self.weight_gate.shape[1]), dtype=x.dtype, device=x.device)
+        enqueue(lib.srtMatmulGated, x.device, *descriptor_args(x, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up),
+                int(self.activation), *descriptor_args(gate, up, y))
+        return y
+
+    def __call__(self, input: torch.Tensor) -> torch.Tensor:
+        on_one_device(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up)
+        x = input if input.dim() == 2 else input.reshape(-1, input.shape[-1])
+        try:
+            y = self._forward(x, None, None)
+        except MatmulError as e:
+            if e.code != _lib.cudaErrorNotSupported:
+                raise
+            y = self._forward(x, *self._pre_activations(x))          # two products and an elementwise pass
+        return y if input.dim() == 2 else y.view(*input.shape[:-1], -1)
+
+    def _pre_activations(self, x: torch.Tensor):
+        shape = (x.shape[0], self.weight_gate.shape[1])
+        return tuple(torch.empty(shape, dtype=x.dtype, device=x.device) for _ in range(2))
+
+    def forward_keep(self, input: torch.Tensor):
+        """(output, saved) for training; `saved` is the pair of pre-activations that backward() needs."""
+        on_one_device(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up)
+        x = input.reshape(-1, input.shape[-1])
+        saved = self._pre_activations(x)
+        return self._forward(x, *saved).view(*input.shape[:-1], -1), saved
+
+    def backward(self, input: torch.Tensor, saved: tuple, out_grad: torch.Tensor):
+        """Gradients of (input, weightGate, weightUp, biasGate, biasUp); None for a bias that is None.  `saved` is the
+        second value of forward_keep."""
+        gate, up = saved
+        on_one_device(input, out_grad, gate, up, self.weight_gate, self.weight_up)
+        x, dy = input.reshape(-1, input.shape[-1]), out_grad.reshape(-1, out_grad.shape[-1])
+
+        def like(t, wanted=True):
+            return torch.empty(t.shape, dtype=x.dtype, device=x.device) if wanted else None
+
+        dgate, dup, dx, dwg, dwu = like(gate), like(up), like(x), like(self.weight_gate), like(self.weight_up)
+        dbg = like(self.bias_gate) if self.bias_gate is not None else None
+        dbu = like(self.bias_up) if self.bias_up is not None else None
+
+        def call(dx2):
+            enqueue(lib.srtMatmulGatedBackward, x.device, *descriptor_args(dy, x, self.weight_gate, self.weight_up, gate, up), int(self.activation),
+                    *descriptor_args(dgate, dup, dx, dx2, dwg, dwu, dbg, dbu))
+
+        try:
+            call(like(x, x.dtype == torch.float32))
+        except MatmulError as e:
+            if e.code != _lib.cudaErrorNotSupported:
+                raise
+            call(like(x))
+        return dx.view(input.shape), dwg, dwu, dbg, dbu

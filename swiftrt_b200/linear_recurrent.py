@@ -10,21 +10,10 @@ import torch
 
 from ._lib import lib
 from .dense import bias_activation_backward
-from .matmul import _descriptor, enqueue, matmul, on_one_device
+from .matmul import descriptor_args, enqueue, matmul, on_one_device
 from .tensor import ActivationType
 
 STATE_CHUNK = 64            # steps between two kept states (SRT_GATED_RECURRENCE_CHUNK)
-
-
-def _args(*tensors) -> list:
-    """(data pointer, descriptor address) of every tensor, two nulls for None."""
-    out = []
-    for t in tensors:
-        if t is None:
-            out += (None, None)
-        else:
-            out += (t.data_ptr(), _descriptor(t).address)
-    return out
 
 
 def _lengths(lengths: torch.Tensor | None, batch: int) -> int | None:
@@ -59,8 +48,8 @@ def gated_recurrence(update: torch.Tensor, forget: torch.Tensor, input: torch.Te
     if keep:
         steps = update.shape[1] if update.dim() == 3 else 1
         states = torch.empty((update.shape[0], -(-steps // STATE_CHUNK), update.shape[-1]), dtype=torch.float32, device=update.device)
-    enqueue(lib.srtGatedRecurrence, update.device, *_args(update, forget, input, output, initial), _lengths(lengths, update.shape[0]),
-            *_args(hidden, last, states))
+    enqueue(lib.srtGatedRecurrence, update.device, *descriptor_args(update, forget, input, output, initial), _lengths(lengths, update.shape[0]),
+            *descriptor_args(hidden, last, states))
     return (hidden, last, states) if keep else (hidden, last)
 
 
@@ -75,8 +64,8 @@ def gated_recurrence_backward(out_grad: torch.Tensor, update: torch.Tensor, forg
         out = tuple(torch.empty(update.shape, dtype=update.dtype, device=update.device) if t is not None else None
                     for t in (update, forget, input, output))
     initial_grad = torch.empty(_state_shape(update), dtype=torch.float32, device=update.device)
-    enqueue(lib.srtGatedRecurrenceBackward, update.device, *_args(out_grad, last_grad, update, forget, input, output, states),
-            _lengths(lengths, update.shape[0]), *_args(*out, initial_grad))
+    enqueue(lib.srtGatedRecurrenceBackward, update.device, *descriptor_args(out_grad, last_grad, update, forget, input, output, states),
+            _lengths(lengths, update.shape[0]), *descriptor_args(*out, initial_grad))
     return (*out, initial_grad)
 
 

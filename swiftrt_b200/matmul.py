@@ -56,6 +56,17 @@ def _descriptor(t: torch.Tensor) -> Descriptor:
     return d
 
 
+def descriptor_args(*tensors) -> list:
+    """(data pointer, descriptor address) of every tensor, two nulls for None."""
+    out = []
+    for t in tensors:
+        if t is None:
+            out += (None, None)
+        else:
+            out += (t.data_ptr(), _descriptor(t).address)
+    return out
+
+
 def enqueue(fn, device: torch.device, *args) -> None:
     """Calls `fn(*args, stream)` with torch's current stream of `device`, that device being current (a legacy
     default stream belongs to whatever device is); raises MatmulError for a non-zero status."""

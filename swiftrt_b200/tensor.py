@@ -32,7 +32,7 @@ class Order(enum.IntEnum):
 
 
 class ActivationType(enum.IntEnum):
-    """Raw values of ActivationType (platform/common/FunctionProperties.swift:44-51) plus gelu."""
+    """Raw values of ActivationType (platform/common/FunctionProperties.swift:44-51) plus gelu and silu."""
     sigmoid = 0
     relu = 1
     tanh = 2
@@ -41,6 +41,7 @@ class ActivationType(enum.IntEnum):
     identity = 5
     gelu = 6
     geluTanh = 7
+    silu = 8                # gated and 4-bit products only
 
 
 _TORCH2SRT = {torch.float32: DataType.real32F, torch.float16: DataType.real16F,

@@ -483,6 +483,62 @@ cudaError_t srtMatmulGatedBackward(
     cudaStream_t stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Products with 4-bit weights, for a few rows (the tokens of a generation step).
+ *
+ * A weight [rows x cols] is held as unsigned nibbles q with one scale, and possibly one zero point, per column and group of
+ * groupSize consecutive rows:   W[k, n] = (q[k, n] - z[k / groupSize, n]) * scale[k / groupSize, n].
+ * packed: 32-bit words [ceil(rows / 8) x cols]; word (j, n) holds q[8 j + i, n] in its bits 4 i .. 4 i + 3 (nibbles behind the last
+ * row are ignored).  scales [ceil(rows / groupSize) x cols] have `type`, real16F or real16BF; zeros, one byte each of which
+ * the low four bits count, may be NULL: every zero point is 8.  Columns are contiguous, the strides count elements
+ * between rows (column blocks of a wider weight are such views).  groupSize is 32, 64 or a multiple of 128; the last group may
+ * be shorter.  All pointers are device addresses. */
+typedef struct {
+    srtDataType type;
+    uint32_t groupSize;
+    uint64_t rows;
+    uint64_t cols;
+    const int32_t* packed;
+    int64_t packedStride;
+    const void* scales;
+    int64_t scalesStride;
+    const uint8_t* zeros;
+    int64_t zerosStride;
+} srtInt4Matrix;
+
+/* out = activation(x . W + bias): what srtMatmulBiasActivation computes with the weight above.  x [M x rows], out [M x cols] and bias
+ * [cols] (NULL: none) have the weight's `type`; x and out any strides, out must not overlap anything.  The products of x
+ * and the integers q - z are summed in fp32 and scaled group by group, in fp32: no weight is rounded, and the result is
+ * rounded once.  Any M; the weight is read once for every 32 rows, so that many rows are better served by srtDequantizeInt4 and
+ * srtMatmul.  One launch, no workspace, and a result that does not depend on timing.  All activations but clippedRelu and elu. */
+cudaError_t srtMatmulInt4(
+    const void* x, const srtTensorDescriptor* xDesc,
+    const srtInt4Matrix* weight,
+    const void* bias, const srtTensorDescriptor* biasDesc,
+    srtActivationType activation,
+    void* out, const srtTensorDescriptor* outDesc,
+    cudaStream_t stream);
+
+/* out = activation(x . Wgate + biasGate) * (x . Wup + biasUp): srtMatmulGated with two such weights of one type, shape and
+ * group size, in one launch. */
+cudaError_t srtMatmulGatedInt4(
+    const void* x, const srtTensorDescriptor* xDesc,
+    const srtInt4Matrix* wGate, const srtInt4Matrix* wUp,
+    const void* biasGate, const srtTensorDescriptor* biasGateDesc,
+    const void* biasUp, const srtTensorDescriptor* biasUpDesc,
+    srtActivationType activation,
+    void* out, const srtTensorDescriptor* outDesc,
+    cudaStream_t stream);
+
+/* Writes packed, scales and zeros (where not NULL) of `weight` from w [rows x cols] of its type.  Without zero points
+ * scale = max |w| / 7 and q = round(w / scale) + 8; with them scale = (max - min) / 15 over the group's values and 0,
+ * z = round(-min / scale) and q = round(w / scale) + z; q and z clamped to 0 .. 15, ties to even, in fp32 with the scale
+ * as stored.  A group of zeros has scale 0, one with a value that is not finite scale NaN. */
+cudaError_t srtQuantizeInt4(const void* w, const srtTensorDescriptor* wDesc, const srtInt4Matrix* weight, cudaStream_t stream);
+
+/* out [rows x cols] = W, each element rounded once to the weight's type. */
+cudaError_t srtDequantizeInt4(const srtInt4Matrix* weight, void* out, const srtTensorDescriptor* outDesc, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------------------------
  * srtGatedRecurrence: a gated linear recurrence over whole sequences, and its backward pass.
  *
  * The reference's recurrent cells multiply the previous hidden state by a weight at every step

@@ -16,3 +16,4 @@ from .peer import PeerBuffer  # noqa: F401,E402
 from .recurrent import BasicRNNCell, GRUCell, GraphedSequence, LSTMCell, LSTMState, run_sequence, run_sequence_preconcatenated  # noqa: F401,E402
 from .transform import MatrixLayout, leading_dimension, matrix_transform  # noqa: F401,E402
 from .linear_recurrent import STATE_CHUNK, LinearRecurrentCell, gated_recurrence, gated_recurrence_backward  # noqa: F401,E402
+from .int4 import Int4Weight, gated_matmul_int4, matmul_int4, quantize_int4  # noqa: F401,E402

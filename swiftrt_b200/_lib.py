@@ -45,7 +45,8 @@ EXPORTS = ["srtMatmul", "srtMatmulBiasActivation", "srtMatmulQueryPlan", "srtMat
            "srtActivationForward", "srtMatmulReleaseWorkspaces", "srtGruCell", "srtShardRange", "srtMatmulSharded",
            "srtMatmulShardedDevices", "srtMatmulSetWaitLimit", "srtLstmCellFused", "srtLstmInterleaveGates", "srtPeerSignal", "srtPeerWait", "srtMulticastAlloc", "srtMulticastFree",
            "srtMatrixTransform", "srtMatrixLayoutLeadingDimension", "srtMatrixLayoutElementCount",
-           "srtGatedRecurrence", "srtGatedRecurrenceBackward", "srtMatmulGated", "srtMatmulGatedBackward"]
+           "srtGatedRecurrence", "srtGatedRecurrenceBackward", "srtMatmulGated", "srtMatmulGatedBackward",
+           "srtMatmulInt4", "srtMatmulGatedInt4", "srtQuantizeInt4", "srtDequantizeInt4"]
 
 if not os.path.exists(SO):
     raise ImportError(
@@ -169,6 +170,23 @@ lib.srtMatmulGated.restype = ctypes.c_int
 lib.srtMatmulGated.argtypes = [_P] * 10 + [ctypes.c_int] + [_P] * 7
 lib.srtMatmulGatedBackward.restype = ctypes.c_int
 lib.srtMatmulGatedBackward.argtypes = [_P] * 12 + [ctypes.c_int] + [_P] * 17
+
+
+class Int4Matrix(ctypes.Structure):
+    """srtInt4Matrix of include/srt_matmul_api.h."""
+    _fields_ = [("type", ctypes.c_int), ("groupSize", ctypes.c_uint32), ("rows", ctypes.c_uint64), ("cols", ctypes.c_uint64),
+                ("packed", _P), ("packedStride", ctypes.c_int64), ("scales", _P), ("scalesStride", ctypes.c_int64),
+                ("zeros", _P), ("zerosStride", ctypes.c_int64)]
+
+
+lib.srtMatmulInt4.restype = ctypes.c_int
+lib.srtMatmulInt4.argtypes = [_P] * 5 + [ctypes.c_int] + [_P] * 3
+lib.srtMatmulGatedInt4.restype = ctypes.c_int
+lib.srtMatmulGatedInt4.argtypes = [_P] * 8 + [ctypes.c_int] + [_P] * 3
+lib.srtQuantizeInt4.restype = ctypes.c_int
+lib.srtQuantizeInt4.argtypes = [_P] * 4
+lib.srtDequantizeInt4.restype = ctypes.c_int
+lib.srtDequantizeInt4.argtypes = [_P] * 4
 
 
 def last_error() -> str:

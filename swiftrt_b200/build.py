@@ -13,7 +13,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 SO = os.path.join(PKG, "libsrt_b200.so")
-SOURCES = [os.path.join(PKG, "csrc", f) for f in ("srt_matmul.cu", "srt_sequence.cu")]
+SOURCES = [os.path.join(PKG, "csrc", f) for f in ("srt_matmul.cu", "srt_sequence.cu", "srt_int4.cu")]
 HEADERS = [os.path.join(PKG, "csrc", h) for h in sorted(os.listdir(os.path.join(PKG, "csrc"))) if h.endswith((".cuh", ".h"))] + [
     os.path.join(ROOT, "include", "srt_matmul_api.h")]
 

@@ -1590,7 +1590,7 @@ cudaError_t gated_matrix(const char* op, const char* what, const void* ptr, cons
     v = Matrix{static_cast<const char*>(ptr), d->shape[0], d->shape[1], (long long)d->strides[0], (long long)d->strides[1]};
     if (!ptr && v.rows * v.cols != 0) return fail(cudaErrorInvalidValue, "%s: %s is null", op, what);
     if (v.rows > 0x7fffffffull || v.cols > 0x7fffffffull) return fail(cudaErrorInvalidValue, "%s: dimension exceeds the supported range", op);
-    if (written && ((v.rows > 1 && v.m == 0) || (v.cols > 1 && v.n == 0)))
+    if (written && v.rows * v.cols != 0 && ((v.rows > 1 && v.m == 0) || (v.cols > 1 && v.n == 0)))
         return fail(cudaErrorInvalidValue, "%s: %s must not repeat elements (zero stride)", op, what);
     return cudaSuccess;
 }

@@ -42,7 +42,7 @@ cudaError_t sequence_arg(const char* op, const char* what, const void* ptr, cons
         return fail(cudaErrorInvalidValue, "%s: %s must be [%llu x %llu x %llu] like update", op, what, (unsigned long long)want.B,
                     (unsigned long long)want.T, (unsigned long long)want.D);
     if (!ptr && s.B * s.T * s.D != 0) return fail(cudaErrorInvalidValue, "%s: %s is null", op, what);
-    if (written && ((s.B > 1 && strides[0] == 0) || (s.T > 1 && strides[1] == 0) || (s.D > 1 && strides[2] == 0)))
+    if (written && s.B * s.T * s.D != 0 && ((s.B > 1 && strides[0] == 0) || (s.T > 1 && strides[1] == 0) || (s.D > 1 && strides[2] == 0)))
         return fail(cudaErrorInvalidValue, "%s: %s must not repeat elements (zero stride)", op, what);
     return cudaSuccess;
 }

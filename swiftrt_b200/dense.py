@@ -9,6 +9,7 @@ import torch
 
 from . import _lib
 from ._lib import lib
+from .int4 import Int4Weight, gated_matmul_int4, matmul_int4
 from .matmul import MatmulError, _descriptor, descriptor_args, enqueue, matmul, on_one_device
 from .tensor import ActivationType, order_of
 
@@ -62,16 +63,23 @@ _NEEDS_PRE_ACTIVATION = (ActivationType.gelu, ActivationType.geluTanh)
 
 
 class Dense:
-    def __init__(self, weight: torch.Tensor, bias: torch.Tensor, activation: ActivationType):
+    """`weight` may be an Int4Weight (forward only, `bias` may then be None)."""
+
+    def __init__(self, weight: torch.Tensor | Int4Weight, bias: torch.Tensor | None, activation: ActivationType):
+        self.int4 = isinstance(weight, Int4Weight)
         # Dense.swift:48-49
-        assert order_of(weight) == order_of(bias) or bias.dim() == 1
-        assert bias.shape[0] == weight.shape[-1], "bias.shape[0] must equal weight.shape[1]"
+        if not self.int4:
+            assert order_of(weight) == order_of(bias) or bias.dim() == 1
+        if bias is not None:
+            assert bias.shape[0] == weight.shape[-1], "bias.shape[0] must equal weight.shape[1]"
         self.weight = weight
         self.bias = bias
         self.activation = ActivationType(activation)
         self.plan = None            # Dense.plan (Dense.swift:29): the plan is chosen per call
 
     def __call__(self, input: torch.Tensor) -> torch.Tensor:
+        if self.int4:
+            return matmul_int4(input, self.weight, self.bias, self.activation)
         return matmul(input, self.weight, bias=self.bias, activation=self.activation)
 
     def forward_keep(self, input: torch.Tensor):
@@ -80,6 +88,8 @@ class Dense:
         the fused call and saved is the output itself; GELU's derivative needs the pre-activation
         values, so the product runs with the identity epilogue, its result is kept, and the activation
         is a second elementwise pass."""
+        if self.int4:
+            raise ValueError("a 4-bit weight has no backward pass")
         if self.activation in _NEEDS_PRE_ACTIVATION:
             z = matmul(input, self.weight, bias=self.bias, activation=ActivationType.identity)
             return activation_forward(z, self.activation), z
@@ -100,13 +110,16 @@ class Dense:
 
 class GatedDense:
     """y = activation(x . weightGate + biasGate) * (x . weightUp + biasUp): two Dense layers over one input and the
-    product of their results, as one launch (srtMatmulGated).  Weights [inputSize x outputSize], biases [outputSize] or
-    None.  Inputs may have any leading dimensions."""
+    product of their results, as one launch (srtMatmulGated).  Weights [inputSize x outputSize], both tensors or both
+    Int4Weight (forward only), biases [outputSize] or None.  Inputs may have any leading dimensions."""
 
     def __init__(self, weight_gate, weight_up, bias_gate: torch.Tensor | None = None, bias_up: torch.Tensor | None = None,
                  activation: ActivationType = ActivationType.silu):
         if tuple(weight_gate.shape) != tuple(weight_up.shape) or len(weight_gate.shape) != 2:
             raise ValueError("weightGate and weightUp must be matrices of one shape")
+        self.int4 = isinstance(weight_gate, Int4Weight)
+        if self.int4 != isinstance(weight_up, Int4Weight):
+            raise ValueError("weightGate and weightUp are both 4-bit weights or neither is")
         for bias in (bias_gate, bias_up):
             if bias is not None and tuple(bias.shape) != (weight_gate.shape[1],):
                 raise ValueError("a bias has one element per column of its weight")
@@ -121,6 +134,8 @@ class GatedDense:
         return y
 
     def __call__(self, input: torch.Tensor) -> torch.Tensor:
+        if self.int4:
+            return gated_matmul_int4(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up, self.activation)
         on_one_device(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up)
         x = input if input.dim() == 2 else input.reshape(-1, input.shape[-1])
         try:
@@ -137,6 +152,8 @@ class GatedDense:
 
     def forward_keep(self, input: torch.Tensor):
         """(output, saved) for training; `saved` is the pair of pre-activations that backward() needs."""
+        if self.int4:
+            raise ValueError("4-bit weights have no backward pass")
         on_one_device(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up)
         x = input.reshape(-1, input.shape[-1])
         saved = self._pre_activations(x)

@@ -1,0 +1,75 @@
+"""Weights in 4 bits with one scale (and possibly one zero point) per column and group of rows, and products of a few
+rows with them (srtMatmulInt4): W[k, n] = (q[k, n] - z[k // group, n]) * scale[k // group, n]."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import lib
+from .matmul import descriptor_args, enqueue, on_one_device
+from .tensor import ActivationType, data_type
+
+
+class Int4Weight:
+    """A [rows, cols] weight: `packed` int32 [ceil(rows / 8), cols] (row 8 j + i of column n in bits 4 i .. 4 i + 3 of word
+    (j, n)), `scales` [ceil(rows / group), cols] in Float16 or BFloat16, `zeros` uint8 of the same shape or None (8).
+    Stands where a layer takes a weight (Dense, GatedDense) for its forward pass."""
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group: int, rows: int):
+        self.rows, self.cols, self.group = int(rows), int(packed.shape[-1]), int(group)
+        groups = -(-self.rows // self.group) if self.group > 0 else 0
+        for name, t, dtypes, count in (("packed", packed, (torch.int32,), -(-self.rows // 8)),
+                                       ("scales", scales, (torch.float16, torch.bfloat16), groups), ("zeros", zeros, (torch.uint8,), groups)):
+            if t is None:
+                continue
+            if t.dtype not in dtypes or tuple(t.shape) != (count, self.cols) or (self.cols > 1 and t.stride(1) != 1):
+                raise ValueError(f"{name} must be [{count}, {self.cols}] of {' or '.join(map(str, dtypes))} with contiguous columns")
+        on_one_device(packed, scales, zeros)
+        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self.shape, self.dtype, self.device = (self.rows, self.cols), scales.dtype, packed.device
+        stride = lambda t: max(t.stride(0), self.cols)  # noqa: E731  (a single row may have any stride)
+        self._struct = _lib.Int4Matrix(data_type(scales), self.group, self.rows, self.cols, packed.data_ptr(), stride(packed), scales.data_ptr(),
+                                       stride(scales), zeros.data_ptr() if zeros is not None else None, stride(zeros) if zeros is not None else 0)
+        self.address = ctypes.addressof(self._struct)
+
+    def dequantize(self) -> torch.Tensor:
+        """The weight as a [rows, cols] tensor of its type, each element rounded once (srtDequantizeInt4)."""
+        out = torch.empty(self.shape, dtype=self.dtype, device=self.device)
+        enqueue(lib.srtDequantizeInt4, self.device, self.address, *descriptor_args(out))
+        return out
+
+
+def quantize_int4(weight: torch.Tensor, group: int = 128, zero_points: bool = False) -> Int4Weight:
+    """A Float16 or BFloat16 [rows, cols] weight to 4 bits (srtQuantizeInt4): symmetric about zero, or with a zero point
+    per column and group."""
+    on_one_device(weight)
+    rows, cols = weight.shape
+    groups = -(-rows // group)
+    q = Int4Weight(torch.empty((-(-rows // 8), cols), dtype=torch.int32, device=weight.device),
+                   torch.empty((groups, cols), dtype=weight.dtype, device=weight.device),
+                   torch.empty((groups, cols), dtype=torch.uint8, device=weight.device) if zero_points else None, group, rows)
+    enqueue(lib.srtQuantizeInt4, weight.device, *descriptor_args(weight), q.address)
+    return q
+
+
+def matmul_int4(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None = None,
+                activation: ActivationType = ActivationType.identity) -> torch.Tensor:
+    """activation(x . weight + bias) for an [..., rows] tensor x; asynchronous on torch's current stream."""
+    on_one_device(x, weight, bias)
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    out = torch.empty((flat.shape[0], weight.cols), dtype=x.dtype, device=x.device)
+    enqueue(lib.srtMatmulInt4, x.device, *descriptor_args(flat), weight.address, *descriptor_args(bias), int(activation), *descriptor_args(out))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], -1)
+
+
+def gated_matmul_int4(x: torch.Tensor, weight_gate: Int4Weight, weight_up: Int4Weight, bias_gate: torch.Tensor | None = None,
+                      bias_up: torch.Tensor | None = None, activation: ActivationType = ActivationType.silu) -> torch.Tensor:
+    """activation(x . weight_gate + bias_gate) * (x . weight_up + bias_up) (srtMatmulGatedInt4)."""
+    on_one_device(x, weight_gate, weight_up, bias_gate, bias_up)
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    out = torch.empty((flat.shape[0], weight_gate.cols), dtype=x.dtype, device=x.device)
+    enqueue(lib.srtMatmulGatedInt4, x.device, *descriptor_args(flat), weight_gate.address, weight_up.address,
+            *descriptor_args(bias_gate, bias_up), int(activation), *descriptor_args(out))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], -1)

@@ -1,0 +1,111 @@
+"""The language-model operators together: a residual block of a linear recurrence and a gated feed-forward layer, trained
+on a padded batch, then quantized to 4 bits and run token by token."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def srt():
+    import swiftrt_b200 as s
+    assert torch.cuda.is_available()
+    return s
+
+
+def _weights(nx, nh, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s, scale: (torch.randn(*s, generator=g) * scale).to(dtype).to(DEV)  # noqa: E731
+    return {"mix": n(nx, 3 * nx, scale=nx ** -0.5), "mix_bias": n(3 * nx, scale=0.5), "gate": n(nx, nh, scale=nx ** -0.5),
+            "up": n(nx, nh, scale=nx ** -0.5), "down": n(nh, nx, scale=nh ** -0.5), "down_bias": n(nx, scale=0.1)}
+
+
+def _reference(x, w, lengths):
+    """x + recurrence(x) -> r;  r + down(gated(r)), in 64 bits with autograd."""
+    B, T, nx = x.shape
+    update, forget, output = (x @ w["mix"] + w["mix_bias"]).split(nx, -1)
+    f, c, hs = torch.sigmoid(forget), torch.zeros(B, nx, dtype=x.dtype), []
+    for t in range(T):
+        on = (t < lengths)[:, None]
+        c = torch.where(on, f[:, t] * c + (1 - f[:, t]) * update[:, t], c)
+        hs.append(torch.where(on, c * torch.sigmoid(output[:, t]), torch.zeros_like(c)))
+    r = x + torch.stack(hs, 1)
+    return r + ((torch.nn.functional.silu(r @ w["gate"]) * (r @ w["up"])) @ w["down"] + w["down_bias"])
+
+
+def _block(srt, w, nx):
+    act = srt.ActivationType
+    return (srt.LinearRecurrentCell(w["mix"], w["mix_bias"], nx), srt.GatedDense(w["gate"], w["up"], activation=act.silu),
+            srt.Dense(w["down"], w["down_bias"], act.identity))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_training_step_of_a_block(srt, dtype):
+    B, T, nx, nh = 3, 90, 64, 136
+    w = _weights(nx, nh, dtype)
+    mix, gated, down = _block(srt, w, nx)
+    x = torch.randn(B, T, nx, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    lengths = torch.tensor([T, 0, 33], dtype=torch.int32, device=DEV)
+    h, _, saved_mix = mix.forward_keep(x, lengths=lengths)
+    r = x + h
+    y1, saved_gate = gated.forward_keep(r)
+    y2, kept = down.forward_keep(y1.view(-1, nh))
+    y = r + y2.view_as(r)
+    dy = torch.randn(B, T, nx, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+    d1, d_down, d_down_bias = down.backward(y1.view(-1, nh), kept, dy.view(-1, nx))
+    dr, d_gate, d_up, _, _ = gated.backward(r, saved_gate, d1.view(B, T, nh))
+    dr = dr + dy
+    dx, d_mix, d_mix_bias, _ = mix.backward(x, saved_mix, dr)
+    dx = dx + dr
+    leaves = {k: v.double().cpu().requires_grad_() for k, v in w.items()}
+    x64 = x.double().cpu().requires_grad_()
+    want = _reference(x64, leaves, lengths.cpu())
+    want.backward(dy.double().cpu())
+    # in relative 2-norm: Float32 products are within 1e-5 each, five of them in a row; every 16-bit tensor between two
+    # operators is rounded by at most 2^-8, at most ten of them along a path
+    limit = 5e-5 if dtype == torch.float32 else 10 * 2.0 ** -8
+    for name, got, ref in (("y", y, want.detach()), ("x", dx, x64.grad), ("mix", d_mix, leaves["mix"].grad), ("mix bias", d_mix_bias, leaves["mix_bias"].grad),
+                           ("gate", d_gate, leaves["gate"].grad), ("up", d_up, leaves["up"].grad), ("down", d_down, leaves["down"].grad),
+                           ("down bias", d_down_bias, leaves["down_bias"].grad)):
+        off = float((got.double().cpu() - ref).norm() / ref.norm())
+        assert off <= limit, (name, off)
+
+
+def test_generation_with_4_bit_weights_follows_the_sequence(srt):
+    """A prompt through the 16-bit layers' dequantized weights, then the same block token by token through the 4-bit ones."""
+    B, T, nx, nh = 2, 40, 128, 256
+    act, dt = srt.ActivationType, torch.bfloat16
+    w = _weights(nx, nh, dt, seed=3)
+    q = {k: srt.quantize_int4(w[k], 64, zero_points=True) for k in ("mix", "gate", "up", "down")}
+    exact = {**{k: v.dequantize() for k, v in q.items()}, "mix_bias": w["mix_bias"], "down_bias": w["down_bias"]}
+    x = torch.randn(B, T, nx, generator=torch.Generator().manual_seed(4)).to(dt).to(DEV)
+    want = _reference(x.double().cpu(), {k: v.double().cpu() for k, v in exact.items()}, torch.full((B,), T))
+    mix, gated, down = _block(srt, exact, nx)
+    h, state = mix(x[:, :20])
+    r = x[:, :20] + h
+    parts = [r + down(gated(r).view(-1, nh)).view_as(r)]
+    mix4 = srt.Dense(q["mix"], w["mix_bias"], act.identity)
+    gated4, down4 = srt.GatedDense(q["gate"], q["up"], activation=act.silu), srt.Dense(q["down"], w["down_bias"], act.identity)
+    token, result = torch.empty(B, nx, dtype=dt, device=DEV), torch.empty(B, nx, dtype=dt, device=DEV)
+
+    def step():
+        update, forget, output = mix4(token).split(nx, -1)
+        r = token + srt.gated_recurrence(update, forget, None, output, state, last=state)[0]
+        result.copy_(r + down4(gated4(r)))
+
+    before = state.clone()
+    token.copy_(x[:, 20])
+    step()
+    state.copy_(before)
+    graph = torch.cuda.CUDAGraph()                 # one token as a graph, replayed with a new token in place
+    with torch.cuda.graph(graph):
+        step()
+    for t in range(20, T):
+        token.copy_(x[:, t])
+        graph.replay()
+        parts.append(result.clone()[:, None])
+    got = torch.cat(parts, 1).double().cpu()
+    # rounding of at most 2^-8 at each of the five tensors between the operators, and 2^-9 for the dequantized weights
+    off = float((got - want).norm() / want.norm())
+    assert off <= 6 * 2.0 ** -8, off

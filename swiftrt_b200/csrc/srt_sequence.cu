@@ -108,14 +108,62 @@ cudaError_t recurrence_shape(const char* op, const srtTensorDescriptor* updateDe
     return cudaSuccess;
 }
 
+template <typename T, bool HAS_I, bool HAS_O, int VEC>
+cudaError_t launch_spans(const RecurrenceParams& p, bool backward, cudaStream_t stream)
+{
+    const uint32_t blocks_d = (p.D + 32 * VEC - 1) / (32 * VEC), chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
+    const uint64_t blocks = (uint64_t)p.B * blocks_d;
+    // neighbouring spans of one item and channel block side by side, as long as they all run at once
+    const uint64_t room = 148ull * (backward ? 2 : 3);
+    uint32_t cluster = 1;
+    while (cluster < 8 && blocks * cluster * 2 <= room && cluster < chunks) cluster *= 2;
+    if (blocks * cluster > 0x7fffffffull) return fail(cudaErrorInvalidValue, "too many channels for one call");
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3((unsigned)(blocks * cluster), 1, 1);
+    cfg.blockDim = dim3(256, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return backward ? cudaLaunchKernelEx(&cfg, recurrence_span_backward_kernel<T, HAS_I, HAS_O, VEC>, p, blocks_d, cluster)
+                    : cudaLaunchKernelEx(&cfg, recurrence_span_kernel<T, HAS_I, HAS_O, VEC>, p, blocks_d, cluster);
+}
+
+template <typename T, int VEC>
+cudaError_t launch_spans_gates(const RecurrenceParams& p, bool backward, cudaStream_t stream)
+{
+    if (p.i.p) return p.o.p ? launch_spans<T, true, true, VEC>(p, backward, stream) : launch_spans<T, true, false, VEC>(p, backward, stream);
+    return p.o.p ? launch_spans<T, false, true, VEC>(p, backward, stream) : launch_spans<T, false, false, VEC>(p, backward, stream);
+}
+
+// up to this many steps one thread walks a channel
+constexpr uint32_t kFewSteps = 8;
+
 template <typename T>
 cudaError_t launch_recurrence(const RecurrenceParams& p, bool backward, cudaStream_t stream)
 {
-    const unsigned long long threads = (unsigned long long)p.B * p.D;
-    const unsigned blocks = (unsigned)((threads + 127) / 128);
-    if (backward) recurrence_steps_backward_kernel<T><<<blocks, 128, 0, stream>>>(p);
-    else          recurrence_steps_kernel<T><<<blocks, 128, 0, stream>>>(p);
-    const cudaError_t e = cudaGetLastError();
+    cudaError_t e;
+    if (p.T <= kFewSteps) {
+        const unsigned long long threads = (unsigned long long)p.B * p.D;
+        const unsigned blocks = (unsigned)((threads + 127) / 128);
+        if (backward) recurrence_steps_backward_kernel<T><<<blocks, 128, 0, stream>>>(p);
+        else          recurrence_steps_kernel<T><<<blocks, 128, 0, stream>>>(p);
+        e = cudaGetLastError();
+    } else {
+        // two channels per access where every tensor has them side by side and aligned
+        bool pairs = p.D % 2 == 0;
+        auto look = [&](const void* ptr, long long b, long long t, long long d) {
+            pairs = pairs && (!ptr || (reinterpret_cast<uintptr_t>(ptr) % (2 * sizeof(T)) == 0 && d == 1 && b % 2 == 0 && t % 2 == 0));
+        };
+        for (const Strided3* s : {&p.x, &p.f, &p.i, &p.o, &p.dy}) look(s->p, s->b, s->t, s->d);
+        for (const Strided3W* s : {&p.y, &p.dx, &p.df, &p.di, &p.dout}) look(s->p, s->b, s->t, s->d);
+        e = pairs ? launch_spans_gates<T, 2>(p, backward, stream) : launch_spans_gates<T, 1>(p, backward, stream);
+    }
     if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;
 }

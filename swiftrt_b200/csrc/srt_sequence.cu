@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstring>
 
 #include "gated_recurrence.cuh"
@@ -108,20 +109,36 @@ cudaError_t recurrence_shape(const char* op, const srtTensorDescriptor* updateDe
     return cudaSuccess;
 }
 
-template <typename T, bool HAS_I, bool HAS_O, int VEC>
-cudaError_t launch_spans(const RecurrenceParams& p, bool backward, cudaStream_t stream)
+template <typename Kernel>
+cudaError_t launch_spans_kernel(Kernel kernel, std::atomic<int>* resident, uint32_t smem, const RecurrenceParams& p, uint32_t channels, cudaStream_t stream)
 {
-    const uint32_t blocks_d = (p.D + 32 * VEC - 1) / (32 * VEC), chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
-    const uint64_t blocks = (uint64_t)p.B * blocks_d;
-    // neighbouring spans of one item and channel block side by side, as long as they all run at once
-    const uint64_t room = 148ull * (backward ? 2 : 3);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    // CTAs an SM holds, asked once per kernel and device
+    int per_sm = resident[dev & 63].load(std::memory_order_acquire);
+    if (per_sm == 0) {
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
+        if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kSpanThreads, smem)) != cudaSuccess) return e;
+        if (per_sm < 1) return cudaErrorLaunchOutOfResources;
+        resident[dev & 63].store(per_sm, std::memory_order_release);
+    }
+    const uint32_t blocks_d = (p.D + channels - 1) / channels, chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
+    const uint64_t blocks = (uint64_t)p.B * blocks_d, room = 148ull * (uint64_t)per_sm;
+    // spans of one item and channel block side by side: the cluster that leaves the fewest rounds of resident CTAs, in
+    // units of one CTA's whole sequence (512 blocks with 444 places: two rounds alone, five rounds of an eighth with 8)
     uint32_t cluster = 1;
-    while (cluster < 8 && blocks * cluster * 2 <= room && cluster < chunks) cluster *= 2;
+    double best = 1e300;
+    for (uint32_t c = 1; c <= 8 && c < 2 * chunks; c *= 2) {
+        const double rounds = (double)((blocks * c + room - 1) / room) * ((chunks + c - 1) / c);
+        if (rounds < best * 0.97) { best = rounds; cluster = c; }
+    }
     if (blocks * cluster > 0x7fffffffull) return fail(cudaErrorInvalidValue, "too many channels for one call");
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3((unsigned)(blocks * cluster), 1, 1);
-    cfg.blockDim = dim3(256, 1, 1);
+    cfg.blockDim = dim3(kSpanThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -130,8 +147,16 @@ cudaError_t launch_spans(const RecurrenceParams& p, bool backward, cudaStream_t 
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return backward ? cudaLaunchKernelEx(&cfg, recurrence_span_backward_kernel<T, HAS_I, HAS_O, VEC>, p, blocks_d, cluster)
-                    : cudaLaunchKernelEx(&cfg, recurrence_span_kernel<T, HAS_I, HAS_O, VEC>, p, blocks_d, cluster);
+    return cudaLaunchKernelEx(&cfg, kernel, p, blocks_d, cluster);
+}
+
+template <typename T, bool HAS_I, bool HAS_O, int VEC>
+cudaError_t launch_spans(const RecurrenceParams& p, bool backward, cudaStream_t stream)
+{
+    static std::atomic<int> resident[2][64];
+    constexpr uint32_t kInputs = 2 + HAS_I + HAS_O;
+    return backward ? launch_spans_kernel(recurrence_span_backward_kernel<T, HAS_I, HAS_O, VEC>, resident[1], span_smem_bytes<T, VEC>(kInputs + 1), p, 32 * VEC, stream)
+                    : launch_spans_kernel(recurrence_span_kernel<T, HAS_I, HAS_O, VEC>, resident[0], span_smem_bytes<T, VEC>(kInputs), p, 32 * VEC, stream);
 }
 
 template <typename T, int VEC>

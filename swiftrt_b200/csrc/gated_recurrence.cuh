@@ -10,6 +10,8 @@
 // The forward pass keeps the state before every 64th step (fp32), from which the backward pass recomputes the
 // states in between: 1/16 of the bytes of one 16-bit tensor instead of a second output of 4 bytes per element.
 #pragma once
+#include <cuda.h>
+
 #include <type_traits>
 
 #include "element.cuh"
@@ -35,12 +37,14 @@ struct RecurrenceParams {
     Strided3W dx, df, di, dout;
     float* dinitial; long long dinitial_b, dinitial_d;
     uint32_t B, T, D;
+    uint32_t* status;                    // the device's status word, and the limit of a wait in SM cycles (TMA loads only)
+    unsigned long long wait_cycles;
 };
 
-// s(a), and s(a) with 1 - s(a), each to a relative error of a few 2^-23.  The pair comes from e = exp(-|a|), so the small one
-// of the two is not the difference of 1 and its neighbour (a gate at 0.9999 keeps its decay 1 - f to full precision).  The
-// .ftz forms of the two approximations take one instruction each where the others rescale denormals around them: what is
-// below 2^-126 counts as closed.
+// s(a), and s(a) with 1 - s(a), each to a relative error of a few 2^-23: with e = exp(-a) they are 1 / (1 + e) and
+// e / (1 + e), neither of which is the difference of 1 and its neighbour (a gate at 0.9999 keeps its decay 1 - f to full
+// precision).  The .ftz forms of the two approximations take one instruction each where the others rescale denormals
+// around them.  For the pair e is capped at 2^126, so that a closed gate is 2^-126 and not 0 times infinity.
 struct Gate { float on, off; };
 __device__ __forceinline__ float exp2_ftz(float x)
 {
@@ -54,6 +58,12 @@ __device__ __forceinline__ float reciprocal_ftz(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float min_or_nan(float a, float b)
+{
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 constexpr float kLog2E = 1.4426950408889634f;
 __device__ __forceinline__ float logistic(float a)
 {
@@ -61,9 +71,64 @@ __device__ __forceinline__ float logistic(float a)
 }
 __device__ __forceinline__ Gate logistic_pair(float a)
 {
-    const float e = exp2_ftz(-kLog2E * fabsf(a));
-    const float big = reciprocal_ftz(1.0f + e), small = e * big;
-    return a >= 0.0f ? Gate{big, small} : Gate{small, big};          // a NaN is in e already
+    const float e = exp2_ftz(min_or_nan(-kLog2E * a, 126.0f));
+    const float on = reciprocal_ftz(1.0f + e);
+    return Gate{on, e * on};
+}
+
+// Two neighbouring channels at a time where VEC is 2 (one instruction for both products or sums)
+template <int VEC> __device__ __forceinline__ void mul_to(float (&d)[VEC], const float (&a)[VEC], const float (&b)[VEC])
+{
+    if constexpr (VEC == 2) {
+        asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+    } else {
+        d[0] = a[0] * b[0];
+    }
+}
+template <int VEC> __device__ __forceinline__ void add_to(float (&d)[VEC], const float (&a)[VEC], const float (&b)[VEC])
+{
+    if constexpr (VEC == 2) {
+        asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+    } else {
+        d[0] = a[0] + b[0];
+    }
+}
+template <int VEC> __device__ __forceinline__ void fma_to(float (&d)[VEC], const float (&a)[VEC], const float (&b)[VEC], const float (&c)[VEC])
+{
+    if constexpr (VEC == 2) {
+        asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\t"
+            "mov.b64 {%0, %1}, x;\n\t}"
+            : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
+    } else {
+        d[0] = fmaf(a[0], b[0], c[0]);
+    }
+}
+template <int VEC> __device__ __forceinline__ void logistic_to(float (&on)[VEC], const float (&a)[VEC])
+{
+    float e[VEC], k[VEC], one[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) k[j] = -kLog2E, one[j] = 1.0f;
+    mul_to<VEC>(e, a, k);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) e[j] = exp2_ftz(e[j]);
+    add_to<VEC>(e, e, one);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) on[j] = reciprocal_ftz(e[j]);
+}
+template <int VEC> __device__ __forceinline__ void logistic_pair_to(float (&on)[VEC], float (&off)[VEC], const float (&a)[VEC])
+{
+    float e[VEC], k[VEC], one[VEC], sum[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) k[j] = -kLog2E, one[j] = 1.0f;
+    mul_to<VEC>(e, a, k);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) e[j] = exp2_ftz(min_or_nan(e[j], 126.0f));
+    add_to<VEC>(sum, e, one);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) on[j] = reciprocal_ftz(sum[j]);
+    mul_to<VEC>(off, e, on);
 }
 
 template <typename T> __device__ __forceinline__ float load3(const Strided3& s, uint32_t b, uint32_t t, uint32_t d)
@@ -161,15 +226,27 @@ recurrence_steps_backward_kernel(const __grid_constant__ RecurrenceParams p)
 
 // ------------------------------------------------------------------------------------------ long sequences
 // A step is an affine map c -> f c + u, and maps compose: a span of steps is (A, H) with A the product of its f and H its
-// result from c = 0.  A CTA takes 64 steps of 64 channels (32 with VEC = 1) at a time: 8 warps of 8 steps, a lane VEC
-// neighbouring channels.  Every warp folds its steps into (A, H), the spans are joined in order of time through shared memory, and a second
+// result from c = 0.  A CTA takes 64 steps of 32 VEC channels at a time: 8 warps of 8 steps, a lane VEC neighbouring
+// channels.  Every warp folds its steps into (A, H), the spans are joined in order of time through shared memory, and a second
 // pass over the gates, which are still in registers, produces the values: one read and one write of everything.  Where
 // batch items and channels alone leave SMs idle, the CTAs of a cluster take neighbouring spans of 64 steps and exchange
 // their (A, H) through distributed shared memory, once per 64 x cluster steps.
-// While a span is computed, every thread's own elements of the next one are on their way into shared memory (cp.async, read back
-// by the thread that asked for them, so no barrier is involved).
+//
+// How the elements travel (SRC):
+//   kFromTiles   TMA: one thread asks for a [64 steps x 128 bytes] box of every tensor, two spans ahead, and every warp stores its
+//                [8 x 128 bytes] of the results the same way (of up to three): no addresses, bounds or predicates per
+//                element.  Needs 16-byte aligned rows.
+//   kFromWords   cp.async of 4 or 8 bytes, by the thread that will use them (no barrier), one span ahead.
+//   kFromMemory  plain loads: 16-bit elements at odd offsets.
 constexpr uint32_t kSpanWarps = 8, kSpanSteps = 8, kSpanThreads = 32 * kSpanWarps, kSpanStages = 2;
 static_assert(kSpanWarps * kSpanSteps == kRecurrenceChunk, "a CTA's span is what lies between two kept states");
+enum : int { kFromMemory = 0, kFromWords = 1, kFromTiles = 2 };
+
+// tensor maps of a kFromTiles launch: forget, update, input, output, outGrad; results
+struct RecurrenceMaps { CUtensorMap f, x, i, o, dy, y, dx, df, di, dout; };
+struct NoMaps { uint32_t unused; };
+template <int SRC> struct MapsOf { using type = NoMaps; };
+template <> struct MapsOf<kFromTiles> { using type = RecurrenceMaps; };
 
 // VEC neighbouring elements as one word
 template <typename T, int VEC> struct Lane;
@@ -212,43 +289,59 @@ template <> struct Lane<__half, 2> {
     static __device__ __forceinline__ Raw infinity() { return 0x7c007c00u; }
 };
 
-// One tensor as a thread sees it: its elements of 8 consecutive steps, by way of a ring in shared memory where a word is one
-// that cp.async can move (4 or 8 bytes), else straight into registers.
-template <typename T, int VEC>
+template <typename Raw> __device__ __forceinline__ Raw shared_word(uint32_t at)
+{
+    Raw r;
+    if constexpr (sizeof(Raw) == 2) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(at) : "memory");
+    else if constexpr (sizeof(Raw) == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(at) : "memory");
+    else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at) : "memory");
+    return r;
+}
+template <typename Raw> __device__ __forceinline__ void store_shared_word(uint32_t at, Raw r)
+{
+    if constexpr (sizeof(Raw) == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(r) : "memory");
+    else if constexpr (sizeof(Raw) == 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(r) : "memory");
+    else asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(r.x), "r"(r.y) : "memory");
+}
+
+template <typename T, int VEC> struct SpanTile {
+    using Raw = typename Lane<T, VEC>::Raw;
+    static constexpr uint32_t kRow = 32 * static_cast<uint32_t>(sizeof(Raw)), kBytes = kRecurrenceChunk * kRow;      // one tensor's span in shared memory
+    static constexpr uint32_t kWarpBytes = kSpanSteps * kRow;
+};
+
+// One tensor as a thread sees it: its elements of 8 consecutive steps.
+template <typename T, int VEC, int SRC>
 struct StepReader {
     using Raw = typename Lane<T, VEC>::Raw;
-    static constexpr bool kAsync = sizeof(Raw) >= 4;
+    using Tile = SpanTile<T, VEC>;
     const T* base;
     long long stride;
-    uint32_t ring;                       // shared address of this thread's first word; words of a thread are 256 apart
-    __device__ __forceinline__ StepReader(const Strided3& s, uint32_t b, uint32_t d, uint32_t ring_base, uint32_t which)
+    uint32_t at;                         // shared address of this thread's element of its first step, stage 0
+    __device__ __forceinline__ StepReader(const Strided3& s, uint32_t b, uint32_t d, uint32_t ring, uint32_t which)
         : base(static_cast<const T*>(s.p) + b * s.b + d * s.d), stride(s.t),
-          ring(ring_base + (which * kSpanSteps * kSpanThreads + threadIdx.x) * static_cast<uint32_t>(sizeof(Raw))) {}
+          at(ring + which * Tile::kBytes + (threadIdx.x >> 5) * Tile::kWarpBytes + (threadIdx.x & 31) * static_cast<uint32_t>(sizeof(Raw))) {}
     __device__ __forceinline__ void fetch(uint32_t t0, uint32_t live, uint32_t stage_bytes) const
     {
-        if constexpr (kAsync) {
-            const T* at = base + t0 * stride;
+        const T* from = base + t0 * stride;
 #pragma unroll
-            for (uint32_t k = 0; k < kSpanSteps; ++k, at += stride)
-                if (k < live)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;"
-                                 ::"r"(ring + stage_bytes + k * kSpanThreads * static_cast<uint32_t>(sizeof(Raw))), "l"(at), "n"(sizeof(Raw)) : "memory");
-        }
+        for (uint32_t k = 0; k < kSpanSteps; ++k, from += stride)
+            if (k < live) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at + stage_bytes + k * Tile::kRow), "l"(from), "n"(sizeof(Raw)) : "memory");
     }
-    __device__ __forceinline__ void read(uint32_t t0, uint32_t live, uint32_t stage_bytes, Raw other, Raw (&v)[kSpanSteps]) const
+    // steps at or behind `live` read as `other`; whole: none of them is (uniform over the warp)
+    __device__ __forceinline__ void read(uint32_t t0, uint32_t live, bool whole, uint32_t stage_bytes, Raw other, Raw (&v)[kSpanSteps]) const
     {
-        const T* at = base + t0 * stride;
+        if constexpr (SRC == kFromMemory) {
+            const T* from = base + t0 * stride;
 #pragma unroll
-        for (uint32_t k = 0; k < kSpanSteps; ++k, at += stride) {
-            v[k] = other;
-            if constexpr (kAsync) {
-                const uint32_t from = ring + stage_bytes + k * kSpanThreads * static_cast<uint32_t>(sizeof(Raw));
-                if (k < live) {
-                    if constexpr (sizeof(Raw) == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t*>(&v[k])) : "r"(from) : "memory");
-                    else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(reinterpret_cast<uint32_t*>(&v[k])[0]), "=r"(reinterpret_cast<uint32_t*>(&v[k])[1]) : "r"(from) : "memory");
-                }
-            } else {
-                if (k < live) v[k] = *reinterpret_cast<const Raw*>(at);
+            for (uint32_t k = 0; k < kSpanSteps; ++k, from += stride) v[k] = k < live ? *reinterpret_cast<const Raw*>(from) : other;
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < kSpanSteps; ++k) v[k] = shared_word<Raw>(at + stage_bytes + k * Tile::kRow);
+            if (!whole) {
+#pragma unroll
+                for (uint32_t k = 0; k < kSpanSteps; ++k)
+                    if (k >= live) v[k] = other;
             }
         }
     }
@@ -256,10 +349,34 @@ struct StepReader {
 __device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename T, int VEC> __host__ __device__ constexpr uint32_t span_smem_bytes(uint32_t tensors)
+template <typename T, int VEC, int SRC> __host__ __device__ constexpr uint32_t span_stage_bytes(uint32_t tensors)
 {
-    return StepReader<T, VEC>::kAsync ? kSpanStages * tensors * kSpanSteps * kSpanThreads * static_cast<uint32_t>(sizeof(typename Lane<T, VEC>::Raw)) : 0;
+    return SRC == kFromMemory ? 0 : tensors * SpanTile<T, VEC>::kBytes;
 }
+template <typename T, int VEC, int SRC> __host__ __device__ constexpr uint32_t span_smem_bytes(uint32_t tensors, uint32_t results)
+{
+    // four results do not fit next to the ring of five tensors while two CTAs share an SM: they are stored from registers
+    return kSpanStages * span_stage_bytes<T, VEC, SRC>(tensors) + (SRC == kFromTiles ? (results < 4 ? results : 0) * SpanTile<T, VEC>::kBytes + 128 : 0);
+}
+
+// Where a warp's results of 8 steps go.
+template <typename T, int VEC, bool TILE>
+struct StepWriter {
+    using Raw = typename Lane<T, VEC>::Raw;
+    using Tile = SpanTile<T, VEC>;
+    T* to;
+    long long stride;
+    uint32_t at;
+    __device__ __forceinline__ StepWriter(const Strided3W& s, uint32_t b, uint32_t d, uint32_t t0, uint32_t staging, uint32_t which)
+        : to(static_cast<T*>(s.p) + b * s.b + d * s.d + t0 * s.t), stride(s.t),
+          at(staging + which * Tile::kBytes + (threadIdx.x >> 5) * Tile::kWarpBytes + (threadIdx.x & 31) * static_cast<uint32_t>(sizeof(Raw))) {}
+    // `there`: how many of the 8 steps exist
+    __device__ __forceinline__ void put(uint32_t k, uint32_t there, Raw v) const
+    {
+        if constexpr (TILE) store_shared_word<Raw>(at + k * Tile::kRow, v);
+        else if (k < there) *reinterpret_cast<Raw*>(to + k * stride) = v;
+    }
+};
 
 // a float2 (VEC = 2) or float per lane and quantity, in shared memory of any CTA of the cluster
 template <int VEC> struct Span { float a[VEC], h[VEC]; };
@@ -273,88 +390,137 @@ template <int VEC> __device__ __forceinline__ void span_to_cta(const Span<VEC>* 
         asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(s.a[0]), "f"(s.h[0]) : "memory");
 }
 
-template <typename T, bool HAS_I, bool HAS_O, int VEC>
+// What a kFromTiles CTA waits with.  A wait that runs over the limit is noted in the status word (the result of the launch is
+// invalid then); the thread still waits, as long again as kDrainCycles allows, for the copies to land before it goes on.
+constexpr uint64_t kTileDrainCycles = 4000000000ull;
+struct TileWaits {
+    uint32_t bars;                       // one mbarrier per stage
+    uint32_t* status;
+    uint64_t limit;
+    uint32_t phases = 0;                 // bit s: parity of stage s's next wait
+    bool dead = false;
+    __device__ __forceinline__ void wait(uint32_t stage)
+    {
+        const uint32_t parity = (phases >> stage) & 1;
+        phases ^= 1u << stage;
+        if (dead || mbar_test_wait(bars + 8 * stage, parity)) return;
+        const uint64_t t0 = sm_clock();
+        while (!mbar_try_wait(bars + 8 * stage, parity) && !dead) dead = sm_clock() - t0 > limit + kTileDrainCycles;
+        if (sm_clock() - t0 > limit) atomicOr(status, 1u);
+    }
+};
+
+template <typename T, bool HAS_I, bool HAS_O, int VEC, int SRC>
 __global__ void __launch_bounds__(kSpanThreads, 3)
-recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, uint32_t blocks_d, uint32_t cluster)
+recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_constant__ typename MapsOf<SRC>::type maps, uint32_t blocks_d, uint32_t cluster)
 {
     using L = Lane<T, VEC>;
     using Raw = typename L::Raw;
-    constexpr uint32_t kTensors = 2 + HAS_I + HAS_O, kStageBytes = span_smem_bytes<T, VEC>(kTensors) / kSpanStages;
-    extern __shared__ __align__(16) uint8_t ring[];
+    using Tile = SpanTile<T, VEC>;
+    constexpr uint32_t kTensors = 2 + HAS_I + HAS_O, kStageBytes = span_stage_bytes<T, VEC, SRC>(kTensors);
+    extern __shared__ __align__(128) uint8_t dynamic_smem[];
     __shared__ alignas(16) Span<VEC> in_cta[2][kSpanWarps][32];
     __shared__ alignas(16) Span<VEC> in_cluster[2][8][32];
+    __shared__ alignas(8) uint64_t full[kSpanStages];
+    const uint32_t ring = SRC == kFromTiles ? (smem_u32(dynamic_smem) + 127u) & ~127u : smem_u32(dynamic_smem);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster > 1 ? cluster_ctarank() : 0;
     const uint32_t block = blockIdx.x / cluster;
-    const uint32_t b = block / blocks_d, d = ((block % blocks_d) * 32 + lane) * VEC;
+    const uint32_t b = block / blocks_d, d0 = (block % blocks_d) * 32 * VEC, d = d0 + lane * VEC;
     const bool on = d < p.D;
     const uint32_t n = live_steps(p, b);
     const uint32_t chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
-    const StepReader<T, VEC> qf(p.f, b, d, smem_u32(ring), 0), qx(p.x, b, d, smem_u32(ring), 1), qi(p.i, b, d, smem_u32(ring), 2),
-        qo(p.o, b, d, smem_u32(ring), 2 + HAS_I);
+    const StepReader<T, VEC, SRC> qf(p.f, b, d, ring, 0), qx(p.x, b, d, ring, 1), qi(p.i, b, d, ring, 2), qo(p.o, b, d, ring, 2 + HAS_I);
+    TileWaits waits{smem_u32(full), p.status, p.wait_cycles};
     // this thread's first step of chunk k, and how many of its 8 belong to the sequence
     auto first_step = [&](uint32_t k) { return (k + rank) * kRecurrenceChunk + warp * kSpanSteps; };
-    auto live_from = [&](uint32_t t0) { return on && t0 < n ? n - t0 : 0u; };
-    auto fetch = [&](uint32_t k, uint32_t stage_bytes) {
-        const uint32_t t0 = first_step(k), live = live_from(t0);
-        qf.fetch(t0, live, stage_bytes);
-        qx.fetch(t0, live, stage_bytes);
-        if constexpr (HAS_I) qi.fetch(t0, live, stage_bytes);
-        if constexpr (HAS_O) qo.fetch(t0, live, stage_bytes);
-        fetch_commit();
+    auto live_from = [&](uint32_t t0) { return t0 < n ? n - t0 : 0u; };
+    auto fetch = [&](uint32_t k, uint32_t stage) {
+        if constexpr (SRC == kFromTiles) {
+            const uint32_t t = (k + rank) * kRecurrenceChunk;
+            if (threadIdx.x == 0 && t < n) {                    // (t < n <= T keeps k below chunks)
+                const uint32_t bar = smem_u32(&full[stage]), to = ring + stage * kStageBytes;
+                mbar_arrive_expect_tx(bar, kStageBytes);
+                tma_load_3d(to, &maps.f, bar, d0, t, b);
+                tma_load_3d(to + Tile::kBytes, &maps.x, bar, d0, t, b);
+                if constexpr (HAS_I) tma_load_3d(to + 2 * Tile::kBytes, &maps.i, bar, d0, t, b);
+                if constexpr (HAS_O) tma_load_3d(to + (2 + HAS_I) * Tile::kBytes, &maps.o, bar, d0, t, b);
+            }
+        } else if constexpr (SRC == kFromWords) {
+            const uint32_t t0 = first_step(k), live = on ? live_from(t0) : 0;
+            qf.fetch(t0, live, stage * kStageBytes);
+            qx.fetch(t0, live, stage * kStageBytes);
+            if constexpr (HAS_I) qi.fetch(t0, live, stage * kStageBytes);
+            if constexpr (HAS_O) qo.fetch(t0, live, stage * kStageBytes);
+            fetch_commit();
+        }
     };
+    if constexpr (SRC == kFromTiles) {
+        if (threadIdx.x == 0) {
+            mbar_init(smem_u32(&full[0]), 1);
+            mbar_init(smem_u32(&full[1]), 1);
+            fence_mbar_init();
+        }
+        __syncthreads();
+    }
+    fetch(0, 0);
+    if constexpr (SRC == kFromTiles) fetch(cluster, 1);
 
     float state[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) state[j] = p.initial && on ? p.initial[b * p.initial_b + (d + j) * p.initial_d] : 0.0f;
 
     uint32_t buf = 0;
-    if (chunks > 0) fetch(0, 0);
     for (uint32_t first = 0; first < chunks; first += cluster, buf ^= 1) {
         const uint32_t chunk = first + rank, t0 = first_step(first), live = live_from(t0);
-        fetch(first + cluster, (buf ^ 1) * kStageBytes);                  // behind the last chunk nothing is live
-        fetch_wait<1>();
+        const bool whole = live >= kSpanSteps;
+        if constexpr (SRC == kFromWords) {
+            fetch(first + cluster, buf ^ 1);                      // behind the last chunk nothing is live
+            fetch_wait<1>();
+        }
+        if constexpr (SRC == kFromTiles) {
+            if (chunk * kRecurrenceChunk < n) waits.wait(buf);
+        }
         // behind the sequence a forget logit of infinity and an update of zero leave the state as it is
         float f[kSpanSteps][VEC], u[kSpanSteps][VEC];
         Span<VEC> mine;
+        Raw ro[kSpanSteps];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) mine.a[j] = 1.0f, mine.h[j] = 0.0f;
         {
             Raw rf[kSpanSteps], rx[kSpanSteps], ri[kSpanSteps];
-            qf.read(t0, live, buf * kStageBytes, L::infinity(), rf);
-            qx.read(t0, live, buf * kStageBytes, Raw{}, rx);
-            if constexpr (HAS_I) qi.read(t0, live, buf * kStageBytes, Raw{}, ri);
+            const uint32_t mem_live = SRC == kFromMemory && !on ? 0 : live;
+            qf.read(t0, mem_live, whole, buf * kStageBytes, L::infinity(), rf);
+            qx.read(t0, mem_live, whole, buf * kStageBytes, Raw{}, rx);
+            if constexpr (HAS_I) qi.read(t0, mem_live, whole, buf * kStageBytes, Raw{}, ri);
+            if constexpr (HAS_O) qo.read(t0, mem_live, whole, buf * kStageBytes, Raw{}, ro);
 #pragma unroll
             for (uint32_t s = 0; s < kSpanSteps; ++s) {
-                float vf[VEC], vx[VEC], vi[VEC];
+                float vf[VEC], vx[VEC], in[VEC];
                 L::unpack(rf[s], vf);
                 L::unpack(rx[s], vx);
-                if constexpr (HAS_I) L::unpack(ri[s], vi);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const Gate g = logistic_pair(vf[j]);
-                    float in = g.off;
-                    if constexpr (HAS_I) in = logistic(vi[j]);
-                    f[s][j] = g.on;
-                    u[s][j] = in * vx[j];
-                    mine.h[j] = fmaf(f[s][j], mine.h[j], u[s][j]);
-                    mine.a[j] *= f[s][j];
+                logistic_pair_to<VEC>(f[s], in, vf);
+                if constexpr (HAS_I) {
+                    float vi[VEC];
+                    L::unpack(ri[s], vi);
+                    logistic_to<VEC>(in, vi);
                 }
+                mul_to<VEC>(u[s], in, vx);
+                fma_to<VEC>(mine.h, f[s], mine.h, u[s]);
+                mul_to<VEC>(mine.a, mine.a, f[s]);
             }
         }
         in_cta[buf][warp][lane] = mine;
         __syncthreads();
+        if constexpr (SRC == kFromTiles) fetch(first + 2 * cluster, buf);         // everyone has read this stage
         if (cluster > 1) {
             if (warp == 0) {
                 Span<VEC> all = mine;
 #pragma unroll
                 for (uint32_t w = 1; w < kSpanWarps; ++w) {
                     const Span<VEC> next = in_cta[buf][w][lane];
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        all.h[j] = fmaf(next.a[j], all.h[j], next.h[j]);
-                        all.a[j] *= next.a[j];
-                    }
+                    fma_to<VEC>(all.h, next.a, all.h, next.h);
+                    mul_to<VEC>(all.a, all.a, next.a);
                 }
                 for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], r, all);
             }
@@ -362,57 +528,69 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, uint32_t bloc
             cluster_wait_acquire();
         }
         // the state before this CTA's span, before this warp's steps, and behind the whole cluster's span
-        float c[VEC], begin[VEC];
+        float c[VEC], begin[VEC], run[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) begin[j] = state[j];
         if (cluster > 1) {
             for (uint32_t r = 0; r < cluster; ++r) {
                 const Span<VEC> s = in_cluster[buf][r][lane];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
+                for (int j = 0; j < VEC; ++j)
                     if (r == rank) begin[j] = state[j];
-                    state[j] = fmaf(s.a[j], state[j], s.h[j]);
-                }
+                fma_to<VEC>(state, s.a, state, s.h);
             }
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) c[j] = begin[j];
-        for (uint32_t w = 0; w < warp; ++w) {
+        for (int j = 0; j < VEC; ++j) c[j] = run[j] = begin[j];
+#pragma unroll
+        for (uint32_t w = 0; w < kSpanWarps; ++w) {
             const Span<VEC> s = in_cta[buf][w][lane];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) c[j] = fmaf(s.a[j], c[j], s.h[j]);
+            for (int j = 0; j < VEC; ++j)
+                if (w == warp) c[j] = run[j];
+            fma_to<VEC>(run, s.a, run, s.h);
         }
         if (cluster == 1) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) state[j] = c[j];
-            for (uint32_t w = warp; w < kSpanWarps; ++w) {
-                const Span<VEC> s = in_cta[buf][w][lane];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) state[j] = fmaf(s.a[j], state[j], s.h[j]);
-            }
+            for (int j = 0; j < VEC; ++j) state[j] = run[j];
         }
         if (p.states && warp == 0 && on && chunk < chunks) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) p.states[b * p.states_b + chunk * p.states_c + (d + j) * p.states_d] = begin[j];
         }
-        Raw ro[kSpanSteps];
-        if constexpr (HAS_O) qo.read(t0, live, buf * kStageBytes, Raw{}, ro);
-        T* at = static_cast<T*>(p.y.p) + b * p.y.b + d * p.y.d + t0 * p.y.t;
         const uint32_t there = on && t0 < p.T ? p.T - t0 : 0;
+        const StepWriter<T, VEC, SRC == kFromTiles> out(p.y, b, d, t0, ring + kSpanStages * kStageBytes, 0);
+        if constexpr (SRC == kFromTiles) {
+            if (lane == 0) bulk_wait_group_read<0>();             // the last span's results have left the staging rows
+            __syncwarp();
+        }
 #pragma unroll
-        for (uint32_t s = 0; s < kSpanSteps; ++s, at += p.y.t) {
-            float v[VEC], vo[VEC];
-            if constexpr (HAS_O) L::unpack(ro[s], vo);
+        for (uint32_t s = 0; s < kSpanSteps; ++s) {
+            float v[VEC];
+            fma_to<VEC>(c, f[s], c, u[s]);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                c[j] = fmaf(f[s][j], c[j], u[s][j]);
-                v[j] = c[j];
-                if constexpr (HAS_O) v[j] *= logistic(vo[j]);
+            for (int j = 0; j < VEC; ++j) v[j] = c[j];
+            if constexpr (HAS_O) {
+                float vo[VEC];
+                L::unpack(ro[s], vo);
+                logistic_to<VEC>(vo, vo);
+                mul_to<VEC>(v, v, vo);
             }
             Raw y = L::pack(v);
-            if (s >= live) y = Raw{};
-            if (s < there) *reinterpret_cast<Raw*>(at) = y;
+            if (!whole && s >= live) y = Raw{};
+            out.put(s, there, y);
         }
+        if constexpr (SRC == kFromTiles) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && t0 < p.T) {                          // steps and channels that do not exist are not written
+                tma_store_3d(&maps.y, ring + kSpanStages * kStageBytes + warp * Tile::kWarpBytes, d0, t0, b);
+                bulk_commit_group();
+            }
+        }
+    }
+    if constexpr (SRC == kFromTiles) {
+        if (lane == 0) bulk_wait_group<0>();
     }
     if (p.last && rank == 0 && warp == 0 && on) {
 #pragma unroll
@@ -424,90 +602,134 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, uint32_t bloc
 // the state runs the other way, e -> f (p + e) per step, with the same product A and E the span's result from e = 0.
 template <int VEC> struct SpanBoth { float a[VEC], h[VEC], e[VEC]; };
 
-template <typename T, bool HAS_I, bool HAS_O, int VEC>
+template <typename T, bool HAS_I, bool HAS_O, int VEC, int SRC>
 __global__ void __launch_bounds__(kSpanThreads, 2)
-recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, uint32_t blocks_d, uint32_t cluster)
+recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, const __grid_constant__ typename MapsOf<SRC>::type maps, uint32_t blocks_d, uint32_t cluster)
 {
     using L = Lane<T, VEC>;
     using Raw = typename L::Raw;
-    constexpr uint32_t kTensors = 3 + HAS_I + HAS_O, kStageBytes = span_smem_bytes<T, VEC>(kTensors) / kSpanStages;
-    extern __shared__ __align__(16) uint8_t ring[];
+    using Tile = SpanTile<T, VEC>;
+    constexpr uint32_t kTensors = 3 + HAS_I + HAS_O, kStageBytes = span_stage_bytes<T, VEC, SRC>(kTensors);
+    constexpr bool kTileStores = SRC == kFromTiles && !(HAS_I && HAS_O);
+    extern __shared__ __align__(128) uint8_t dynamic_smem[];
     __shared__ SpanBoth<VEC> in_cta[2][kSpanWarps][32];
     __shared__ alignas(16) Span<VEC> in_cluster[2][8][32];
+    __shared__ alignas(8) uint64_t full[kSpanStages];
+    const uint32_t ring = SRC == kFromTiles ? (smem_u32(dynamic_smem) + 127u) & ~127u : smem_u32(dynamic_smem);
+    const uint32_t staging = ring + kSpanStages * kStageBytes;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster > 1 ? cluster_ctarank() : 0;
     const uint32_t block = blockIdx.x / cluster;
-    const uint32_t b = block / blocks_d, d = ((block % blocks_d) * 32 + lane) * VEC;
+    const uint32_t b = block / blocks_d, d0 = (block % blocks_d) * 32 * VEC, d = d0 + lane * VEC;
     const bool on = d < p.D;
     const uint32_t n = live_steps(p, b);
     const uint32_t chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
-    const StepReader<T, VEC> qf(p.f, b, d, smem_u32(ring), 0), qx(p.x, b, d, smem_u32(ring), 1), qy(p.dy, b, d, smem_u32(ring), 2),
-        qi(p.i, b, d, smem_u32(ring), 3), qo(p.o, b, d, smem_u32(ring), 3 + HAS_I);
+    const StepReader<T, VEC, SRC> qf(p.f, b, d, ring, 0), qx(p.x, b, d, ring, 1), qy(p.dy, b, d, ring, 2), qi(p.i, b, d, ring, 3), qo(p.o, b, d, ring, 3 + HAS_I);
+    TileWaits waits{smem_u32(full), p.status, p.wait_cycles};
     // after `done` chunks from the end this CTA has chunk chunks - 1 - done - rank, if that is one
-    auto first_step = [&](uint32_t done) { return done + rank < chunks ? (chunks - 1 - done - rank) * kRecurrenceChunk + warp * kSpanSteps : p.T; };
-    auto live_from = [&](uint32_t t0) { return on && t0 < n ? n - t0 : 0u; };
+    auto chunk_start = [&](uint32_t done) { return done + rank < chunks ? (chunks - 1 - done - rank) * kRecurrenceChunk : p.T; };
+    auto live_from = [&](uint32_t t0) { return t0 < n ? n - t0 : 0u; };
     float c[VEC], c_next[VEC];                              // the kept state of the chunk, fetched one chunk ahead
-    auto fetch = [&](uint32_t done, uint32_t stage_bytes) {
-        const uint32_t t0 = first_step(done), live = live_from(t0);
-        qf.fetch(t0, live, stage_bytes);
-        qx.fetch(t0, live, stage_bytes);
-        qy.fetch(t0, live, stage_bytes);
-        if constexpr (HAS_I) qi.fetch(t0, live, stage_bytes);
-        if constexpr (HAS_O) qo.fetch(t0, live, stage_bytes);
-        fetch_commit();
+    auto fetch_state = [&](uint32_t done) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
             c_next[j] = done + rank < chunks && on ? p.states[b * p.states_b + (chunks - 1 - done - rank) * p.states_c + (d + j) * p.states_d] : 0.0f;
     };
+    auto fetch = [&](uint32_t done, uint32_t stage) {
+        if constexpr (SRC == kFromTiles) {
+            const uint32_t t = chunk_start(done);
+            if (threadIdx.x == 0 && t < n) {
+                const uint32_t bar = smem_u32(&full[stage]), to = ring + stage * kStageBytes;
+                mbar_arrive_expect_tx(bar, kStageBytes);
+                tma_load_3d(to, &maps.f, bar, d0, t, b);
+                tma_load_3d(to + Tile::kBytes, &maps.x, bar, d0, t, b);
+                tma_load_3d(to + 2 * Tile::kBytes, &maps.dy, bar, d0, t, b);
+                if constexpr (HAS_I) tma_load_3d(to + 3 * Tile::kBytes, &maps.i, bar, d0, t, b);
+                if constexpr (HAS_O) tma_load_3d(to + (3 + HAS_I) * Tile::kBytes, &maps.o, bar, d0, t, b);
+            }
+        } else if constexpr (SRC == kFromWords) {
+            const uint32_t t0 = chunk_start(done) + warp * kSpanSteps, live = on ? live_from(t0) : 0;
+            qf.fetch(t0, live, stage * kStageBytes);
+            qx.fetch(t0, live, stage * kStageBytes);
+            qy.fetch(t0, live, stage * kStageBytes);
+            if constexpr (HAS_I) qi.fetch(t0, live, stage * kStageBytes);
+            if constexpr (HAS_O) qo.fetch(t0, live, stage * kStageBytes);
+            fetch_commit();
+        }
+    };
+    if constexpr (SRC == kFromTiles) {
+        if (threadIdx.x == 0) {
+            mbar_init(smem_u32(&full[0]), 1);
+            mbar_init(smem_u32(&full[1]), 1);
+            fence_mbar_init();
+        }
+        __syncthreads();
+    }
+    fetch(0, 0);
+    if constexpr (SRC == kFromTiles) fetch(cluster, 1);
+    fetch_state(0);
 
     float carry[VEC];                                       // f_{t+1} dc_{t+1} behind what is left
 #pragma unroll
     for (int j = 0; j < VEC; ++j) carry[j] = p.dlast && on ? p.dlast[b * p.dlast_b + (d + j) * p.dlast_d] : 0.0f;
 
     uint32_t buf = 0;
-    if (chunks > 0) fetch(0, 0);
     for (uint32_t done = 0; done < chunks; done += cluster, buf ^= 1) {
-        const uint32_t t0 = first_step(done), live = live_from(t0);
+        const uint32_t start = chunk_start(done), t0 = start + warp * kSpanSteps, live = live_from(t0);
+        const bool whole = live >= kSpanSteps;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) c[j] = c_next[j];
-        fetch(done + cluster, (buf ^ 1) * kStageBytes);
-        fetch_wait<1>();
+        fetch_state(done + cluster);
+        if constexpr (SRC == kFromWords) {
+            fetch(done + cluster, buf ^ 1);
+            fetch_wait<1>();
+        }
+        if constexpr (SRC == kFromTiles) {
+            if (start < n) waits.wait(buf);
+        }
         Raw rf[kSpanSteps], rx[kSpanSteps], ri[kSpanSteps], ro[kSpanSteps], ry[kSpanSteps];
-        qf.read(t0, live, buf * kStageBytes, L::infinity(), rf);          // 1 - f = 0 where nothing is live
-        qx.read(t0, live, buf * kStageBytes, Raw{}, rx);
-        qy.read(t0, live, buf * kStageBytes, Raw{}, ry);
-        if constexpr (HAS_I) qi.read(t0, live, buf * kStageBytes, Raw{}, ri);
-        if constexpr (HAS_O) qo.read(t0, live, buf * kStageBytes, Raw{}, ro);
+        const uint32_t mem_live = SRC == kFromMemory && !on ? 0 : live;
+        qf.read(t0, mem_live, whole, buf * kStageBytes, L::infinity(), rf);       // 1 - f = 0 where nothing is live
+        qx.read(t0, mem_live, whole, buf * kStageBytes, Raw{}, rx);
+        qy.read(t0, mem_live, whole, buf * kStageBytes, Raw{}, ry);
+        if constexpr (HAS_I) qi.read(t0, mem_live, whole, buf * kStageBytes, Raw{}, ri);
+        if constexpr (HAS_O) qo.read(t0, mem_live, whole, buf * kStageBytes, Raw{}, ro);
         float f[kSpanSteps][VEC], off[kSpanSteps][VEC], dp[kSpanSteps][VEC];
         SpanBoth<VEC> mine;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) mine.a[j] = 1.0f, mine.h[j] = mine.e[j] = 0.0f;
 #pragma unroll
         for (uint32_t s = 0; s < kSpanSteps; ++s) {
-            float vf[VEC], vx[VEC], vi[VEC], vo[VEC];
+            float vf[VEC], vx[VEC], in[VEC];
             L::unpack(rf[s], vf);
             L::unpack(rx[s], vx);
             L::unpack(ry[s], dp[s]);
-            if constexpr (HAS_I) L::unpack(ri[s], vi);
-            if constexpr (HAS_O) L::unpack(ro[s], vo);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const Gate g = logistic_pair(vf[j]);
-                f[s][j] = g.on;
-                off[s][j] = g.off;
-                float in = g.off;
-                if constexpr (HAS_I) in = logistic(vi[j]);
-                mine.h[j] = fmaf(f[s][j], mine.h[j], in * vx[j]);
-                mine.a[j] *= f[s][j];
-                if constexpr (HAS_O) dp[s][j] *= logistic(vo[j]);
+            logistic_pair_to<VEC>(f[s], off[s], vf);
+            if constexpr (HAS_I) {
+                float vi[VEC];
+                L::unpack(ri[s], vi);
+                logistic_to<VEC>(in, vi);
+                mul_to<VEC>(in, in, vx);
+            } else {
+                mul_to<VEC>(in, off[s], vx);
+            }
+            fma_to<VEC>(mine.h, f[s], mine.h, in);
+            mul_to<VEC>(mine.a, mine.a, f[s]);
+            if constexpr (HAS_O) {
+                float vo[VEC];
+                L::unpack(ro[s], vo);
+                logistic_to<VEC>(vo, vo);
+                mul_to<VEC>(dp[s], dp[s], vo);
             }
         }
 #pragma unroll
-        for (int s = kSpanSteps - 1; s >= 0; --s)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) mine.e[j] = f[s][j] * (dp[s][j] + mine.e[j]);
+        for (int s = kSpanSteps - 1; s >= 0; --s) {
+            add_to<VEC>(mine.e, dp[s], mine.e);
+            mul_to<VEC>(mine.e, f[s], mine.e);
+        }
         in_cta[buf][warp][lane] = mine;
         __syncthreads();
+        if constexpr (SRC == kFromTiles) fetch(done + 2 * cluster, buf);          // everyone has read this stage
         if (cluster > 1) {
             if (warp == 0) {
                 Span<VEC> all;
@@ -516,109 +738,130 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, uint
 #pragma unroll
                 for (int w = kSpanWarps - 1; w >= 0; --w) {
                     const SpanBoth<VEC>& s = in_cta[buf][w][lane];
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        all.h[j] = fmaf(s.a[j], all.h[j], s.e[j]);
-                        all.a[j] *= s.a[j];
-                    }
+                    fma_to<VEC>(all.h, s.a, all.h, s.e);
+                    mul_to<VEC>(all.a, all.a, s.a);
                 }
                 for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], r, all);
             }
             cluster_arrive_release();
             cluster_wait_acquire();
         }
-        float e[VEC];
+        float e[VEC], run[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) e[j] = carry[j];
+        for (int j = 0; j < VEC; ++j) run[j] = carry[j];
         if (cluster > 1) {
             for (uint32_t r = 0; r < cluster; ++r) {
                 const Span<VEC> s = in_cluster[buf][r][lane];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    if (r == rank) e[j] = carry[j];
-                    carry[j] = fmaf(s.a[j], carry[j], s.h[j]);
-                }
+                for (int j = 0; j < VEC; ++j)
+                    if (r == rank) run[j] = carry[j];
+                fma_to<VEC>(carry, s.a, carry, s.h);
             }
         }
-        for (uint32_t w = kSpanWarps - 1; w > warp; --w) {
-            const SpanBoth<VEC>& s = in_cta[buf][w][lane];
+        float fore[VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) e[j] = fmaf(s.a[j], e[j], s.e[j]);
+        for (int j = 0; j < VEC; ++j) {
+            e[j] = run[j];
+            fore[j] = c[j];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kSpanWarps; ++k) {
+            const uint32_t w = kSpanWarps - 1 - k;
+            const SpanBoth<VEC>& back = in_cta[buf][w][lane];
+            const SpanBoth<VEC>& forth = in_cta[buf][k][lane];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (w == warp) e[j] = run[j];
+                if (k == warp) c[j] = fore[j];
+            }
+            fma_to<VEC>(run, back.a, run, back.e);
+            if (k + 1 < kSpanWarps) fma_to<VEC>(fore, forth.a, fore, forth.h);
         }
         if (cluster == 1) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) carry[j] = e[j];
-            for (int w = warp; w >= 0; --w) {
-                const SpanBoth<VEC>& s = in_cta[buf][w][lane];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) carry[j] = fmaf(s.a[j], carry[j], s.e[j]);
-            }
-        }
-        for (uint32_t w = 0; w < warp; ++w) {
-            const SpanBoth<VEC>& s = in_cta[buf][w][lane];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) c[j] = fmaf(s.a[j], c[j], s.h[j]);
+            for (int j = 0; j < VEC; ++j) carry[j] = run[j];
         }
         float before[kSpanSteps][VEC];
 #pragma unroll
         for (uint32_t s = 0; s < kSpanSteps; ++s) {
-            float vx[VEC], vi[VEC];
+            float vx[VEC], in[VEC];
             L::unpack(rx[s], vx);
-            if constexpr (HAS_I) L::unpack(ri[s], vi);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                before[s][j] = c[j];
-                float in = off[s][j];
-                if constexpr (HAS_I) in = logistic(vi[j]);
-                c[j] = fmaf(f[s][j], c[j], in * vx[j]);
+            if constexpr (HAS_I) {
+                float vi[VEC];
+                L::unpack(ri[s], vi);
+                logistic_to<VEC>(in, vi);
+                mul_to<VEC>(in, in, vx);
+            } else {
+                mul_to<VEC>(in, off[s], vx);
             }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) before[s][j] = c[j];
+            fma_to<VEC>(c, f[s], c, in);
         }
         const uint32_t there = on && t0 < p.T ? p.T - t0 : 0;
-        const long long top = t0 + kSpanSteps - 1;
-        T* ax = static_cast<T*>(p.dx.p) + b * p.dx.b + d * p.dx.d + top * p.dx.t;
-        T* af = static_cast<T*>(p.df.p) + b * p.df.b + d * p.df.d + top * p.df.t;
-        T* ai = static_cast<T*>(p.di.p) + b * p.di.b + d * p.di.d + top * p.di.t;
-        T* ao = static_cast<T*>(p.dout.p) + b * p.dout.b + d * p.dout.d + top * p.dout.t;
+        const StepWriter<T, VEC, kTileStores> out_x(p.dx, b, d, t0, staging, 0), out_f(p.df, b, d, t0, staging, 1), out_i(p.di, b, d, t0, staging, 2),
+            out_o(p.dout, b, d, t0, staging, 2 + HAS_I);
+        if constexpr (kTileStores) {
+            if (lane == 0) bulk_wait_group_read<0>();
+            __syncwarp();
+        }
 #pragma unroll
-        for (int s = kSpanSteps - 1; s >= 0; --s, ax -= p.dx.t, af -= p.df.t, ai -= p.di.t, ao -= p.dout.t) {
-            float vx[VEC], vi[VEC], vo[VEC], vy[VEC], dx[VEC], df[VEC], di[VEC], dout[VEC];
+        for (int s = kSpanSteps - 1; s >= 0; --s) {
+            float vx[VEC], dx[VEC], df[VEC], di[VEC], dout[VEC], dc[VEC], slope[VEC];
             L::unpack(rx[s], vx);
-            if constexpr (HAS_I) L::unpack(ri[s], vi);
+            add_to<VEC>(dc, dp[s], e);
+            mul_to<VEC>(slope, f[s], off[s]);
+            mul_to<VEC>(slope, slope, dc);
+            if constexpr (HAS_I) {
+                float vi[VEC], in[VEC], closed[VEC];
+                L::unpack(ri[s], vi);
+                logistic_pair_to<VEC>(in, closed, vi);
+                mul_to<VEC>(dx, dc, in);
+                mul_to<VEC>(di, dx, vx);
+                mul_to<VEC>(di, di, closed);
+                mul_to<VEC>(df, slope, before[s]);
+            } else {
+                mul_to<VEC>(dx, dc, off[s]);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) df[j] = before[s][j] - vx[j];
+                mul_to<VEC>(df, df, slope);
+            }
             if constexpr (HAS_O) {
+                float vo[VEC], vy[VEC], closed[VEC];
                 L::unpack(ro[s], vo);
                 L::unpack(ry[s], vy);
+                logistic_pair_to<VEC>(vo, closed, vo);
+                mul_to<VEC>(dout, vy, c);
+                mul_to<VEC>(dout, dout, vo);
+                mul_to<VEC>(dout, dout, closed);
             }
+            mul_to<VEC>(e, f[s], dc);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float dc = dp[s][j] + e[j];
-                const float slope = dc * (f[s][j] * off[s][j]);
-                if constexpr (HAS_I) {
-                    const Gate in = logistic_pair(vi[j]);
-                    dx[j] = dc * in.on;
-                    di[j] = dx[j] * vx[j] * in.off;
-                    df[j] = slope * before[s][j];
-                } else {
-                    dx[j] = dc * off[s][j];
-                    df[j] = slope * (before[s][j] - vx[j]);
-                }
-                if constexpr (HAS_O) {
-                    const Gate out = logistic_pair(vo[j]);
-                    dout[j] = vy[j] * c[j] * out.on * out.off;
-                }
-                e[j] = f[s][j] * dc;
-                c[j] = before[s][j];
-            }
+            for (int j = 0; j < VEC; ++j) c[j] = before[s][j];
             Raw wx = L::pack(dx), wf = L::pack(df), wi{}, wo{};
             if constexpr (HAS_I) wi = L::pack(di);
             if constexpr (HAS_O) wo = L::pack(dout);
-            if (static_cast<uint32_t>(s) >= live) wx = wf = wi = wo = Raw{};
-            if (static_cast<uint32_t>(s) < there) {
-                *reinterpret_cast<Raw*>(ax) = wx;
-                *reinterpret_cast<Raw*>(af) = wf;
-                if constexpr (HAS_I) *reinterpret_cast<Raw*>(ai) = wi;
-                if constexpr (HAS_O) *reinterpret_cast<Raw*>(ao) = wo;
+            if (!whole && static_cast<uint32_t>(s) >= live) wx = wf = wi = wo = Raw{};
+            out_x.put(s, there, wx);
+            out_f.put(s, there, wf);
+            if constexpr (HAS_I) out_i.put(s, there, wi);
+            if constexpr (HAS_O) out_o.put(s, there, wo);
+        }
+        if constexpr (kTileStores) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && t0 < p.T) {
+                const uint32_t from = staging + warp * Tile::kWarpBytes;
+                tma_store_3d(&maps.dx, from, d0, t0, b);
+                tma_store_3d(&maps.df, from + Tile::kBytes, d0, t0, b);
+                if constexpr (HAS_I) tma_store_3d(&maps.di, from + 2 * Tile::kBytes, d0, t0, b);
+                if constexpr (HAS_O) tma_store_3d(&maps.dout, from + (2 + HAS_I) * Tile::kBytes, d0, t0, b);
+                bulk_commit_group();
             }
         }
+    }
+    if constexpr (kTileStores) {
+        if (lane == 0) bulk_wait_group<0>();
     }
     if (p.dinitial && rank == 0 && warp == 0 && on) {
 #pragma unroll

@@ -3,6 +3,7 @@
 #pragma once
 #include "srt_matmul_api.h"
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -77,6 +78,18 @@ inline uint32_t elem_size(srtDataType t)
     default: return 0;
     }
 }
+
+// What kernels with TMA loads need from the host: the driver's tensor-map encoder, the status word of the device (which is current)
+// and the limit of a wait in SM cycles.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+struct TileServices {
+    EncodeTiledFn encode;
+    uint32_t* status;
+    unsigned long long wait_cycles;
+};
+cudaError_t tile_services(int device, TileServices& out);
 
 }  // namespace host
 }  // namespace srt

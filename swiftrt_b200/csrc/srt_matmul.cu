@@ -220,9 +220,6 @@ struct DeviceInfo {
 std::mutex g_mutex;
 DeviceInfo g_devices[64];
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn g_encode = nullptr;
 
 cudaError_t device_info(int dev, DeviceInfo& out)
@@ -1792,6 +1789,31 @@ cudaError_t launch_gate_backward(const GateBackwardParams& gp, bool vec, cudaStr
 }
 
 }  // namespace
+
+// ------------------------------------------------------------------ services for the other translation units
+namespace srt {
+namespace host {
+
+cudaError_t tile_services(int device, TileServices& out)
+{
+    static std::atomic<uint32_t*> status[64];
+    DeviceInfo info;
+    cudaError_t e = device_info(device, info);
+    if (e != cudaSuccess) return e;
+    if (!info.sm100) return fail(cudaErrorNotSupported, "this library is built for sm_100a devices only");
+    uint32_t* word = status[device].load(std::memory_order_acquire);
+    if (!word) {
+        void* ptr = nullptr;
+        if ((e = cudaGetSymbolAddress(&ptr, g_gemm_status)) != cudaSuccess) return e;
+        word = static_cast<uint32_t*>(ptr);
+        status[device].store(word, std::memory_order_release);
+    }
+    out = TileServices{g_encode, word, g_wait_limit_ns.load(std::memory_order_relaxed) * 2};
+    return cudaSuccess;
+}
+
+}  // namespace host
+}  // namespace srt
 
 // ===================================================================== exported entry points
 extern "C" {

@@ -109,8 +109,9 @@ cudaError_t recurrence_shape(const char* op, const srtTensorDescriptor* updateDe
     return cudaSuccess;
 }
 
-template <typename Kernel>
-cudaError_t launch_spans_kernel(Kernel kernel, std::atomic<int>* resident, uint32_t smem, const RecurrenceParams& p, uint32_t channels, cudaStream_t stream)
+template <typename Kernel, typename Maps>
+cudaError_t launch_spans_kernel(Kernel kernel, const Maps& maps, std::atomic<int>* resident, uint32_t smem, const RecurrenceParams& p, uint32_t channels,
+                                cudaStream_t stream)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -147,30 +148,60 @@ cudaError_t launch_spans_kernel(Kernel kernel, std::atomic<int>* resident, uint3
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p, blocks_d, cluster);
+    return cudaLaunchKernelEx(&cfg, kernel, p, maps, blocks_d, cluster);
 }
 
-template <typename T, bool HAS_I, bool HAS_O, int VEC>
-cudaError_t launch_spans(const RecurrenceParams& p, bool backward, cudaStream_t stream)
+template <typename T, bool HAS_I, bool HAS_O, int VEC, int SRC>
+cudaError_t launch_spans(const RecurrenceParams& p, const typename MapsOf<SRC>::type& maps, bool backward, cudaStream_t stream)
 {
     static std::atomic<int> resident[2][64];
     constexpr uint32_t kInputs = 2 + HAS_I + HAS_O;
-    return backward ? launch_spans_kernel(recurrence_span_backward_kernel<T, HAS_I, HAS_O, VEC>, resident[1], span_smem_bytes<T, VEC>(kInputs + 1), p, 32 * VEC, stream)
-                    : launch_spans_kernel(recurrence_span_kernel<T, HAS_I, HAS_O, VEC>, resident[0], span_smem_bytes<T, VEC>(kInputs), p, 32 * VEC, stream);
+    return backward ? launch_spans_kernel(recurrence_span_backward_kernel<T, HAS_I, HAS_O, VEC, SRC>, maps, resident[1],
+                                          span_smem_bytes<T, VEC, SRC>(kInputs + 1, kInputs), p, 32 * VEC, stream)
+                    : launch_spans_kernel(recurrence_span_kernel<T, HAS_I, HAS_O, VEC, SRC>, maps, resident[0],
+                                          span_smem_bytes<T, VEC, SRC>(kInputs, 1), p, 32 * VEC, stream);
 }
 
-template <typename T, int VEC>
-cudaError_t launch_spans_gates(const RecurrenceParams& p, bool backward, cudaStream_t stream)
+template <typename T, int VEC, int SRC>
+cudaError_t launch_spans_gates(const RecurrenceParams& p, const typename MapsOf<SRC>::type& maps, bool backward, cudaStream_t stream)
 {
-    if (p.i.p) return p.o.p ? launch_spans<T, true, true, VEC>(p, backward, stream) : launch_spans<T, true, false, VEC>(p, backward, stream);
-    return p.o.p ? launch_spans<T, false, true, VEC>(p, backward, stream) : launch_spans<T, false, false, VEC>(p, backward, stream);
+    if (p.i.p) return p.o.p ? launch_spans<T, true, true, VEC, SRC>(p, maps, backward, stream) : launch_spans<T, true, false, VEC, SRC>(p, maps, backward, stream);
+    return p.o.p ? launch_spans<T, false, true, VEC, SRC>(p, maps, backward, stream) : launch_spans<T, false, false, VEC, SRC>(p, maps, backward, stream);
+}
+
+template <typename T> constexpr CUtensorMapDataType kMapType = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+template <> constexpr CUtensorMapDataType kMapType<__half> = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+template <> constexpr CUtensorMapDataType kMapType<__nv_bfloat16> = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+
+// Tensor maps of every tensor of the call, boxes of 128 bytes of channels by 64 steps (inputs) or 8 steps (results); false when one
+// cannot have it: rows that do not start on 16 bytes, channels apart from each other, repeated or overlapping rows.
+template <typename T>
+bool encode_maps(const RecurrenceParams& p, EncodeTiledFn encode, RecurrenceMaps& maps)
+{
+    auto one = [&](const void* ptr, long long b, long long t, long long d, uint32_t steps, CUtensorMap* map) {
+        if (!ptr) return true;
+        const long long elem = sizeof(T);
+        if (p.T == 1) t = (long long)(p.D + 7) / 8 * 8;
+        if (p.B == 1) b = t;
+        if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0 || (d != 1 && p.D > 1) || t < (long long)p.D || b <= 0 || t * elem % 16 != 0 || b * elem % 16 != 0 ||
+            t * elem >= (1ll << 40) || b * elem >= (1ll << 40))
+            return false;
+        const cuuint64_t dims[3] = {p.D, p.T, p.B}, strides[2] = {(cuuint64_t)(t * elem), (cuuint64_t)(b * elem)};
+        const cuuint32_t box[3] = {(cuuint32_t)(128 / elem), steps, 1}, unit[3] = {1, 1, 1};
+        return encode(map, kMapType<T>, 3, const_cast<void*>(ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    auto in = [&](const Strided3& s, CUtensorMap* map) { return one(s.p, s.b, s.t, s.d, kRecurrenceChunk, map); };
+    auto out = [&](const Strided3W& s, CUtensorMap* map) { return one(s.p, s.b, s.t, s.d, kSpanSteps, map); };
+    return in(p.f, &maps.f) && in(p.x, &maps.x) && in(p.i, &maps.i) && in(p.o, &maps.o) && in(p.dy, &maps.dy) && out(p.y, &maps.y) && out(p.dx, &maps.dx) &&
+           out(p.df, &maps.df) && out(p.di, &maps.di) && out(p.dout, &maps.dout);
 }
 
 // up to this many steps one thread walks a channel
 constexpr uint32_t kFewSteps = 8;
 
 template <typename T>
-cudaError_t launch_recurrence(const RecurrenceParams& p, bool backward, cudaStream_t stream)
+cudaError_t launch_recurrence(RecurrenceParams& p, bool backward, int device, cudaStream_t stream)
 {
     cudaError_t e;
     if (p.T <= kFewSteps) {
@@ -180,6 +211,12 @@ cudaError_t launch_recurrence(const RecurrenceParams& p, bool backward, cudaStre
         else          recurrence_steps_kernel<T><<<blocks, 128, 0, stream>>>(p);
         e = cudaGetLastError();
     } else {
+        TileServices services;
+        if ((e = tile_services(device, services)) != cudaSuccess) return e;
+        p.status = services.status;
+        p.wait_cycles = services.wait_cycles;
+        RecurrenceMaps maps;
+        memset(&maps, 0, sizeof maps);
         // two channels per access where every tensor has them side by side and aligned
         bool pairs = p.D % 2 == 0;
         auto look = [&](const void* ptr, long long b, long long t, long long d) {
@@ -187,18 +224,21 @@ cudaError_t launch_recurrence(const RecurrenceParams& p, bool backward, cudaStre
         };
         for (const Strided3* s : {&p.x, &p.f, &p.i, &p.o, &p.dy}) look(s->p, s->b, s->t, s->d);
         for (const Strided3W* s : {&p.y, &p.dx, &p.df, &p.di, &p.dout}) look(s->p, s->b, s->t, s->d);
-        e = pairs ? launch_spans_gates<T, 2>(p, backward, stream) : launch_spans_gates<T, 1>(p, backward, stream);
+        constexpr int kTileVec = sizeof(T) == 2 ? 2 : 1, kOddSource = sizeof(T) == 2 ? kFromMemory : kFromWords;
+        if (encode_maps<T>(p, services.encode, maps)) e = launch_spans_gates<T, kTileVec, kFromTiles>(p, maps, backward, stream);
+        else if (pairs) e = launch_spans_gates<T, 2, kFromWords>(p, NoMaps{}, backward, stream);
+        else e = launch_spans_gates<T, 1, kOddSource>(p, NoMaps{}, backward, stream);
     }
     if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;
 }
 
-cudaError_t launch_recurrence_type(srtDataType type, const RecurrenceParams& p, bool backward, cudaStream_t stream)
+cudaError_t launch_recurrence_type(srtDataType type, RecurrenceParams& p, bool backward, int device, cudaStream_t stream)
 {
     switch (type) {
-    case real32F: return launch_recurrence<float>(p, backward, stream);
-    case real16F: return launch_recurrence<__half>(p, backward, stream);
-    default: return launch_recurrence<__nv_bfloat16>(p, backward, stream);
+    case real32F: return launch_recurrence<float>(p, backward, device, stream);
+    case real16F: return launch_recurrence<__half>(p, backward, device, stream);
+    default: return launch_recurrence<__nv_bfloat16>(p, backward, device, stream);
     }
 }
 
@@ -234,7 +274,7 @@ cudaError_t srtGatedRecurrence(const void* update, const srtTensorDescriptor* up
     p.states = static_cast<float*>(states);
     DeviceScope scope(stream);
     if (scope.status != cudaSuccess) return scope.status;
-    return launch_recurrence_type(type, p, false, stream);
+    return launch_recurrence_type(type, p, false, scope.device, stream);
 }
 
 cudaError_t srtGatedRecurrenceBackward(const void* outGrad, const srtTensorDescriptor* outGradDesc, const void* lastGrad, const srtTensorDescriptor* lastGradDesc,
@@ -272,7 +312,7 @@ cudaError_t srtGatedRecurrenceBackward(const void* outGrad, const srtTensorDescr
     p.dinitial = static_cast<float*>(dInitial);
     DeviceScope scope(stream);
     if (scope.status != cudaSuccess) return scope.status;
-    return launch_recurrence_type(type, p, true, stream);
+    return launch_recurrence_type(type, p, true, scope.device, stream);
 }
 
 }  // extern "C"

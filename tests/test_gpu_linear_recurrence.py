@@ -273,3 +273,24 @@ def test_layer_trains_and_generates_like_its_definition(srt):
             assert float((token.double().cpu() - want[:, t].detach()).norm() / want[:, t].detach().norm()) <= 2e-5
         assert float((moving - last).norm() / last.norm()) <= 2e-5
         assert torch.equal(cell(x, state)[0], hidden)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_a_wait_that_runs_out_is_reported_and_ends_in_order(srt, dtype):
+    """A limit of one nanosecond on the waits for the tiles of a long sequence: the status word says so, the kernel ends, and
+    the same calls with the default limit give what they gave before."""
+    tensors = _make(2, 700, 256, TYPES[dtype], False, True)
+    dy = torch.randn(2, 700, 256, device=DEV).to(TYPES[dtype])
+    both = lambda: (r := srt.gated_recurrence(*tensors, keep=True), srt.gated_recurrence_backward(dy, *tensors, r[2]))  # noqa: E731
+    want = both()
+    assert srt.check_status() == 0
+    try:
+        srt.set_wait_limit(1)
+        both()
+        assert srt.check_status() != 0
+    finally:
+        srt.set_wait_limit(0)
+    got = both()
+    assert srt.check_status() == 0
+    for a, b in zip(want[0] + want[1], got[0] + got[1]):
+        assert a is b is None or torch.equal(a, b)

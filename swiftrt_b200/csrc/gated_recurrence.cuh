@@ -381,23 +381,27 @@ struct StepWriter {
 // a float2 (VEC = 2) or float per lane and quantity, in shared memory of any CTA of the cluster
 template <int VEC> struct Span { float a[VEC], h[VEC]; };
 
-template <int VEC> __device__ __forceinline__ void span_to_cta(const Span<VEC>* local, uint32_t rank, const Span<VEC>& s)
+// `s` to the same place in the shared memory of CTA `rank`, counted there on its barrier: no fence and no barrier of the whole
+// cluster, which would wait for the results' stores as well
+template <int VEC> __device__ __forceinline__ void span_to_cta(const Span<VEC>* local, uint32_t bar, uint32_t rank, const Span<VEC>& s)
 {
-    const uint32_t at = map_to_cta(smem_u32(local), rank);
+    const uint32_t at = map_to_cta(smem_u32(local), rank), done = map_to_cta(bar, rank);
     if constexpr (VEC == 2)
-        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(s.a[0]), "f"(s.a[1]), "f"(s.h[0]), "f"(s.h[1]) : "memory");
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                     ::"r"(at), "r"(__float_as_uint(s.a[0])), "r"(__float_as_uint(s.a[1])), "r"(__float_as_uint(s.h[0])), "r"(__float_as_uint(s.h[1])), "r"(done) : "memory");
     else
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(s.a[0]), "f"(s.h[0]) : "memory");
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];"
+                     ::"r"(at), "r"(__float_as_uint(s.a[0])), "r"(__float_as_uint(s.h[0])), "r"(done) : "memory");
 }
 
-// What a kFromTiles CTA waits with.  A wait that runs over the limit is noted in the status word (the result of the launch is
-// invalid then); the thread still waits, as long again as kDrainCycles allows, for the copies to land before it goes on.
-constexpr uint64_t kTileDrainCycles = 4000000000ull;
-struct TileWaits {
-    uint32_t bars;                       // one mbarrier per stage
+// Bounded waits on a pair of barriers: for the tiles of a stage, or for the spans of the cluster's CTAs.  A wait that runs over the limit is noted in the status word (the result of the launch is
+// invalid then); the thread still waits, up to kDrainLimitCycles longer, for what is on its way before it goes on.
+constexpr uint64_t kDrainLimitCycles = 4000000000ull;
+struct PhaseWaits {
+    uint32_t bars;                       // two mbarriers
     uint32_t* status;
     uint64_t limit;
-    uint32_t phases = 0;                 // bit s: parity of stage s's next wait
+    uint32_t phases = 0;                 // bit s: parity of the next wait on barrier s
     bool dead = false;
     __device__ __forceinline__ void wait(uint32_t stage)
     {
@@ -405,7 +409,7 @@ struct TileWaits {
         phases ^= 1u << stage;
         if (dead || mbar_test_wait(bars + 8 * stage, parity)) return;
         const uint64_t t0 = sm_clock();
-        while (!mbar_try_wait(bars + 8 * stage, parity) && !dead) dead = sm_clock() - t0 > limit + kTileDrainCycles;
+        while (!mbar_try_wait(bars + 8 * stage, parity) && !dead) dead = sm_clock() - t0 > limit + kDrainLimitCycles;
         if (sm_clock() - t0 > limit) atomicOr(status, 1u);
     }
 };
@@ -421,7 +425,7 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
     extern __shared__ __align__(128) uint8_t dynamic_smem[];
     __shared__ alignas(16) Span<VEC> in_cta[2][kSpanWarps][32];
     __shared__ alignas(16) Span<VEC> in_cluster[2][8][32];
-    __shared__ alignas(8) uint64_t full[kSpanStages];
+    __shared__ alignas(8) uint64_t full[kSpanStages], arrived[2];
     const uint32_t ring = SRC == kFromTiles ? (smem_u32(dynamic_smem) + 127u) & ~127u : smem_u32(dynamic_smem);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster > 1 ? cluster_ctarank() : 0;
@@ -431,7 +435,7 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
     const uint32_t n = live_steps(p, b);
     const uint32_t chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
     const StepReader<T, VEC, SRC> qf(p.f, b, d, ring, 0), qx(p.x, b, d, ring, 1), qi(p.i, b, d, ring, 2), qo(p.o, b, d, ring, 2 + HAS_I);
-    TileWaits waits{smem_u32(full), p.status, p.wait_cycles};
+    PhaseWaits waits{smem_u32(full), p.status, p.wait_cycles}, arrivals{smem_u32(arrived), p.status, p.wait_cycles};
     // this thread's first step of chunk k, and how many of its 8 belong to the sequence
     auto first_step = [&](uint32_t k) { return (k + rank) * kRecurrenceChunk + warp * kSpanSteps; };
     auto live_from = [&](uint32_t t0) { return t0 < n ? n - t0 : 0u; };
@@ -455,12 +459,17 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
             fetch_commit();
         }
     };
-    if constexpr (SRC == kFromTiles) {
-        if (threadIdx.x == 0) {
-            mbar_init(smem_u32(&full[0]), 1);
-            mbar_init(smem_u32(&full[1]), 1);
-            fence_mbar_init();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&full[i]), 1);
+            mbar_init(smem_u32(&arrived[i]), 1);
         }
+        fence_mbar_init();
+    }
+    if (cluster > 1) {
+        cluster_arrive_release();                                 // before anyone sends to a barrier
+        cluster_wait_acquire();
+    } else {
         __syncthreads();
     }
     fetch(0, 0);
@@ -522,10 +531,10 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
                     fma_to<VEC>(all.h, next.a, all.h, next.h);
                     mul_to<VEC>(all.a, all.a, next.a);
                 }
-                for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], r, all);
+                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&arrived[buf]), cluster * 32 * static_cast<uint32_t>(sizeof(Span<VEC>)));
+                for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], smem_u32(&arrived[buf]), r, all);
             }
-            cluster_arrive_release();
-            cluster_wait_acquire();
+            arrivals.wait(buf);
         }
         // the state before this CTA's span, before this warp's steps, and behind the whole cluster's span
         float c[VEC], begin[VEC], run[VEC];
@@ -614,7 +623,7 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
     extern __shared__ __align__(128) uint8_t dynamic_smem[];
     __shared__ SpanBoth<VEC> in_cta[2][kSpanWarps][32];
     __shared__ alignas(16) Span<VEC> in_cluster[2][8][32];
-    __shared__ alignas(8) uint64_t full[kSpanStages];
+    __shared__ alignas(8) uint64_t full[kSpanStages], arrived[2];
     const uint32_t ring = SRC == kFromTiles ? (smem_u32(dynamic_smem) + 127u) & ~127u : smem_u32(dynamic_smem);
     const uint32_t staging = ring + kSpanStages * kStageBytes;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -625,7 +634,7 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
     const uint32_t n = live_steps(p, b);
     const uint32_t chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
     const StepReader<T, VEC, SRC> qf(p.f, b, d, ring, 0), qx(p.x, b, d, ring, 1), qy(p.dy, b, d, ring, 2), qi(p.i, b, d, ring, 3), qo(p.o, b, d, ring, 3 + HAS_I);
-    TileWaits waits{smem_u32(full), p.status, p.wait_cycles};
+    PhaseWaits waits{smem_u32(full), p.status, p.wait_cycles}, arrivals{smem_u32(arrived), p.status, p.wait_cycles};
     // after `done` chunks from the end this CTA has chunk chunks - 1 - done - rank, if that is one
     auto chunk_start = [&](uint32_t done) { return done + rank < chunks ? (chunks - 1 - done - rank) * kRecurrenceChunk : p.T; };
     auto live_from = [&](uint32_t t0) { return t0 < n ? n - t0 : 0u; };
@@ -657,12 +666,17 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
             fetch_commit();
         }
     };
-    if constexpr (SRC == kFromTiles) {
-        if (threadIdx.x == 0) {
-            mbar_init(smem_u32(&full[0]), 1);
-            mbar_init(smem_u32(&full[1]), 1);
-            fence_mbar_init();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&full[i]), 1);
+            mbar_init(smem_u32(&arrived[i]), 1);
         }
+        fence_mbar_init();
+    }
+    if (cluster > 1) {
+        cluster_arrive_release();                                 // before anyone sends to a barrier
+        cluster_wait_acquire();
+    } else {
         __syncthreads();
     }
     fetch(0, 0);
@@ -741,10 +755,10 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
                     fma_to<VEC>(all.h, s.a, all.h, s.e);
                     mul_to<VEC>(all.a, all.a, s.a);
                 }
-                for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], r, all);
+                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&arrived[buf]), cluster * 32 * static_cast<uint32_t>(sizeof(Span<VEC>)));
+                for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], smem_u32(&arrived[buf]), r, all);
             }
-            cluster_arrive_release();
-            cluster_wait_acquire();
+            arrivals.wait(buf);
         }
         float e[VEC], run[VEC];
 #pragma unroll

@@ -795,6 +795,14 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
 #pragma unroll
             for (int j = 0; j < VEC; ++j) carry[j] = run[j];
         }
+        const uint32_t there = on && t0 < p.T ? p.T - t0 : 0;
+        const StepWriter<T, VEC, kTileStores> out_x(p.dx, b, d, t0, staging, 0), out_f(p.df, b, d, t0, staging, 1), out_i(p.di, b, d, t0, staging, 2),
+            out_o(p.dout, b, d, t0, staging, 2 + HAS_I);
+        if constexpr (kTileStores) {
+            if (lane == 0) bulk_wait_group_read<0>();
+            __syncwarp();
+        }
+        // the states, and the output gate's gradient, which needs nothing else: its operands make room for the states
         float before[kSpanSteps][VEC];
 #pragma unroll
         for (uint32_t s = 0; s < kSpanSteps; ++s) {
@@ -811,17 +819,22 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
 #pragma unroll
             for (int j = 0; j < VEC; ++j) before[s][j] = c[j];
             fma_to<VEC>(c, f[s], c, in);
-        }
-        const uint32_t there = on && t0 < p.T ? p.T - t0 : 0;
-        const StepWriter<T, VEC, kTileStores> out_x(p.dx, b, d, t0, staging, 0), out_f(p.df, b, d, t0, staging, 1), out_i(p.di, b, d, t0, staging, 2),
-            out_o(p.dout, b, d, t0, staging, 2 + HAS_I);
-        if constexpr (kTileStores) {
-            if (lane == 0) bulk_wait_group_read<0>();
-            __syncwarp();
+            if constexpr (HAS_O) {
+                float vo[VEC], dout[VEC], closed[VEC];
+                L::unpack(ro[s], vo);
+                L::unpack(ry[s], dout);
+                logistic_pair_to<VEC>(vo, closed, vo);
+                mul_to<VEC>(dout, dout, c);
+                mul_to<VEC>(dout, dout, vo);
+                mul_to<VEC>(dout, dout, closed);
+                Raw wo = L::pack(dout);
+                if (!whole && s >= live) wo = Raw{};
+                out_o.put(s, there, wo);
+            }
         }
 #pragma unroll
         for (int s = kSpanSteps - 1; s >= 0; --s) {
-            float vx[VEC], dx[VEC], df[VEC], di[VEC], dout[VEC], dc[VEC], slope[VEC];
+            float vx[VEC], dx[VEC], df[VEC], di[VEC], dc[VEC], slope[VEC];
             L::unpack(rx[s], vx);
             add_to<VEC>(dc, dp[s], e);
             mul_to<VEC>(slope, f[s], off[s]);
@@ -840,26 +853,13 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
                 for (int j = 0; j < VEC; ++j) df[j] = before[s][j] - vx[j];
                 mul_to<VEC>(df, df, slope);
             }
-            if constexpr (HAS_O) {
-                float vo[VEC], vy[VEC], closed[VEC];
-                L::unpack(ro[s], vo);
-                L::unpack(ry[s], vy);
-                logistic_pair_to<VEC>(vo, closed, vo);
-                mul_to<VEC>(dout, vy, c);
-                mul_to<VEC>(dout, dout, vo);
-                mul_to<VEC>(dout, dout, closed);
-            }
             mul_to<VEC>(e, f[s], dc);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) c[j] = before[s][j];
-            Raw wx = L::pack(dx), wf = L::pack(df), wi{}, wo{};
+            Raw wx = L::pack(dx), wf = L::pack(df), wi{};
             if constexpr (HAS_I) wi = L::pack(di);
-            if constexpr (HAS_O) wo = L::pack(dout);
-            if (!whole && static_cast<uint32_t>(s) >= live) wx = wf = wi = wo = Raw{};
+            if (!whole && static_cast<uint32_t>(s) >= live) wx = wf = wi = Raw{};
             out_x.put(s, there, wx);
             out_f.put(s, there, wf);
             if constexpr (HAS_I) out_i.put(s, there, wi);
-            if constexpr (HAS_O) out_o.put(s, there, wo);
         }
         if constexpr (kTileStores) {
             fence_proxy_async_smem();

@@ -110,30 +110,25 @@ cudaError_t recurrence_shape(const char* op, const srtTensorDescriptor* updateDe
 }
 
 template <typename Kernel, typename Maps>
-cudaError_t launch_spans_kernel(Kernel kernel, const Maps& maps, std::atomic<int>* resident, uint32_t smem, const RecurrenceParams& p, uint32_t channels,
+cudaError_t launch_spans_kernel(Kernel kernel, const Maps& maps, std::atomic<uint64_t>* ready, uint32_t smem, const RecurrenceParams& p, uint32_t channels,
                                 cudaStream_t stream)
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    // CTAs an SM holds, asked once per kernel and device
-    int per_sm = resident[dev & 63].load(std::memory_order_acquire);
-    if (per_sm == 0) {
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(ready->load(std::memory_order_acquire) & bit)) {            // once per kernel and device
         if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return e;
-        if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kSpanThreads, smem)) != cudaSuccess) return e;
-        if (per_sm < 1) return cudaErrorLaunchOutOfResources;
-        resident[dev & 63].store(per_sm, std::memory_order_release);
+        ready->fetch_or(bit, std::memory_order_release);
     }
     const uint32_t blocks_d = (p.D + channels - 1) / channels, chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
-    const uint64_t blocks = (uint64_t)p.B * blocks_d, room = 148ull * (uint64_t)per_sm;
-    // spans of one item and channel block side by side: the cluster that leaves the fewest rounds of resident CTAs, in
-    // units of one CTA's whole sequence (512 blocks with 444 places: two rounds alone, five rounds of an eighth with 8)
+    const uint64_t blocks = (uint64_t)p.B * blocks_d;
+    // Spans of one item and channel block side by side until there are CTAs for most places: each CTA then goes through a
+    // longer part of its sequence, which hides its start, and exchanges with fewer.  Forward of 2048 steps, 4096
+    // channels, 1 / 2 / 4 / 8 CTAs a cluster: 4 items (256 blocks) 63 / 79 / 76 / 86 us; 8191 steps of one item (64 blocks) 172 /
+    // 127 / 84 / 95 us; 1024 channels of one item (16 blocks) 45 / 34 / 24 / 24 us.
     uint32_t cluster = 1;
-    double best = 1e300;
-    for (uint32_t c = 1; c <= 8 && c < 2 * chunks; c *= 2) {
-        const double rounds = (double)((blocks * c + room - 1) / room) * ((chunks + c - 1) / c);
-        if (rounds < best * 0.97) { best = rounds; cluster = c; }
-    }
+    while (cluster < 8 && blocks * cluster < 192 && cluster < chunks) cluster *= 2;
     if (blocks * cluster > 0x7fffffffull) return fail(cudaErrorInvalidValue, "too many channels for one call");
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
@@ -154,11 +149,11 @@ cudaError_t launch_spans_kernel(Kernel kernel, const Maps& maps, std::atomic<int
 template <typename T, bool HAS_I, bool HAS_O, int VEC, int SRC>
 cudaError_t launch_spans(const RecurrenceParams& p, const typename MapsOf<SRC>::type& maps, bool backward, cudaStream_t stream)
 {
-    static std::atomic<int> resident[2][64];
+    static std::atomic<uint64_t> ready[2];
     constexpr uint32_t kInputs = 2 + HAS_I + HAS_O;
-    return backward ? launch_spans_kernel(recurrence_span_backward_kernel<T, HAS_I, HAS_O, VEC, SRC>, maps, resident[1],
+    return backward ? launch_spans_kernel(recurrence_span_backward_kernel<T, HAS_I, HAS_O, VEC, SRC>, maps, &ready[1],
                                           span_smem_bytes<T, VEC, SRC>(kInputs + 1, kInputs), p, 32 * VEC, stream)
-                    : launch_spans_kernel(recurrence_span_kernel<T, HAS_I, HAS_O, VEC, SRC>, maps, resident[0],
+                    : launch_spans_kernel(recurrence_span_kernel<T, HAS_I, HAS_O, VEC, SRC>, maps, &ready[0],
                                           span_smem_bytes<T, VEC, SRC>(kInputs, 1), p, 32 * VEC, stream);
 }
 

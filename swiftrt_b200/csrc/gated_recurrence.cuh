@@ -328,6 +328,12 @@ struct StepReader {
         for (uint32_t k = 0; k < kSpanSteps; ++k, from += stride)
             if (k < live) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at + stage_bytes + k * Tile::kRow), "l"(from), "n"(sizeof(Raw)) : "memory");
     }
+    // step k again, from the stage (behind the sequence: whatever is there)
+    __device__ __forceinline__ Raw again(uint32_t k, uint32_t stage_bytes, const Raw (&kept)[kSpanSteps]) const
+    {
+        if constexpr (SRC == kFromMemory) return kept[k];
+        else return shared_word<Raw>(at + stage_bytes + k * Tile::kRow);
+    }
     // steps at or behind `live` read as `other`; whole: none of them is (uniform over the warp)
     __device__ __forceinline__ void read(uint32_t t0, uint32_t live, bool whole, uint32_t stage_bytes, Raw other, Raw (&v)[kSpanSteps]) const
     {
@@ -691,6 +697,7 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
     for (uint32_t done = 0; done < chunks; done += cluster, buf ^= 1) {
         const uint32_t start = chunk_start(done), t0 = start + warp * kSpanSteps, live = live_from(t0);
         const bool whole = live >= kSpanSteps;
+        const uint32_t stage = buf * kStageBytes;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) c[j] = c_next[j];
         fetch_state(done + cluster);
@@ -743,7 +750,10 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
         }
         in_cta[buf][warp][lane] = mine;
         __syncthreads();
-        if constexpr (SRC == kFromTiles) fetch(done + 2 * cluster, buf);          // everyone has read this stage
+        // everyone is done with the other stage: this one is read again below, so that its elements need no registers meanwhile
+        if constexpr (SRC == kFromTiles) {
+            if (done > 0) fetch(done + cluster, buf ^ 1);
+        }
         if (cluster > 1) {
             if (warp == 0) {
                 Span<VEC> all;
@@ -807,10 +817,15 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
 #pragma unroll
         for (uint32_t s = 0; s < kSpanSteps; ++s) {
             float vx[VEC], in[VEC];
-            L::unpack(rx[s], vx);
+            const bool dead = !whole && s >= live;
+            Raw wx = qx.again(s, stage, rx);
+            if (dead) wx = Raw{};
+            L::unpack(wx, vx);
             if constexpr (HAS_I) {
                 float vi[VEC];
-                L::unpack(ri[s], vi);
+                Raw wi = qi.again(s, stage, ri);
+                if (dead) wi = Raw{};
+                L::unpack(wi, vi);
                 logistic_to<VEC>(in, vi);
                 mul_to<VEC>(in, in, vx);
             } else {
@@ -821,27 +836,28 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
             fma_to<VEC>(c, f[s], c, in);
             if constexpr (HAS_O) {
                 float vo[VEC], dout[VEC], closed[VEC];
-                L::unpack(ro[s], vo);
-                L::unpack(ry[s], dout);
+                L::unpack(qo.again(s, stage, ro), vo);
+                L::unpack(qy.again(s, stage, ry), dout);
                 logistic_pair_to<VEC>(vo, closed, vo);
                 mul_to<VEC>(dout, dout, c);
                 mul_to<VEC>(dout, dout, vo);
                 mul_to<VEC>(dout, dout, closed);
                 Raw wo = L::pack(dout);
-                if (!whole && s >= live) wo = Raw{};
+                if (dead) wo = Raw{};
                 out_o.put(s, there, wo);
             }
         }
 #pragma unroll
         for (int s = kSpanSteps - 1; s >= 0; --s) {
             float vx[VEC], dx[VEC], df[VEC], di[VEC], dc[VEC], slope[VEC];
-            L::unpack(rx[s], vx);
+            const bool dead = !whole && static_cast<uint32_t>(s) >= live;
+            L::unpack(qx.again(s, stage, rx), vx);
             add_to<VEC>(dc, dp[s], e);
             mul_to<VEC>(slope, f[s], off[s]);
             mul_to<VEC>(slope, slope, dc);
             if constexpr (HAS_I) {
                 float vi[VEC], in[VEC], closed[VEC];
-                L::unpack(ri[s], vi);
+                L::unpack(qi.again(s, stage, ri), vi);
                 logistic_pair_to<VEC>(in, closed, vi);
                 mul_to<VEC>(dx, dc, in);
                 mul_to<VEC>(di, dx, vx);
@@ -856,7 +872,7 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
             mul_to<VEC>(e, f[s], dc);
             Raw wx = L::pack(dx), wf = L::pack(df), wi{};
             if constexpr (HAS_I) wi = L::pack(di);
-            if (!whole && static_cast<uint32_t>(s) >= live) wx = wf = wi = Raw{};
+            if (dead) wx = wf = wi = Raw{};
             out_x.put(s, there, wx);
             out_f.put(s, there, wf);
             if constexpr (HAS_I) out_i.put(s, there, wi);

@@ -528,25 +528,30 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
         in_cta[buf][warp][lane] = mine;
         __syncthreads();
         if constexpr (SRC == kFromTiles) fetch(first + 2 * cluster, buf);         // everyone has read this stage
-        if (cluster > 1) {
-            if (warp == 0) {
-                Span<VEC> all = mine;
+        // this CTA's spans in order: `whole_span` all of them, `ahead` those before this warp's
+        Span<VEC> whole_span, ahead;
 #pragma unroll
-                for (uint32_t w = 1; w < kSpanWarps; ++w) {
-                    const Span<VEC> next = in_cta[buf][w][lane];
-                    fma_to<VEC>(all.h, next.a, all.h, next.h);
-                    mul_to<VEC>(all.a, all.a, next.a);
-                }
-                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&arrived[buf]), cluster * 32 * static_cast<uint32_t>(sizeof(Span<VEC>)));
-                for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], smem_u32(&arrived[buf]), r, all);
-            }
-            arrivals.wait(buf);
+        for (int j = 0; j < VEC; ++j) {
+            whole_span.a[j] = ahead.a[j] = 1.0f;
+            whole_span.h[j] = ahead.h[j] = 0.0f;
+        }
+#pragma unroll
+        for (uint32_t w = 0; w < kSpanWarps; ++w) {
+            const Span<VEC> s = in_cta[buf][w][lane];
+            if (w == warp) ahead = whole_span;
+            fma_to<VEC>(whole_span.h, s.a, whole_span.h, s.h);
+            mul_to<VEC>(whole_span.a, whole_span.a, s.a);
         }
         // the state before this CTA's span, before this warp's steps, and behind the whole cluster's span
-        float c[VEC], begin[VEC], run[VEC];
+        float c[VEC], begin[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) begin[j] = state[j];
         if (cluster > 1) {
+            if (warp == 0) {
+                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&arrived[buf]), cluster * 32 * static_cast<uint32_t>(sizeof(Span<VEC>)));
+                for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], smem_u32(&arrived[buf]), r, whole_span);
+            }
+            arrivals.wait(buf);
             for (uint32_t r = 0; r < cluster; ++r) {
                 const Span<VEC> s = in_cluster[buf][r][lane];
 #pragma unroll
@@ -554,21 +559,10 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
                     if (r == rank) begin[j] = state[j];
                 fma_to<VEC>(state, s.a, state, s.h);
             }
+        } else {
+            fma_to<VEC>(state, whole_span.a, state, whole_span.h);
         }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) c[j] = run[j] = begin[j];
-#pragma unroll
-        for (uint32_t w = 0; w < kSpanWarps; ++w) {
-            const Span<VEC> s = in_cta[buf][w][lane];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (w == warp) c[j] = run[j];
-            fma_to<VEC>(run, s.a, run, s.h);
-        }
-        if (cluster == 1) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) state[j] = run[j];
-        }
+        fma_to<VEC>(c, ahead.a, begin, ahead.h);
         if (p.states && warp == 0 && on && chunk < chunks) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) p.states[b * p.states_b + chunk * p.states_c + (d + j) * p.states_d] = begin[j];
@@ -754,38 +748,13 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
         if constexpr (SRC == kFromTiles) {
             if (done > 0) fetch(done + cluster, buf ^ 1);
         }
-        if (cluster > 1) {
-            if (warp == 0) {
-                Span<VEC> all;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) all.a[j] = 1.0f, all.h[j] = 0.0f;
-#pragma unroll
-                for (int w = kSpanWarps - 1; w >= 0; --w) {
-                    const SpanBoth<VEC>& s = in_cta[buf][w][lane];
-                    fma_to<VEC>(all.h, s.a, all.h, s.e);
-                    mul_to<VEC>(all.a, all.a, s.a);
-                }
-                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&arrived[buf]), cluster * 32 * static_cast<uint32_t>(sizeof(Span<VEC>)));
-                for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], smem_u32(&arrived[buf]), r, all);
-            }
-            arrivals.wait(buf);
-        }
-        float e[VEC], run[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) run[j] = carry[j];
-        if (cluster > 1) {
-            for (uint32_t r = 0; r < cluster; ++r) {
-                const Span<VEC> s = in_cluster[buf][r][lane];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if (r == rank) run[j] = carry[j];
-                fma_to<VEC>(carry, s.a, carry, s.h);
-            }
-        }
-        float fore[VEC];
+        // this CTA's spans from the end: `whole_span` all of them, `behind` those after this warp's; and the state before this warp's
+        Span<VEC> whole_span, behind;
+        float e[VEC], fore[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            e[j] = run[j];
+            whole_span.a[j] = behind.a[j] = 1.0f;
+            whole_span.h[j] = behind.h[j] = 0.0f;
             fore[j] = c[j];
         }
 #pragma unroll
@@ -793,18 +762,33 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
             const uint32_t w = kSpanWarps - 1 - k;
             const SpanBoth<VEC>& back = in_cta[buf][w][lane];
             const SpanBoth<VEC>& forth = in_cta[buf][k][lane];
+            if (w == warp) behind = whole_span;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                if (w == warp) e[j] = run[j];
+            for (int j = 0; j < VEC; ++j)
                 if (k == warp) c[j] = fore[j];
-            }
-            fma_to<VEC>(run, back.a, run, back.e);
+            fma_to<VEC>(whole_span.h, back.a, whole_span.h, back.e);
+            mul_to<VEC>(whole_span.a, whole_span.a, back.a);
             if (k + 1 < kSpanWarps) fma_to<VEC>(fore, forth.a, fore, forth.h);
         }
-        if (cluster == 1) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) carry[j] = run[j];
+        for (int j = 0; j < VEC; ++j) e[j] = carry[j];
+        if (cluster > 1) {
+            if (warp == 0) {
+                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&arrived[buf]), cluster * 32 * static_cast<uint32_t>(sizeof(Span<VEC>)));
+                for (uint32_t r = 0; r < cluster; ++r) span_to_cta<VEC>(&in_cluster[buf][rank][lane], smem_u32(&arrived[buf]), r, whole_span);
+            }
+            arrivals.wait(buf);
+            for (uint32_t r = 0; r < cluster; ++r) {
+                const Span<VEC> s = in_cluster[buf][r][lane];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (r == rank) e[j] = carry[j];
+                fma_to<VEC>(carry, s.a, carry, s.h);
+            }
+        } else {
+            fma_to<VEC>(carry, whole_span.a, carry, whole_span.h);
         }
+        fma_to<VEC>(e, behind.a, e, behind.h);
         const uint32_t there = on && t0 < p.T ? p.T - t0 : 0;
         const StepWriter<T, VEC, kTileStores> out_x(p.dx, b, d, t0, staging, 0), out_f(p.df, b, d, t0, staging, 1), out_i(p.di, b, d, t0, staging, 2),
             out_o(p.dout, b, d, t0, staging, 2 + HAS_I);

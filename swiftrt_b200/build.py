@@ -51,6 +51,33 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return SO
 
 
+BINDING_SRC = os.path.join(PKG, "csrc", "binding.cpp")
+BINDING = os.path.join(PKG, "_binding.so")
+
+
+def build_binding(force: bool = False) -> str:
+    """Compiles the Python binding of the latency-bound calls against torch's headers and the built library."""
+    deps = [BINDING_SRC, HEADERS[-1]]
+    if force or not os.path.exists(BINDING) or any(os.path.getmtime(f) > os.path.getmtime(BINDING) for f in deps):
+        build()
+        import sysconfig
+
+        import torch
+        from torch.utils import cpp_extension
+        nvcc = nvcc_path()
+        include = cpp_extension.include_paths() + [os.path.join(os.path.dirname(os.path.dirname(nvcc)), "include"), sysconfig.get_paths()["include"],
+                                                   os.path.join(ROOT, "include")]
+        torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wno-deprecated",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *("-I" + d for d in include), "-o", BINDING, BINDING_SRC,
+               "-L" + PKG, "-lsrt_b200", "-L" + torch_lib, "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+               "-Wl,-rpath,$ORIGIN"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("g++ failed on the Python binding:\n" + res.stdout + res.stderr)
+    return BINDING
+
+
 HOST_TEST_SRC = os.path.join(ROOT, "tests", "cpp", "test_host_kat.cpp")
 HOST_TEST_BIN = os.path.join(ROOT, "tests", "cpp", "test_host_kat")
 
@@ -75,3 +102,4 @@ def build_host_test(force: bool = False) -> str:
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
     print(build_host_test(force="--force" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))

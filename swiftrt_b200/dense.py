@@ -10,7 +10,7 @@ import torch
 from . import _lib
 from ._lib import lib
 from .int4 import Int4Weight, gated_matmul_int4, matmul_int4
-from .matmul import MatmulError, _descriptor, descriptor_args, enqueue, matmul, on_one_device
+from .matmul import MatmulError, _descriptor, binding, descriptor_args, enqueue, matmul, on_one_device
 from .tensor import ActivationType, order_of
 
 
@@ -127,37 +127,22 @@ class GatedDense:
         self.bias_gate, self.bias_up = bias_gate, bias_up
         self.activation = ActivationType(activation)
 
-    def _forward(self, x: torch.Tensor, gate, up) -> torch.Tensor:
-        y = torch.empty((x.shape[0], self.weight_gate.shape[1]), dtype=x.dtype, device=x.device)
-        enqueue(lib.srtMatmulGated, x.device, *descriptor_args(x, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up),
-                int(self.activation), *descriptor_args(gate, up, y))
-        return y
+    def _forward(self, x: torch.Tensor, keep: bool):
+        return binding.gated(x, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up, int(self.activation), keep)
 
     def __call__(self, input: torch.Tensor) -> torch.Tensor:
         if self.int4:
             return gated_matmul_int4(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up, self.activation)
-        on_one_device(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up)
-        x = input if input.dim() == 2 else input.reshape(-1, input.shape[-1])
-        try:
-            y = self._forward(x, None, None)
-        except MatmulError as e:
-            if e.code != _lib.cudaErrorNotSupported:
-                raise
-            y = self._forward(x, *self._pre_activations(x))          # two products and an elementwise pass
-        return y if input.dim() == 2 else y.view(*input.shape[:-1], -1)
-
-    def _pre_activations(self, x: torch.Tensor):
-        shape = (x.shape[0], self.weight_gate.shape[1])
-        return tuple(torch.empty(shape, dtype=x.dtype, device=x.device) for _ in range(2))
+        if input.dim() == 2:
+            return self._forward(input, False)
+        return self._forward(input.reshape(-1, input.shape[-1]), False).view(*input.shape[:-1], -1)
 
     def forward_keep(self, input: torch.Tensor):
         """(output, saved) for training; `saved` is the pair of pre-activations that backward() needs."""
         if self.int4:
             raise ValueError("4-bit weights have no backward pass")
-        on_one_device(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up)
-        x = input.reshape(-1, input.shape[-1])
-        saved = self._pre_activations(x)
-        return self._forward(x, *saved).view(*input.shape[:-1], -1), saved
+        y, gate, up = self._forward(input.reshape(-1, input.shape[-1]), True)
+        return y.view(*input.shape[:-1], -1), (gate, up)
 
     def backward(self, input: torch.Tensor, saved: tuple, out_grad: torch.Tensor):
         """Gradients of (input, weightGate, weightUp, biasGate, biasUp); None for a bias that is None.  `saved` is the

@@ -8,24 +8,11 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import lib
 from .dense import bias_activation_backward
-from .matmul import descriptor_args, enqueue, matmul, on_one_device
+from .matmul import binding, matmul
 from .tensor import ActivationType
 
 STATE_CHUNK = 64            # steps between two kept states (SRT_GATED_RECURRENCE_CHUNK)
-
-
-def _lengths(lengths: torch.Tensor | None, batch: int) -> int | None:
-    if lengths is None:
-        return None
-    if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != batch or (batch > 1 and lengths.stride(0) != 1):
-        raise ValueError(f"lengths must be a contiguous int32 tensor of {batch} elements")
-    return lengths.data_ptr()
-
-
-def _state_shape(update: torch.Tensor) -> tuple:
-    return (update.shape[0], update.shape[-1])
 
 
 def gated_recurrence(update: torch.Tensor, forget: torch.Tensor, input: torch.Tensor | None = None,
@@ -40,17 +27,7 @@ def gated_recurrence(update: torch.Tensor, forget: torch.Tensor, input: torch.Te
     Float32 [batch, channels]; `last` names the tensor that receives the latter and may be `initial` itself (a
     state advanced in place).  `lengths` (int32, one per batch item): steps behind them leave the state alone and
     have a hidden value of zero.  Asynchronous on torch's current stream of update's device."""
-    on_one_device(update, forget, input, output, initial, lengths, last)
-    hidden = torch.empty(update.shape, dtype=update.dtype, device=update.device)
-    if last is None:
-        last = torch.empty(_state_shape(update), dtype=torch.float32, device=update.device)
-    states = None
-    if keep:
-        steps = update.shape[1] if update.dim() == 3 else 1
-        states = torch.empty((update.shape[0], -(-steps // STATE_CHUNK), update.shape[-1]), dtype=torch.float32, device=update.device)
-    enqueue(lib.srtGatedRecurrence, update.device, *descriptor_args(update, forget, input, output, initial), _lengths(lengths, update.shape[0]),
-            *descriptor_args(hidden, last, states))
-    return (hidden, last, states) if keep else (hidden, last)
+    return binding.recurrence(update, forget, input, output, initial, lengths, keep, last)
 
 
 def gated_recurrence_backward(out_grad: torch.Tensor, update: torch.Tensor, forget: torch.Tensor, input: torch.Tensor | None,
@@ -59,14 +36,7 @@ def gated_recurrence_backward(out_grad: torch.Tensor, update: torch.Tensor, forg
     """Gradients of (update, forget, input, output, initial) of gated_recurrence for the gradient of its hidden
     values and, with `last_grad`, of its last state; None for a gate that is None.  `states` are the ones that the
     forward pass kept.  `out` names the four tensors (None for an absent gate) that receive the first four."""
-    on_one_device(update, out_grad, forget, input, output, states, lengths, last_grad, *(out or ()))
-    if out is None:
-        out = tuple(torch.empty(update.shape, dtype=update.dtype, device=update.device) if t is not None else None
-                    for t in (update, forget, input, output))
-    initial_grad = torch.empty(_state_shape(update), dtype=torch.float32, device=update.device)
-    enqueue(lib.srtGatedRecurrenceBackward, update.device, *descriptor_args(out_grad, last_grad, update, forget, input, output, states),
-            _lengths(lengths, update.shape[0]), *descriptor_args(*out, initial_grad))
-    return (*out, initial_grad)
+    return binding.recurrence_backward(out_grad, update, forget, input, output, states, lengths, last_grad, *(out or (None,) * 4))
 
 
 class LinearRecurrentCell:

@@ -15,6 +15,11 @@ import torch
 
 from . import _lib
 from ._lib import lib
+
+try:
+    from . import _binding as binding
+except ImportError as e:
+    raise ImportError(f"the Python binding has not been built ({e}). Run `python swiftrt_b200/build.py`; there is no fallback.") from e
 from .tensor import ActivationType, Descriptor, Order, empty, order_of
 
 
@@ -22,6 +27,9 @@ class MatmulError(RuntimeError):
     def __init__(self, code: int, what: str):
         super().__init__(f"srtMatmul failed with cudaError {code}: {what}")
         self.code = code
+
+
+binding.set_error_classes(MatmulError, torch.OutOfMemoryError)
 
 
 def _stream_ptr(device) -> int:

@@ -275,6 +275,30 @@ def test_layer_trains_and_generates_like_its_definition(srt):
         assert torch.equal(cell(x, state)[0], hidden)
 
 
+def test_python_refuses_what_the_header_refuses(srt):
+    """Errors of the C ABI come as MatmulError with their code, bad arguments as ValueError, and nothing is launched."""
+    x = torch.zeros(2, 3, 4, device=DEV)
+    before = srt.launch_count()
+    for bad in (torch.zeros(2, dtype=torch.int64, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV), torch.zeros(4, dtype=torch.int32, device=DEV)[::2]):
+        with pytest.raises(ValueError, match="lengths"):
+            srt.gated_recurrence(x, x, lengths=bad)
+    with pytest.raises(ValueError, match="different devices"):
+        srt.gated_recurrence(x, x.cpu())
+    with pytest.raises(ValueError, match="steps"):
+        srt.gated_recurrence(x[0, 0], x[0, 0])
+    with pytest.raises(srt.MatmulError, match="forget must be") as e:
+        srt.gated_recurrence(x, x[:, :2])
+    assert e.value.code == 1
+    with pytest.raises(srt.MatmulError, match="not computed") as e:
+        srt.gated_recurrence(x.double(), x.double())
+    assert e.value.code == 801
+    with pytest.raises(srt.MatmulError, match="Float32"):
+        srt.gated_recurrence(x, x, initial=torch.zeros(2, 4, device=DEV, dtype=torch.float16))
+    with pytest.raises(srt.MatmulError, match="states must be"):
+        srt.gated_recurrence_backward(x, x, x, None, None, torch.zeros(2, 2, 4, device=DEV))
+    assert srt.launch_count() == before
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_a_wait_that_runs_out_is_reported_and_ends_in_order(srt, dtype):
     """A limit of one nanosecond on the waits for the tiles of a long sequence: the status word says so, the kernel ends, and

@@ -96,17 +96,19 @@ def test_recurrence_backward_refuses(change, code, needle):
     assert rc == code and needle in _lib.last_error(), (rc, _lib.last_error())
 
 
-def test_python_refuses_host_tensors_and_bad_lengths():
+def test_python_refuses_host_tensors_and_other_objects():
     import torch
 
     import swiftrt_b200 as srt
     x = torch.zeros(2, 3, 4)
     with pytest.raises(ValueError, match="device tensors"):
         srt.gated_recurrence(x, x)
-    from swiftrt_b200.linear_recurrent import _lengths
-    for bad in (torch.zeros(2, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)[::2]):
-        with pytest.raises(ValueError, match="lengths"):
-            _lengths(bad, 2)
+    with pytest.raises(TypeError, match="update must be a tensor"):
+        srt.gated_recurrence(None, x)
+    with pytest.raises(TypeError, match="states must be a tensor"):
+        srt.gated_recurrence_backward(x, x, x, None, None, None)
+    with pytest.raises(ValueError, match="device tensors"):
+        srt.GatedDense(torch.zeros(4, 6), torch.zeros(4, 6))(torch.zeros(2, 4))
     with pytest.raises(ValueError, match="fusedWeight"):
         srt.LinearRecurrentCell(torch.zeros(4, 10), None, 4)
 

@@ -10,6 +10,8 @@
 #include <cstdarg>
 #include <cstdio>
 
+namespace srt { struct FewRowsParams; }
+
 // internal to the library: none of this is part of its dynamic symbols
 namespace srt __attribute__((visibility("hidden"))) {
 namespace host {
@@ -90,6 +92,8 @@ struct TileServices {
     unsigned long long wait_cycles;
 };
 cudaError_t tile_services(int device, TileServices& out);
+
+cudaError_t gated_few_rows(srtDataType type, const FewRowsParams& params, bool k_contiguous, cudaStream_t stream);
 
 }  // namespace host
 }  // namespace srt

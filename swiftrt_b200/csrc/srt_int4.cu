@@ -64,16 +64,19 @@ cudaError_t launch_few_rows(FewRowsParams& p, cudaStream_t stream)
 {
     const uint32_t batches = (p.K + Format::kBatch - 1) / Format::kBatch, row_blocks = (p.M + 8 * NT - 1) / (8 * NT);
     const uint32_t tiles = (p.N + Format::kCols - 1) / Format::kCols;
+    if (row_blocks > 65535) return fail(cudaErrorInvalidValue, "too many rows for a product of a few rows: %u", p.M);
     p.warps_n = 1;
-    // parts of K beyond the eight warps, while the CTAs do not fill the device twice and a warp still has a batch of its own
+    // Four warps to a column tile where there are tiles for every SM, else eight, and parts of K beyond them (a cluster) while the
+    // CTAs do not fill the device twice and a warp still has a batch of its own.
+    const uint32_t warps = (uint64_t)tiles * row_blocks >= 2 * 148 ? 4 : 8;
     uint32_t parts = 1;
-    while (parts < 8 && (uint64_t)tiles * row_blocks * parts * 2 <= 2 * 148 && 8 * parts * 2 <= batches) parts *= 2;
-    const uint32_t workers = 8 / p.warps_n * parts;
+    while (parts < 8 && (uint64_t)tiles * row_blocks * parts * 2 <= 2 * 148 && warps * parts * 2 <= batches) parts *= 2;
+    const uint32_t workers = warps / p.warps_n * parts;
     p.k_per_warp = (batches + workers - 1) / workers * Format::kBatch;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = dim3((tiles + p.warps_n - 1) / p.warps_n, parts, row_blocks);
-    cfg.blockDim = dim3(kFewRowsThreads, 1, 1);
+    cfg.blockDim = dim3(32 * warps, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -82,7 +85,6 @@ cudaError_t launch_few_rows(FewRowsParams& p, cudaStream_t stream)
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (row_blocks > 65535) return fail(cudaErrorInvalidValue, "too many rows for a product with 4-bit weights: %u", p.M);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, few_rows_kernel<T, Format, NW, NT>, p);
     if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;
@@ -92,8 +94,9 @@ template <typename T, int GPB, int NW>
 cudaError_t launch_int4_rows(FewRowsParams& p, cudaStream_t stream)
 {
     if (p.M <= 8) return launch_few_rows<T, Int4Format<T, GPB>, NW, 1>(p, stream);
-    if (p.M <= 16) return launch_few_rows<T, Int4Format<T, GPB>, NW, 2>(p, stream);
-    return launch_few_rows<T, Int4Format<T, GPB>, NW, 4>(p, stream);
+    // (two weights' sums of 32 rows do not fit into registers)
+    if (p.M <= 16 || NW == 2) return launch_few_rows<T, Int4Format<T, GPB>, NW, 2>(p, stream);
+    return launch_few_rows<T, Int4Format<T, GPB>, 1, 4>(p, stream);
 }
 
 template <typename T, int NW>
@@ -157,7 +160,27 @@ cudaError_t run_int4(const char* op, const void* x, const srtTensorDescriptor* x
     return w1 ? launch_int4_groups<__nv_bfloat16, 2>(p, stream) : launch_int4_groups<__nv_bfloat16, 1>(p, stream);
 }
 
+template <typename T>
+cudaError_t launch_gated_rows(FewRowsParams& p, bool k_contiguous, cudaStream_t stream)
+{
+    if (k_contiguous) return p.M <= 8 ? launch_few_rows<T, ColsFormat<T>, 2, 1>(p, stream) : launch_few_rows<T, ColsFormat<T>, 2, 2>(p, stream);
+    return p.M <= 8 ? launch_few_rows<T, RowsFormat<T>, 2, 1>(p, stream) : launch_few_rows<T, RowsFormat<T>, 2, 2>(p, stream);
+}
+
 }  // namespace
+
+namespace srt {
+namespace host {
+
+// the gated product of a few rows with 16-bit weights (srtMatmulGated)
+cudaError_t gated_few_rows(srtDataType type, const FewRowsParams& params, bool k_contiguous, cudaStream_t stream)
+{
+    FewRowsParams p = params;
+    return type == real16F ? launch_gated_rows<__half>(p, k_contiguous, stream) : launch_gated_rows<__nv_bfloat16>(p, k_contiguous, stream);
+}
+
+}  // namespace host
+}  // namespace srt
 
 extern "C" {
 

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "dense_backward.cuh"
+#include "few_rows.cuh"
 #include "gated_dense.cuh"
 #include "gemm_simt.cuh"
 #include "gemm_splitk.cuh"
@@ -1727,6 +1728,42 @@ cudaError_t gated_fused(srtDataType type, const Matrix& x, const Matrix& wg, con
     return e;
 }
 
+// Up to this many rows the weights are streamed past them instead of through the tiles of the tensor cores' own memory.
+constexpr uint64_t kFewRows = 16;
+
+// the gated product of a few rows; any strides of x and the results, weights contiguous along K or along their columns
+cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, const Matrix& wu, const void* bg, long long bg_n, const void* bu, long long bu_n,
+                       uint32_t act, const Matrix* gate, const Matrix* up, const Matrix& out, cudaStream_t stream)
+{
+    if (type == real32F || x.rows > kFewRows || x.cols == 0) return cudaErrorNotSupported;
+    const bool by_rows = (wg.n == 1 || wg.cols == 1) && (wu.n == 1 || wu.cols == 1);
+    const bool by_cols = (wg.m == 1 || wg.rows == 1) && (wu.m == 1 || wu.rows == 1);
+    if (!by_rows && !by_cols) return cudaErrorNotSupported;
+    FewRowsParams p;
+    memset(&p, 0, sizeof p);
+    const Matrix* w[2] = {&wg, &wu};
+    const Matrix* keep[2] = {gate, up};
+    for (int i = 0; i < 2; ++i) {
+        FewRowsWeight& f = p.w[i];
+        f.w = w[i]->p;
+        f.ld = by_rows ? w[i]->m : w[i]->n;
+        f.vec = reinterpret_cast<uintptr_t>(f.w) % 16 == 0 && f.ld % 8 == 0 && (!by_rows || wg.cols % 8 == 0);
+        f.bias = i == 0 ? bg : bu;
+        f.bias_n = i == 0 ? bg_n : bu_n;
+        if (keep[i]) {
+            f.keep = const_cast<char*>(keep[i]->p);
+            f.keep_m = keep[i]->m;
+            f.keep_n = keep[i]->n;
+        }
+    }
+    p.x = x.p; p.x_m = x.m; p.x_k = x.n;
+    p.x_vec = reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && (x.n == 1 || x.cols == 1) && (x.rows == 1 || x.m % 8 == 0);
+    p.out = const_cast<char*>(out.p); p.o_m = out.m; p.o_n = out.n;
+    p.M = (uint32_t)x.rows; p.N = (uint32_t)wg.cols; p.K = (uint32_t)x.cols;
+    p.act = act;
+    return gated_few_rows(type, p, !by_rows, stream);
+}
+
 // out = a1 . b1^T + a2 . b2^T (a [M x K], b [N x K]) in one launch
 cudaError_t sum_fused(srtDataType type, const Matrix& a1, const Matrix& b1, const Matrix& a2, const Matrix& b2, const Matrix& out, const DeviceInfo& dev,
                       cudaStream_t stream)
@@ -2574,6 +2611,8 @@ cudaError_t srtMatmulGated(const void* x, const srtTensorDescriptor* xDesc, cons
     if ((e = device_info(scope.device, info)) != cudaSuccess) return e;
     if (!info.sm100) return fail(cudaErrorNotSupported, "this library is built for sm_100a devices only");
     if (K > 0) {
+        e = gated_rows(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, stream);
+        if (e != cudaErrorNotSupported) return e;
         e = gated_fused(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, info, stream);
         if (e != cudaErrorNotSupported) return e;
     }

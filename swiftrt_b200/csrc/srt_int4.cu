@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstring>
 #include <type_traits>
 
@@ -53,58 +54,150 @@ FewRowsWeight weight_arg(const srtInt4Matrix* w)
     f.w = w->packed; f.ld = w->packedStride;
     f.scales = w->scales; f.scales_ld = w->scalesStride;
     f.zeros = w->zeros; f.zeros_ld = w->zerosStride;
-    // four columns at a time: 16 bytes of words, 8 of scales, 4 of zero points
-    f.vec = w->cols % 4 == 0 && w->packedStride % 4 == 0 && w->scalesStride % 4 == 0 && reinterpret_cast<uintptr_t>(w->packed) % 16 == 0 &&
-            reinterpret_cast<uintptr_t>(w->scales) % 8 == 0 && (!w->zeros || (w->zerosStride % 4 == 0 && reinterpret_cast<uintptr_t>(w->zeros) % 4 == 0));
+    // rows of words on 16 bytes, and four columns' scales on 8 and zero points on 4
+    auto rows_on = [&](const void* ptr, int64_t stride, int64_t bytes, uint64_t rows, uintptr_t to) {
+        return reinterpret_cast<uintptr_t>(ptr) % to == 0 && (rows <= 1 || stride * bytes % (int64_t)to == 0);
+    };
+    const uint64_t groups = (w->rows + w->groupSize - 1) / w->groupSize;
+    f.vec = rows_on(w->packed, w->packedStride, 4, (w->rows + 7) / 8, 16) && rows_on(w->scales, w->scalesStride, 2, groups, 8) &&
+            (!w->zeros || rows_on(w->zeros, w->zerosStride, 1, groups, 4));
     return f;
 }
 
-template <typename T, typename Format, int NW, int NT>
-cudaError_t launch_few_rows(FewRowsParams& p, cudaStream_t stream)
+template <typename T, typename Format> constexpr bool kByColumns = std::is_same<Format, ColsFormat<T>>::value;
+
+// the weight's tensor map, as the boxes of a stage (see few_rows_tiles_kernel)
+template <typename T, typename Format>
+bool encode_weight(EncodeTiledFn encode, const FewRowsParams& p, const FewRowsWeight& w, uint32_t parts, CUtensorMap* map)
 {
-    const uint32_t batches = (p.K + Format::kBatch - 1) / Format::kBatch, row_blocks = (p.M + 8 * NT - 1) / (8 * NT);
-    const uint32_t tiles = (p.N + Format::kCols - 1) / Format::kCols;
-    if (row_blocks > 65535) return fail(cudaErrorInvalidValue, "too many rows for a product of a few rows: %u", p.M);
-    p.warps_n = 1;
-    // Four warps to a column tile where there are tiles for every SM, else eight, and parts of K beyond them (a cluster) while the
-    // CTAs do not fill the device twice and a warp still has a batch of its own.
-    const uint32_t warps = (uint64_t)tiles * row_blocks >= 2 * 148 ? 4 : 8;
-    uint32_t parts = 1;
-    while (parts < 8 && (uint64_t)tiles * row_blocks * parts * 2 <= 2 * 148 && warps * parts * 2 <= batches) parts *= 2;
-    const uint32_t workers = warps / p.warps_n * parts;
-    p.k_per_warp = (batches + workers - 1) / workers * Format::kBatch;
+    const bool int4 = Format::kGroups;
+    const cuuint64_t elem = int4 ? 4 : 2, rows = int4 ? (p.K + 7) / 8 : p.K;
+    cuuint64_t dims[3] = {p.N, rows, 1};
+    cuuint32_t box[3] = {(cuuint32_t)(128 / elem), 16 * parts, 1}, unit[3] = {1, 1, 1};
+    if (kByColumns<T, Format>) { dims[0] = p.K; dims[1] = p.N; box[1] = 32; }
+    const cuuint64_t ld = dims[1] == 1 ? (dims[0] * elem + 15) / 16 * 16 : (cuuint64_t)w.ld * elem;
+    const cuuint64_t strides[2] = {ld, ld * dims[1]};
+    if (reinterpret_cast<uintptr_t>(w.w) % 16 != 0 || ld % 16 != 0 || ld < dims[0] * elem || strides[1] >= (1ull << 40)) return false;
+    const CUtensorMapDataType type = int4 ? CU_TENSOR_MAP_DATA_TYPE_INT32 : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return encode(map, type, 3, const_cast<void*>(w.w), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename Kernel, typename... Args>
+cudaError_t launch_rows_kernel(Kernel kernel, std::atomic<uint64_t>& ready, dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t stream, const Args&... args)
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(ready.load(std::memory_order_acquire) & bit)) {            // once per kernel and device
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024)) != cudaSuccess) return e;
+        ready.fetch_or(bit, std::memory_order_release);
+    }
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
-    cfg.gridDim = dim3((tiles + p.warps_n - 1) / p.warps_n, parts, row_blocks);
-    cfg.blockDim = dim3(32 * warps, 1, 1);
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = parts;
+    attr[0].val.clusterDim.y = grid.y;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, few_rows_kernel<T, Format, NW, NT>, p);
+    e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;
 }
 
-template <typename T, int GPB, int NW>
-cudaError_t launch_int4_rows(FewRowsParams& p, cudaStream_t stream)
+template <typename T, typename Format, int NW, int NT>
+cudaError_t launch_few_rows(FewRowsParams& p, int device, cudaStream_t stream)
 {
-    if (p.M <= 8) return launch_few_rows<T, Int4Format<T, GPB>, NW, 1>(p, stream);
+    const uint32_t row_blocks = (p.M + 8 * NT - 1) / (8 * NT), tiles = (p.N + Format::kCols - 1) / Format::kCols;
+    if (row_blocks > 65535) return fail(cudaErrorInvalidValue, "too many rows for a product of a few rows: %u", p.M);
+    if (p.w[0].vec && p.w[NW - 1].vec) {
+        TileServices services;
+        cudaError_t e = tile_services(device, services);
+        if (e != cudaSuccess) return e;
+        p.status = services.status;
+        p.wait_cycles = services.wait_cycles;
+        const uint32_t x_rows = p.M < 8 * NT ? p.M : 8 * NT, stage_bytes = NW * kFewRowsStageBytes;
+        // the ring of a launch with K cut `cluster` ways: two CTAs to an SM while three stages fit beside x, else one
+        struct Fit { uint32_t rounds, per_sm, stages; uint64_t x_bytes; };
+        auto fit = [&](uint32_t groups, uint32_t cluster) {
+            const uint32_t stage_rows = 8 / groups * Format::kWarpRows;
+            Fit f;
+            f.rounds = ((p.K + stage_rows - 1) / stage_rows + cluster - 1) / cluster;
+            p.k_per_part = f.rounds * stage_rows;
+            p.x_pitch = (p.k_per_part * 2 + 127) / 128 * 128 + 16;               // rows of x start four banks apart
+            f.x_bytes = (uint64_t)x_rows * p.x_pitch;
+            for (f.per_sm = 2; f.per_sm >= 1; --f.per_sm) {
+                const uint64_t room = (f.per_sm == 2 ? 110u : 224u) * 1024u - 1024u;
+                f.stages = f.x_bytes < room ? (uint32_t)((room - f.x_bytes) / stage_bytes) : 0;
+                if (f.stages >= 3 || f.stages >= f.rounds || f.per_sm == 1) break;
+            }
+            if (f.stages > kFewRowsMaxStages) f.stages = kFewRowsMaxStages;
+            if (f.stages > f.rounds) f.stages = f.rounds;
+            return f;
+        };
+        // As many column tiles to a CTA, and as many CTAs to a cluster, as run at once; fewer column tiles where that leaves more than
+        // half of the places empty.  (One row, 4096 x 16384 in 4 bits: 8 tiles x 1 / 2 / 4 / 8 CTAs a cluster 37 / 23 / 20 / 23 us.)
+        uint32_t groups = Format::kMaxColumnGroups, cluster = 1;
+        for (;; groups /= 2) {
+            const uint64_t ctas = (uint64_t)((tiles + groups - 1) / groups) * row_blocks;
+            const uint32_t rounds = (p.K + 8 / groups * Format::kWarpRows - 1) / (8 / groups * Format::kWarpRows);
+            uint64_t places = 148;
+            for (cluster = 8; cluster > 1; cluster /= 2) {
+                const Fit f = fit(groups, cluster);
+                places = 148u * f.per_sm;
+                if (cluster <= rounds && f.stages > 0 && ctas * cluster <= places) break;
+            }
+            if (groups == 1 || ctas * cluster * 2 >= places) break;
+        }
+        for (; cluster <= 8; cluster *= 2) {
+            const Fit f = fit(groups, cluster);
+            if (f.stages == 0) continue;
+            p.column_groups = groups;
+            const uint32_t stages = f.stages;
+            const uint64_t x_bytes = f.x_bytes;
+            // the sums take the ring's place
+            constexpr uint32_t kSums = few_rows_sum_bytes<Format, NW>();
+            const uint32_t ring = stages * stage_bytes > kSums ? stages * stage_bytes : (kSums + 127) / 128 * 128;
+            p.stages = stages;
+            FewRowsMaps maps;
+            if (!encode_weight<T, Format>(services.encode, p, p.w[0], 8 / groups, &maps.w[0]) ||
+                !encode_weight<T, Format>(services.encode, p, p.w[NW - 1], 8 / groups, &maps.w[1]))
+                break;
+            static std::atomic<uint64_t> ready{0};
+            return launch_rows_kernel(few_rows_tiles_kernel<T, Format, NW, NT>, ready, dim3((tiles + groups - 1) / groups, cluster, row_blocks),
+                                      kFewRowsTileThreads, 1024 + ring + (uint32_t)x_bytes, stream, p, maps);
+        }
+    }
+    const uint32_t units = (p.K + Format::kUnit - 1) / Format::kUnit;
+    uint32_t cluster = 1;
+    while (cluster < 8 && (uint64_t)tiles * row_blocks * cluster * 2 <= 2 * 148 && kFewRowsWarps * cluster * 2 <= units) cluster *= 2;
+    p.k_per_part = (units + kFewRowsWarps * cluster - 1) / (kFewRowsWarps * cluster) * Format::kUnit;
+    static std::atomic<uint64_t> ready{0};
+    return launch_rows_kernel(few_rows_kernel<T, Format, NW, NT>, ready, dim3(tiles, cluster, row_blocks), 32 * kFewRowsWarps, few_rows_sum_bytes<Format, NW>(), stream, p);
+}
+
+template <typename T, int GPB, int NW>
+cudaError_t launch_int4_rows(FewRowsParams& p, int device, cudaStream_t stream)
+{
+    if (p.M <= 8) return launch_few_rows<T, Int4Format<T, GPB>, NW, 1>(p, device, stream);
     // (two weights' sums of 32 rows do not fit into registers)
-    if (p.M <= 16 || NW == 2) return launch_few_rows<T, Int4Format<T, GPB>, NW, 2>(p, stream);
-    return launch_few_rows<T, Int4Format<T, GPB>, 1, 4>(p, stream);
+    if (p.M <= 16 || NW == 2) return launch_few_rows<T, Int4Format<T, GPB>, NW, 2>(p, device, stream);
+    return launch_few_rows<T, Int4Format<T, GPB>, 1, 4>(p, device, stream);
 }
 
 template <typename T, int NW>
-cudaError_t launch_int4_groups(FewRowsParams& p, cudaStream_t stream)
+cudaError_t launch_int4_groups(FewRowsParams& p, int device, cudaStream_t stream)
 {
-    if (p.group == 32) return launch_int4_rows<T, 4, NW>(p, stream);
-    if (p.group == 64) return launch_int4_rows<T, 2, NW>(p, stream);
-    return launch_int4_rows<T, 1, NW>(p, stream);
+    if (p.group == 32) return launch_int4_rows<T, 4, NW>(p, device, stream);
+    if (p.group == 64) return launch_int4_rows<T, 2, NW>(p, device, stream);
+    return launch_int4_rows<T, 1, NW>(p, device, stream);
 }
 
 cudaError_t run_int4(const char* op, const void* x, const srtTensorDescriptor* xDesc, const srtInt4Matrix* w0, const srtInt4Matrix* w1, const void* bias0,
@@ -153,18 +246,20 @@ cudaError_t run_int4(const char* op, const void* x, const srtTensorDescriptor* x
     p.x_vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && p.x_k == 1 && (M == 1 || p.x_m % 8 == 0);
     p.M = (uint32_t)M; p.N = (uint32_t)N; p.K = (uint32_t)K;
     p.group = w0->groupSize;
+    p.by_group = make_fast_div(p.group);
     p.act = (uint32_t)activation;
     DeviceScope scope(stream);
     if (scope.status != cudaSuccess) return scope.status;
-    if (type == real16F) return w1 ? launch_int4_groups<__half, 2>(p, stream) : launch_int4_groups<__half, 1>(p, stream);
-    return w1 ? launch_int4_groups<__nv_bfloat16, 2>(p, stream) : launch_int4_groups<__nv_bfloat16, 1>(p, stream);
+    const int device = scope.device;
+    if (type == real16F) return w1 ? launch_int4_groups<__half, 2>(p, device, stream) : launch_int4_groups<__half, 1>(p, device, stream);
+    return w1 ? launch_int4_groups<__nv_bfloat16, 2>(p, device, stream) : launch_int4_groups<__nv_bfloat16, 1>(p, device, stream);
 }
 
 template <typename T>
-cudaError_t launch_gated_rows(FewRowsParams& p, bool k_contiguous, cudaStream_t stream)
+cudaError_t launch_gated_rows(FewRowsParams& p, bool k_contiguous, int device, cudaStream_t stream)
 {
-    if (k_contiguous) return p.M <= 8 ? launch_few_rows<T, ColsFormat<T>, 2, 1>(p, stream) : launch_few_rows<T, ColsFormat<T>, 2, 2>(p, stream);
-    return p.M <= 8 ? launch_few_rows<T, RowsFormat<T>, 2, 1>(p, stream) : launch_few_rows<T, RowsFormat<T>, 2, 2>(p, stream);
+    if (k_contiguous) return p.M <= 8 ? launch_few_rows<T, ColsFormat<T>, 2, 1>(p, device, stream) : launch_few_rows<T, ColsFormat<T>, 2, 2>(p, device, stream);
+    return p.M <= 8 ? launch_few_rows<T, RowsFormat<T>, 2, 1>(p, device, stream) : launch_few_rows<T, RowsFormat<T>, 2, 2>(p, device, stream);
 }
 
 }  // namespace
@@ -173,10 +268,10 @@ namespace srt {
 namespace host {
 
 // the gated product of a few rows with 16-bit weights (srtMatmulGated)
-cudaError_t gated_few_rows(srtDataType type, const FewRowsParams& params, bool k_contiguous, cudaStream_t stream)
+cudaError_t gated_few_rows(srtDataType type, const FewRowsParams& params, bool k_contiguous, int device, cudaStream_t stream)
 {
     FewRowsParams p = params;
-    return type == real16F ? launch_gated_rows<__half>(p, k_contiguous, stream) : launch_gated_rows<__nv_bfloat16>(p, k_contiguous, stream);
+    return type == real16F ? launch_gated_rows<__half>(p, k_contiguous, device, stream) : launch_gated_rows<__nv_bfloat16>(p, k_contiguous, device, stream);
 }
 
 }  // namespace host

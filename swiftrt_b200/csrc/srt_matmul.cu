@@ -1733,7 +1733,7 @@ constexpr uint64_t kFewRows = 16;
 
 // the gated product of a few rows; any strides of x and the results, weights contiguous along K or along their columns
 cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, const Matrix& wu, const void* bg, long long bg_n, const void* bu, long long bu_n,
-                       uint32_t act, const Matrix* gate, const Matrix* up, const Matrix& out, cudaStream_t stream)
+                       uint32_t act, const Matrix* gate, const Matrix* up, const Matrix& out, int device, cudaStream_t stream)
 {
     if (type == real32F || x.rows > kFewRows || x.cols == 0) return cudaErrorNotSupported;
     const bool by_rows = (wg.n == 1 || wg.cols == 1) && (wu.n == 1 || wu.cols == 1);
@@ -1747,7 +1747,7 @@ cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, cons
         FewRowsWeight& f = p.w[i];
         f.w = w[i]->p;
         f.ld = by_rows ? w[i]->m : w[i]->n;
-        f.vec = reinterpret_cast<uintptr_t>(f.w) % 16 == 0 && f.ld % 8 == 0 && (!by_rows || wg.cols % 8 == 0);
+        f.vec = reinterpret_cast<uintptr_t>(f.w) % 16 == 0 && f.ld % 8 == 0;
         f.bias = i == 0 ? bg : bu;
         f.bias_n = i == 0 ? bg_n : bu_n;
         if (keep[i]) {
@@ -1761,7 +1761,7 @@ cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, cons
     p.out = const_cast<char*>(out.p); p.o_m = out.m; p.o_n = out.n;
     p.M = (uint32_t)x.rows; p.N = (uint32_t)wg.cols; p.K = (uint32_t)x.cols;
     p.act = act;
-    return gated_few_rows(type, p, !by_rows, stream);
+    return gated_few_rows(type, p, !by_rows, device, stream);
 }
 
 // out = a1 . b1^T + a2 . b2^T (a [M x K], b [N x K]) in one launch
@@ -2611,7 +2611,7 @@ cudaError_t srtMatmulGated(const void* x, const srtTensorDescriptor* xDesc, cons
     if ((e = device_info(scope.device, info)) != cudaSuccess) return e;
     if (!info.sm100) return fail(cudaErrorNotSupported, "this library is built for sm_100a devices only");
     if (K > 0) {
-        e = gated_rows(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, stream);
+        e = gated_rows(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, scope.device, stream);
         if (e != cudaErrorNotSupported) return e;
         e = gated_fused(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, info, stream);
         if (e != cudaErrorNotSupported) return e;

@@ -12,10 +12,22 @@ from .matmul import binding, descriptor_args, enqueue, on_one_device
 from .tensor import ActivationType, data_type
 
 
+def _on_rows_of(t: torch.Tensor, nbytes: int) -> torch.Tensor:
+    """`t` itself where its rows start on multiples of `nbytes`, else a copy whose rows do."""
+    width = nbytes // t.element_size()
+    if t.numel() == 0 or (t.data_ptr() % nbytes == 0 and (t.shape[0] == 1 or t.stride(0) % width == 0)):
+        return t
+    out = torch.empty((t.shape[0], -(-t.shape[1] // width) * width), dtype=t.dtype, device=t.device)[:, :t.shape[1]]
+    return out.copy_(t)
+
+
 class Int4Weight:
     """A [rows, cols] weight: `packed` int32 [ceil(rows / 8), cols] (row 8 j + i of column n in bits 4 i .. 4 i + 3 of word
     (j, n)), `scales` [ceil(rows / group), cols] in Float16 or BFloat16, `zeros` uint8 of the same shape or None (8).
-    Stands where a layer takes a weight (Dense, GatedDense) for its forward pass."""
+    Stands where a layer takes a weight (Dense, GatedDense) for its forward pass.
+
+    The products read 16 bytes of a row at a time: tensors whose rows do not start on 16 bytes (8 for scales, 4 for
+    zeros), as those of 1001 contiguous columns, are copied once into ones whose rows do."""
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group: int, rows: int):
         self.rows, self.cols, self.group = int(rows), int(packed.shape[-1]), int(group)
@@ -27,6 +39,8 @@ class Int4Weight:
             if t.dtype not in dtypes or tuple(t.shape) != (count, self.cols) or (self.cols > 1 and t.stride(1) != 1):
                 raise ValueError(f"{name} must be [{count}, {self.cols}] of {' or '.join(map(str, dtypes))} with contiguous columns")
         on_one_device(packed, scales, zeros)
+        packed, scales = _on_rows_of(packed, 16), _on_rows_of(scales, 8)
+        zeros = _on_rows_of(zeros, 4) if zeros is not None else None
         self.packed, self.scales, self.zeros = packed, scales, zeros
         self.shape, self.dtype, self.device = (self.rows, self.cols), scales.dtype, packed.device
         stride = lambda t: max(t.stride(0), self.cols)  # noqa: E731  (a single row may have any stride)

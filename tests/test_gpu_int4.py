@@ -101,7 +101,7 @@ def test_views_of_x_and_of_a_wider_weight(srt):
     whole = _check_single(srt, x, w)
     for lo, hi in ((0, 64), (64, 200), (3, 50), (199, 200), (4, 9)):
         part = srt.Int4Weight(w.packed[:, lo:hi], w.scales[:, lo:hi], w.zeros[:, lo:hi], G, K)
-        assert torch.equal(srt.matmul_int4(x, part), whole[:, lo:hi])
+        _check_single(srt, x, part)           # (how K is divided, and with it the order of the sums, depends on the columns)
     for view in (x.t().contiguous().t(), torch.cat((x, x), 1)[:, :K], torch.cat((x[:, :1], x), 1)[:, 1:], x.repeat_interleave(2, 1)[:, ::2],
                  x.repeat_interleave(2, 0)[::2]):
         assert torch.equal(srt.matmul_int4(view, w), whole)
@@ -119,6 +119,38 @@ def test_the_result_of_a_row_does_not_depend_on_its_neighbours(srt):
     got = srt.matmul_int4(x, w)
     rest = [0, 1, 2, 4, 6, 7]
     assert torch.equal(got[rest], want[rest]) and bool(torch.isnan(got[3]).all()) and not bool(torch.isfinite(got[5]).any())
+
+
+def _raw(w):
+    """The C structure over the tensors as they are, without the copy that aligns their rows."""
+    import ctypes
+
+    from swiftrt_b200 import _lib
+    from swiftrt_b200.tensor import data_type
+    packed, scales, zeros, group, rows = w
+    m = _lib.Int4Matrix(data_type(scales), group, rows, packed.shape[1], packed.data_ptr(), packed.stride(0), scales.data_ptr(), scales.stride(0),
+                        zeros.data_ptr() if zeros is not None else None, zeros.stride(0) if zeros is not None else 0)
+    return m, ctypes.addressof(m)
+
+
+@pytest.mark.parametrize("M,K,N,G", [(1, 256, 33, 128), (3, 300, 70, 64), (9, 97, 31, 32), (20, 1000, 5, 128), (2, 2048, 130, 64)])
+def test_rows_that_do_not_start_on_16_bytes(srt, M, K, N, G):
+    """The C ABI takes packed weights at any column of a wider one; they run on the kernel without bulk loads."""
+    from swiftrt_b200 import _lib
+    from swiftrt_b200.matmul import descriptor_args, enqueue
+    wide = [_weight(srt, K, N + 6, G, torch.float16, True, seed=s) for s in (0, 4)]
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).half().to(DEV)
+    for at in (0, 1, 3):
+        parts = [(w.packed[:, at:at + N], w.scales[:, at:at + N], w.zeros[:, at:at + N], G, K) for w in wide]
+        (m0, a0), (m1, a1) = (_raw(q) for q in parts)
+        ref = [srt.Int4Weight(*q) for q in parts]
+        out = torch.empty(M, N, dtype=torch.float16, device=DEV)
+        enqueue(_lib.lib.srtMatmulInt4, x.device, *descriptor_args(x), a0, None, None, 5, *descriptor_args(out))
+        z, e = _reference(x, ref[0], None)
+        _check(out, z, e)
+        enqueue(_lib.lib.srtMatmulGatedInt4, x.device, *descriptor_args(x), a0, a1, None, None, None, None, 5, *descriptor_args(out))
+        u, f = _reference(x, ref[1], None)
+        _check(out, z * u, e * (u.abs() + f) + z.abs() * f + 2.0 ** -23 * (z * u).abs())
 
 
 def test_nothing_outside_the_result_is_written(srt):

@@ -343,32 +343,32 @@ template <int NW, int TILES, int NT> __device__ __forceinline__ void clear(float
 
 // ------------------------------------------------------------------------------------------ sums and results
 // The warps' sums to the result, for both kernels: warp `slot` holds part slot / groups of column tile slot mod groups (of this CTA's
-// `groups`); red: room for [weight][warp][8][kCols + 1] floats.  All threads of the CTA call it; `mine`: this thread holds sums.
+// `groups`); red: room for few_rows_sum_bytes.  All threads of the CTA call it; `mine`: this thread holds sums.
 template <typename T, typename Format, int NW, int NT>
 __device__ __forceinline__ void few_rows_finish(const FewRowsParams& p, float* red, uint32_t slot, bool mine, uint32_t groups, uint32_t tile0, uint32_t m0,
                                                 const float (&acc)[NW][Format::kTiles][NT][4])
 {
     constexpr uint32_t kCols = Format::kCols, kPitch = kCols + 1;
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, parts = kFewRowsWarps / groups;
-    auto place = [&](uint32_t w, uint32_t s, uint32_t row, uint32_t col) { return ((w * kFewRowsWarps + s) * 8 + row) * kPitch + col; };
+    auto place = [&](uint32_t w, uint32_t s, uint32_t row, uint32_t col) { return ((w * kFewRowsWarps + s) * (8 * NT) + row) * kPitch + col; };
     const bool split = gridDim.y > 1;
+    __syncthreads();
+    if (mine) {
 #pragma unroll
-    for (uint32_t j = 0; j < NT; ++j) {
-        if (m0 + 8 * j >= p.M) break;                             // uniform over the cluster
-        __syncthreads();
-        if (mine) {
+        for (uint32_t w = 0; w < NW; ++w)
 #pragma unroll
-            for (uint32_t w = 0; w < NW; ++w)
+            for (uint32_t i = 0; i < Format::kTiles; ++i)
 #pragma unroll
-                for (uint32_t i = 0; i < Format::kTiles; ++i)
+                for (uint32_t j = 0; j < NT; ++j)
 #pragma unroll
-                    for (uint32_t c = 0; c < 4; ++c) red[place(w, slot, 2 * t + (c & 1), Format::column(g, i, c >> 1))] = acc[w][i][j][c];
-        }
-        __syncthreads();
-        const uint32_t rows = min(8u, p.M - m0 - 8 * j), items = groups * rows * kCols;
-        // with a cluster, the sum of a CTA's parts takes the place of the first, and every CTA finishes its share of the results
-        uint32_t first = threadIdx.x, end = items;
-        if (split) {
+                    for (uint32_t c = 0; c < 4; ++c) red[place(w, slot, 8 * j + 2 * t + (c & 1), Format::column(g, i, c >> 1))] = acc[w][i][j][c];
+    }
+    __syncthreads();
+    const uint32_t rows = min(8u * NT, p.M - m0), items = groups * rows * kCols;
+    // with a cluster, the sum of a CTA's parts takes the place of the first, and every CTA finishes its share of the results
+    uint32_t first = threadIdx.x, end = items;
+    if (split) {
+        if (parts > 1) {
             for (uint32_t id = threadIdx.x; id < items; id += blockDim.x) {
                 const uint32_t col = id % kCols, row = id / kCols % rows, tile = id / (rows * kCols);
 #pragma unroll
@@ -378,45 +378,45 @@ __device__ __forceinline__ void few_rows_finish(const FewRowsParams& p, float* r
                     red[place(w, tile, row, col)] = s;
                 }
             }
-            cluster_arrive_release();
-            cluster_wait_acquire();
-            const uint32_t share = (items + gridDim.y - 1) / gridDim.y;
-            first += blockIdx.y * share;
-            end = min(items, (blockIdx.y + 1) * share);
         }
-        for (uint32_t id = first; id < end; id += blockDim.x) {
-            const uint32_t col = id % kCols, row = id / kCols % rows, tile = id / (rows * kCols);
-            const uint32_t m = m0 + 8 * j + row, n = (tile0 + tile) * kCols + col;
-            if (n >= p.N) continue;
-            float v[NW];
+        cluster_arrive_release();
+        cluster_wait_acquire();
+        const uint32_t share = (items + gridDim.y - 1) / gridDim.y;
+        first += blockIdx.y * share;
+        end = min(items, (blockIdx.y + 1) * share);
+    }
+    for (uint32_t id = first; id < end; id += blockDim.x) {
+        const uint32_t col = id % kCols, row = id / kCols % rows, tile = id / (rows * kCols);
+        const uint32_t m = m0 + row, n = (tile0 + tile) * kCols + col;
+        if (n >= p.N) continue;
+        float v[NW];
 #pragma unroll
-            for (uint32_t w = 0; w < NW; ++w) {
-                const float* at = &red[place(w, tile, row, col)];
-                if (split) {
-                    float part[8];
+        for (uint32_t w = 0; w < NW; ++w) {
+            const float* at = &red[place(w, tile, row, col)];
+            if (split) {
+                float part[8];
 #pragma unroll
-                    for (uint32_t r = 0; r < 8; ++r) part[r] = r < gridDim.y ? __uint_as_float(ld_shared_remote_u32(smem_u32(at), r)) : 0.0f;
-                    v[w] = part[0];
+                for (uint32_t r = 0; r < 8; ++r) part[r] = r < gridDim.y ? __uint_as_float(ld_shared_remote_u32(smem_u32(at), r)) : 0.0f;
+                v[w] = part[0];
 #pragma unroll
-                    for (uint32_t r = 1; r < 8; ++r) v[w] += part[r];
-                } else {
-                    v[w] = *at;
-                    for (uint32_t q = 1; q < parts; ++q) v[w] += red[place(w, q * groups + tile, row, col)];
-                }
-                if (p.w[w].bias) v[w] += to_float<T>(static_cast<const T*>(p.w[w].bias)[n * p.w[w].bias_n]);
-                if (p.w[w].keep) static_cast<T*>(p.w[w].keep)[m * p.w[w].keep_m + n * p.w[w].keep_n] = from_float<T>(v[w]);
+                for (uint32_t r = 1; r < 8; ++r) v[w] += part[r];
+            } else {
+                v[w] = *at;
+                for (uint32_t q = 1; q < parts; ++q) v[w] += red[place(w, q * groups + tile, row, col)];
             }
-            float y = gate_activation<T>(p.act, v[0]);
-            if constexpr (NW == 2) y *= v[1];
-            static_cast<T*>(p.out)[m * p.o_m + n * p.o_n] = from_float<T>(y);
+            if (p.w[w].bias) v[w] += to_float<T>(static_cast<const T*>(p.w[w].bias)[n * p.w[w].bias_n]);
+            if (p.w[w].keep) static_cast<T*>(p.w[w].keep)[m * p.w[w].keep_m + n * p.w[w].keep_n] = from_float<T>(v[w]);
         }
-        if (split) {                                             // a CTA's sums are read by the others until here
-            cluster_arrive_release();
-            cluster_wait_acquire();
-        }
+        float y = gate_activation<T>(p.act, v[0]);
+        if constexpr (NW == 2) y *= v[1];
+        static_cast<T*>(p.out)[m * p.o_m + n * p.o_n] = from_float<T>(y);
+    }
+    if (split) {                                                 // a CTA's sums are read by the others until here
+        cluster_arrive_release();
+        cluster_wait_acquire();
     }
 }
-template <typename Format, int NW> constexpr uint32_t few_rows_sum_bytes() { return NW * kFewRowsWarps * 8 * (Format::kCols + 1) * 4; }
+template <typename Format, int NW, int NT> constexpr uint32_t few_rows_sum_bytes() { return NW * kFewRowsWarps * 8 * NT * (Format::kCols + 1) * 4; }
 
 // ------------------------------------------------------------------------------------------ any view
 // NW: weights (2: gated).  NT: tiles of 8 rows of x per CTA; grid z walks further rows.  Grid x: column tiles, grid y = the
@@ -464,7 +464,7 @@ few_rows_kernel(const __grid_constant__ FewRowsParams p)
 // Warps 0 .. 7 multiply: warp w takes column tile w mod CG and part w / CG (of KG = 8 / CG) of every stage's rows.  Warp 8 asks for the
 // stages: per weight 16 KB, CG tiles of 128-byte rows.  CG is 8 for wide weights (the rows of a stage are then a kilobyte of memory each)
 // and smaller where column tiles are few.
-constexpr uint32_t kFewRowsTileThreads = 32 * (kFewRowsWarps + 1), kFewRowsStageBytes = 16384, kFewRowsMaxStages = 8;
+constexpr uint32_t kFewRowsTileThreads = 32 * (kFewRowsWarps + 1), kFewRowsStageBytes = 16384, kFewRowsMaxStages = 6;
 
 template <typename T, typename Format, int NW, int NT>
 __global__ void __launch_bounds__(kFewRowsTileThreads)
@@ -525,18 +525,29 @@ few_rows_tiles_kernel(const __grid_constant__ FewRowsParams p, const __grid_cons
     // x of this CTA's rows of W, zeros behind them (the producer's first stages are on their way meanwhile)
     const uint32_t x_rows = min(8u * NT, p.M - m0), x_words = rounds * stage_rows / 8;
     if (warp < kFewRowsWarps) {
-        for (uint32_t id = threadIdx.x; id < x_rows * x_words; id += 32 * kFewRowsWarps) {
-            const uint32_t row = id / x_words, k = k0 + id % x_words * 8;
-            const T* at = static_cast<const T*>(p.x) + static_cast<long long>(m0 + row) * p.x_m + static_cast<long long>(k) * p.x_k;
-            uint32_t v[4];
-            if (p.x_vec && k + 8 <= p.K) {
-                const uint4 q = __ldg(reinterpret_cast<const uint4*>(at));
-                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-            } else {
-                gather_words<8>(at, p.x_k, k < p.K ? p.K - k : 0, v);
+        const uint32_t total = x_rows * x_words;
+        for (uint32_t base = threadIdx.x; base < total; base += 4 * 32 * kFewRowsWarps) {
+            uint32_t v[4][4], to[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {                                     // four loads in flight
+                const uint32_t id = base + u * 32 * kFewRowsWarps;
+                if (id >= total) break;
+                const uint32_t row = id / x_words, word = id - row * x_words, k = k0 + word * 8;
+                const T* at = static_cast<const T*>(p.x) + static_cast<long long>(m0 + row) * p.x_m + static_cast<long long>(k) * p.x_k;
+                to[u] = xs + row * p.x_pitch + word * 16;
+                if (p.x_vec && k + 8 <= p.K) {
+                    const uint4 q = __ldg(reinterpret_cast<const uint4*>(at));
+                    v[u][0] = q.x; v[u][1] = q.y; v[u][2] = q.z; v[u][3] = q.w;
+                } else {
+                    gather_words<8>(at, p.x_k, k < p.K ? p.K - k : 0, v[u]);
+                }
             }
-            if constexpr (Format::kGroups) Format::arrange(v);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(xs + row * p.x_pitch + (k - k0) * 2), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+                if (base + u * 32 * kFewRowsWarps >= total) break;
+                if constexpr (Format::kGroups) Format::arrange(v[u]);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to[u]), "r"(v[u][0]), "r"(v[u][1]), "r"(v[u][2]), "r"(v[u][3]) : "memory");
+            }
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");                              // the eight multiplying warps
         const uint32_t group_of = warp % groups, part = warp / groups;

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -112,92 +113,129 @@ cudaError_t launch_rows_kernel(Kernel kernel, std::atomic<uint64_t>& ready, dim3
     return e;
 }
 
+// How few_rows_tiles_kernel would run a product, and an estimate of its time in microseconds.
+struct RowsPlan {
+    double cost = 1e300;
+    uint32_t groups = 0, cluster = 0, stages = 0, k_per_part = 0, x_pitch = 0, x_bytes = 0;
+};
+
+// The choice of column tiles to a CTA and CTAs to a cluster by what it costs: rounds of CTAs (4 us and what they stream), x to bring in
+// before the first product, the exchange of a cluster, SMs without work or with one CTA's eight warps only.  One row, 4096 x 16384
+// in 4 bits, tiles x cluster: 8 x 4 17.0, 4 x 2 17.0, 2 x 1 16.4 us; 8 x 2 21.3, 8 x 8 22.5 us.  16 rows, 4096 x 2 x 16384 in bf16:
+// 8 x 4 56, 4 x 2 64, 2 x 1 76, 8 x 8 83 us.
 template <typename T, typename Format, int NW, int NT>
-cudaError_t launch_few_rows(FewRowsParams& p, int device, cudaStream_t stream)
+cudaError_t plan_few_rows(const FewRowsParams& p, RowsPlan& best)
+{
+    static std::atomic<uint32_t> by_registers{0};                            // CTAs that an SM's registers hold
+    uint32_t most = by_registers.load(std::memory_order_relaxed);
+    if (most == 0) {
+        cudaFuncAttributes attributes;
+        const cudaError_t e = cudaFuncGetAttributes(&attributes, few_rows_tiles_kernel<T, Format, NW, NT>);
+        if (e != cudaSuccess) return e;
+        most = 65536u / (((uint32_t)attributes.numRegs + 7) / 8 * 8 * kFewRowsTileThreads);
+        most = most > 3 ? 3 : most < 1 ? 1 : most;
+        by_registers.store(most, std::memory_order_relaxed);
+    }
+    const uint32_t row_blocks = (p.M + 8 * NT - 1) / (8 * NT), tiles = (p.N + Format::kCols - 1) / Format::kCols;
+    const uint32_t x_rows = p.M < 8 * NT ? p.M : 8 * NT, stage_bytes = NW * kFewRowsStageBytes;
+    for (uint32_t c = 1; c <= 8; c *= 2)
+        for (uint32_t g = Format::kMaxColumnGroups; g >= 1; g /= 2) {
+            const uint32_t stage_rows = 8 / g * Format::kWarpRows, rounds = ((p.K + stage_rows - 1) / stage_rows + c - 1) / c;
+            const uint32_t x_pitch = (rounds * stage_rows * 2 + 127) / 128 * 128 + 16;      // rows of x start four banks apart
+            const uint64_t x_bytes = (uint64_t)x_rows * x_pitch;
+            // as many CTAs to an SM as leave each three stages beside x
+            uint32_t per_sm = most, stages = 0;
+            for (; per_sm >= 1; --per_sm) {
+                const uint64_t room = (224u / per_sm - 2) * 1024u - 1024u;
+                stages = x_bytes < room ? (uint32_t)((room - x_bytes) / stage_bytes) : 0;
+                if (stages >= 3 || stages >= rounds || per_sm == 1) break;
+            }
+            if (stages > kFewRowsMaxStages) stages = kFewRowsMaxStages;
+            if (stages > rounds) stages = rounds;
+            if (stages == 0) continue;
+            const uint32_t at_once = per_sm > 2 ? 2 : per_sm;
+            const double places = 148.0 * at_once, full = (double)((tiles + g - 1) / g) * row_blocks * c / places;
+            const double stream = rounds * stage_bytes * places / 5.5e6;                    // a round of CTAs at 5.5 TB/s
+            double cost = std::ceil(full) * (4.0 + stream * (at_once == 1 && Format::kGroups ? 1.6 : 1.0)) + x_bytes / 1024.0 * 0.06;
+            if (full < 0.5) cost -= stream * (0.5 - full);                                  // (few CTAs share the bandwidth)
+            if (c > 1) cost += 0.8 + 0.15 * c;
+            if (cost < best.cost) {
+                best.cost = cost;
+                best.groups = g; best.cluster = c; best.stages = stages;
+                best.k_per_part = rounds * stage_rows; best.x_pitch = x_pitch; best.x_bytes = (uint32_t)x_bytes;
+            }
+        }
+    return cudaSuccess;
+}
+
+template <typename T, typename Format, int NW, int NT>
+cudaError_t launch_tiles(FewRowsParams& p, const RowsPlan& plan, EncodeTiledFn encode, bool& done, cudaStream_t stream)
+{
+    const uint32_t row_blocks = (p.M + 8 * NT - 1) / (8 * NT), tiles = (p.N + Format::kCols - 1) / Format::kCols, parts = 8 / plan.groups;
+    p.column_groups = plan.groups;
+    p.stages = plan.stages;
+    p.k_per_part = plan.k_per_part;
+    p.x_pitch = plan.x_pitch;
+    FewRowsMaps maps;
+    done = row_blocks <= 65535 && encode_weight<T, Format>(encode, p, p.w[0], parts, &maps.w[0]) && encode_weight<T, Format>(encode, p, p.w[NW - 1], parts, &maps.w[1]);
+    if (!done) return cudaSuccess;
+    // the sums take the ring's place
+    constexpr uint32_t kSums = (few_rows_sum_bytes<Format, NW, NT>() + 127) / 128 * 128;
+    const uint32_t ring = plan.stages * NW * kFewRowsStageBytes;
+    static std::atomic<uint64_t> ready{0};
+    return launch_rows_kernel(few_rows_tiles_kernel<T, Format, NW, NT>, ready, dim3((tiles + plan.groups - 1) / plan.groups, plan.cluster, row_blocks), kFewRowsTileThreads,
+                              1024 + (ring > kSums ? ring : kSums) + plan.x_bytes, stream, p, maps);
+}
+
+template <typename T, typename Format, int NW, int NT>
+cudaError_t launch_any(FewRowsParams& p, cudaStream_t stream)
 {
     const uint32_t row_blocks = (p.M + 8 * NT - 1) / (8 * NT), tiles = (p.N + Format::kCols - 1) / Format::kCols;
     if (row_blocks > 65535) return fail(cudaErrorInvalidValue, "too many rows for a product of a few rows: %u", p.M);
+    const uint32_t units = (p.K + Format::kUnit - 1) / Format::kUnit;
+    uint32_t cluster = 1;
+    while (cluster < 8 && (uint64_t)tiles * row_blocks * cluster * 2 <= 2 * 148 && kFewRowsWarps * cluster * 2 <= units) cluster *= 2;
+    p.k_per_part = (units + kFewRowsWarps * cluster - 1) / (kFewRowsWarps * cluster) * Format::kUnit;
+    static std::atomic<uint64_t> ready{0};
+    return launch_rows_kernel(few_rows_kernel<T, Format, NW, NT>, ready, dim3(tiles, cluster, row_blocks), 32 * kFewRowsWarps, few_rows_sum_bytes<Format, NW, NT>(), stream, p);
+}
+
+// Eight, 16 or 32 rows of x to a CTA, whichever is estimated to be fastest: more rows read the weights fewer times, fewer rows have
+// less of x to bring in and more CTAs to an SM (two weights' sums of 32 rows do not fit into registers).
+template <typename T, typename Format, int NW>
+cudaError_t launch_few_rows(FewRowsParams& p, int device, cudaStream_t stream)
+{
     if (p.w[0].vec && p.w[NW - 1].vec) {
         TileServices services;
         cudaError_t e = tile_services(device, services);
         if (e != cudaSuccess) return e;
         p.status = services.status;
         p.wait_cycles = services.wait_cycles;
-        const uint32_t x_rows = p.M < 8 * NT ? p.M : 8 * NT, stage_bytes = NW * kFewRowsStageBytes;
-        // the ring of a launch with K cut `cluster` ways: two CTAs to an SM while three stages fit beside x, else one
-        struct Fit { uint32_t rounds, per_sm, stages; uint64_t x_bytes; };
-        auto fit = [&](uint32_t groups, uint32_t cluster) {
-            const uint32_t stage_rows = 8 / groups * Format::kWarpRows;
-            Fit f;
-            f.rounds = ((p.K + stage_rows - 1) / stage_rows + cluster - 1) / cluster;
-            p.k_per_part = f.rounds * stage_rows;
-            p.x_pitch = (p.k_per_part * 2 + 127) / 128 * 128 + 16;               // rows of x start four banks apart
-            f.x_bytes = (uint64_t)x_rows * p.x_pitch;
-            for (f.per_sm = 2; f.per_sm >= 1; --f.per_sm) {
-                const uint64_t room = (f.per_sm == 2 ? 110u : 224u) * 1024u - 1024u;
-                f.stages = f.x_bytes < room ? (uint32_t)((room - f.x_bytes) / stage_bytes) : 0;
-                if (f.stages >= 3 || f.stages >= f.rounds || f.per_sm == 1) break;
-            }
-            if (f.stages > kFewRowsMaxStages) f.stages = kFewRowsMaxStages;
-            if (f.stages > f.rounds) f.stages = f.rounds;
-            return f;
-        };
-        // As many column tiles to a CTA, and as many CTAs to a cluster, as run at once; fewer column tiles where that leaves more than
-        // half of the places empty.  (One row, 4096 x 16384 in 4 bits: 8 tiles x 1 / 2 / 4 / 8 CTAs a cluster 37 / 23 / 20 / 23 us.)
-        uint32_t groups = Format::kMaxColumnGroups, cluster = 1;
-        for (;; groups /= 2) {
-            const uint64_t ctas = (uint64_t)((tiles + groups - 1) / groups) * row_blocks;
-            const uint32_t rounds = (p.K + 8 / groups * Format::kWarpRows - 1) / (8 / groups * Format::kWarpRows);
-            uint64_t places = 148;
-            for (cluster = 8; cluster > 1; cluster /= 2) {
-                const Fit f = fit(groups, cluster);
-                places = 148u * f.per_sm;
-                if (cluster <= rounds && f.stages > 0 && ctas * cluster <= places) break;
-            }
-            if (groups == 1 || ctas * cluster * 2 >= places) break;
-        }
-        for (; cluster <= 8; cluster *= 2) {
-            const Fit f = fit(groups, cluster);
-            if (f.stages == 0) continue;
-            p.column_groups = groups;
-            const uint32_t stages = f.stages;
-            const uint64_t x_bytes = f.x_bytes;
-            // the sums take the ring's place
-            constexpr uint32_t kSums = few_rows_sum_bytes<Format, NW>();
-            const uint32_t ring = stages * stage_bytes > kSums ? stages * stage_bytes : (kSums + 127) / 128 * 128;
-            p.stages = stages;
-            FewRowsMaps maps;
-            if (!encode_weight<T, Format>(services.encode, p, p.w[0], 8 / groups, &maps.w[0]) ||
-                !encode_weight<T, Format>(services.encode, p, p.w[NW - 1], 8 / groups, &maps.w[1]))
-                break;
-            static std::atomic<uint64_t> ready{0};
-            return launch_rows_kernel(few_rows_tiles_kernel<T, Format, NW, NT>, ready, dim3((tiles + groups - 1) / groups, cluster, row_blocks),
-                                      kFewRowsTileThreads, 1024 + ring + (uint32_t)x_bytes, stream, p, maps);
+        RowsPlan plan[3];
+        if ((e = plan_few_rows<T, Format, NW, 1>(p, plan[0])) != cudaSuccess) return e;
+        if (p.M > 8 && (e = plan_few_rows<T, Format, NW, 2>(p, plan[1])) != cudaSuccess) return e;
+        if constexpr (NW == 1)
+            if (p.M > 16 && (e = plan_few_rows<T, Format, NW, 4>(p, plan[2])) != cudaSuccess) return e;
+        bool done = false;
+        int which = plan[1].cost < plan[0].cost ? 1 : 0;
+        if (plan[2].cost < plan[which].cost) which = 2;
+        if (plan[which].cost < 1e300) {
+            if (which == 0) e = launch_tiles<T, Format, NW, 1>(p, plan[0], services.encode, done, stream);
+            else if (which == 1) e = launch_tiles<T, Format, NW, 2>(p, plan[1], services.encode, done, stream);
+            if constexpr (NW == 1)
+                if (which == 2) e = launch_tiles<T, Format, NW, 4>(p, plan[2], services.encode, done, stream);
+            if (done || e != cudaSuccess) return e;
         }
     }
-    const uint32_t units = (p.K + Format::kUnit - 1) / Format::kUnit;
-    uint32_t cluster = 1;
-    while (cluster < 8 && (uint64_t)tiles * row_blocks * cluster * 2 <= 2 * 148 && kFewRowsWarps * cluster * 2 <= units) cluster *= 2;
-    p.k_per_part = (units + kFewRowsWarps * cluster - 1) / (kFewRowsWarps * cluster) * Format::kUnit;
-    static std::atomic<uint64_t> ready{0};
-    return launch_rows_kernel(few_rows_kernel<T, Format, NW, NT>, ready, dim3(tiles, cluster, row_blocks), 32 * kFewRowsWarps, few_rows_sum_bytes<Format, NW>(), stream, p);
-}
-
-template <typename T, int GPB, int NW>
-cudaError_t launch_int4_rows(FewRowsParams& p, int device, cudaStream_t stream)
-{
-    if (p.M <= 8) return launch_few_rows<T, Int4Format<T, GPB>, NW, 1>(p, device, stream);
-    // (two weights' sums of 32 rows do not fit into registers)
-    if (p.M <= 16 || NW == 2) return launch_few_rows<T, Int4Format<T, GPB>, NW, 2>(p, device, stream);
-    return launch_few_rows<T, Int4Format<T, GPB>, 1, 4>(p, device, stream);
+    return p.M <= 8 ? launch_any<T, Format, NW, 1>(p, stream) : launch_any<T, Format, NW, 2>(p, stream);
 }
 
 template <typename T, int NW>
-cudaError_t launch_int4_groups(FewRowsParams& p, int device, cudaStream_t stream)
+cudaError_t launch_int4(FewRowsParams& p, int device, cudaStream_t stream)
 {
-    if (p.group == 32) return launch_int4_rows<T, 4, NW>(p, device, stream);
-    if (p.group == 64) return launch_int4_rows<T, 2, NW>(p, device, stream);
-    return launch_int4_rows<T, 1, NW>(p, device, stream);
+    if (p.group == 32) return launch_few_rows<T, Int4Format<T, 4>, NW>(p, device, stream);
+    if (p.group == 64) return launch_few_rows<T, Int4Format<T, 2>, NW>(p, device, stream);
+    return launch_few_rows<T, Int4Format<T, 1>, NW>(p, device, stream);
 }
 
 cudaError_t run_int4(const char* op, const void* x, const srtTensorDescriptor* xDesc, const srtInt4Matrix* w0, const srtInt4Matrix* w1, const void* bias0,
@@ -251,15 +289,14 @@ cudaError_t run_int4(const char* op, const void* x, const srtTensorDescriptor* x
     DeviceScope scope(stream);
     if (scope.status != cudaSuccess) return scope.status;
     const int device = scope.device;
-    if (type == real16F) return w1 ? launch_int4_groups<__half, 2>(p, device, stream) : launch_int4_groups<__half, 1>(p, device, stream);
-    return w1 ? launch_int4_groups<__nv_bfloat16, 2>(p, device, stream) : launch_int4_groups<__nv_bfloat16, 1>(p, device, stream);
+    if (type == real16F) return w1 ? launch_int4<__half, 2>(p, device, stream) : launch_int4<__half, 1>(p, device, stream);
+    return w1 ? launch_int4<__nv_bfloat16, 2>(p, device, stream) : launch_int4<__nv_bfloat16, 1>(p, device, stream);
 }
 
 template <typename T>
 cudaError_t launch_gated_rows(FewRowsParams& p, bool k_contiguous, int device, cudaStream_t stream)
 {
-    if (k_contiguous) return p.M <= 8 ? launch_few_rows<T, ColsFormat<T>, 2, 1>(p, device, stream) : launch_few_rows<T, ColsFormat<T>, 2, 2>(p, device, stream);
-    return p.M <= 8 ? launch_few_rows<T, RowsFormat<T>, 2, 1>(p, device, stream) : launch_few_rows<T, RowsFormat<T>, 2, 2>(p, device, stream);
+    return k_contiguous ? launch_few_rows<T, ColsFormat<T>, 2>(p, device, stream) : launch_few_rows<T, RowsFormat<T>, 2>(p, device, stream);
 }
 
 }  // namespace

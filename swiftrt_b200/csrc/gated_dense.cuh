@@ -90,10 +90,14 @@ gate_backward_kernel(const __grid_constant__ GateBackwardParams p)
                 const long long r = static_cast<long long>(r0) + k * static_cast<long long>(step);
                 if (r >= p.M) continue;
                 __align__(16) T dg[VEC], du[VEC];
+                float z[VEC], value[VEC], slope[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) z[j] = to_float<T>(g[k][j]);
+                gate_values<T, VEC>(p.act, z, value, slope);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float d = to_float<T>(dy[k][j]), z = to_float<T>(g[k][j]);
-                    const float vg = d * to_float<T>(u[k][j]) * gate_slope<T>(p.act, z), vu = d * gate_activation<T>(p.act, z);
+                    const float d = to_float<T>(dy[k][j]);
+                    const float vg = d * to_float<T>(u[k][j]) * slope[j], vu = d * value[j];
                     dg[j] = from_float<T>(vg);
                     du[j] = from_float<T>(vu);
                     sg[j] += vg;

@@ -46,28 +46,11 @@ struct RecurrenceParams {
 // precision).  The .ftz forms of the two approximations take one instruction each where the others rescale denormals
 // around them.  For the pair e is capped at 2^126, so that a closed gate is 2^-126 and not 0 times infinity.
 struct Gate { float on, off; };
-__device__ __forceinline__ float exp2_ftz(float x)
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float reciprocal_ftz(float x)
-{
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float min_or_nan(float a, float b)
 {
     float y;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
-}
-constexpr float kLog2E = 1.4426950408889634f;
-__device__ __forceinline__ float logistic(float a)
-{
-    return reciprocal_ftz(1.0f + exp2_ftz(-kLog2E * a));
 }
 __device__ __forceinline__ Gate logistic_pair(float a)
 {

@@ -93,7 +93,7 @@ struct TileServices {
 };
 cudaError_t tile_services(int device, TileServices& out);
 
-cudaError_t gated_few_rows(srtDataType type, const FewRowsParams& params, bool k_contiguous, int device, cudaStream_t stream);
+cudaError_t gated_few_rows(srtDataType type, const FewRowsParams& params, bool k_contiguous, double limit, int device, cudaStream_t stream);
 
 }  // namespace host
 }  // namespace srt

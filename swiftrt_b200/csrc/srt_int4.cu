@@ -202,8 +202,9 @@ cudaError_t launch_any(FewRowsParams& p, cudaStream_t stream)
 
 // Eight, 16 or 32 rows of x to a CTA, whichever is estimated to be fastest: more rows read the weights fewer times, fewer rows have
 // less of x to bring in and more CTAs to an SM (two weights' sums of 32 rows do not fit into registers).
+// cudaErrorNotSupported, without text, where the estimate is above `limit` microseconds.
 template <typename T, typename Format, int NW>
-cudaError_t launch_few_rows(FewRowsParams& p, int device, cudaStream_t stream)
+cudaError_t launch_few_rows(FewRowsParams& p, double limit, int device, cudaStream_t stream)
 {
     if (p.w[0].vec && p.w[NW - 1].vec) {
         TileServices services;
@@ -219,6 +220,7 @@ cudaError_t launch_few_rows(FewRowsParams& p, int device, cudaStream_t stream)
         bool done = false;
         int which = plan[1].cost < plan[0].cost ? 1 : 0;
         if (plan[2].cost < plan[which].cost) which = 2;
+        if (plan[which].cost > limit) return cudaErrorNotSupported;
         if (plan[which].cost < 1e300) {
             if (which == 0) e = launch_tiles<T, Format, NW, 1>(p, plan[0], services.encode, done, stream);
             else if (which == 1) e = launch_tiles<T, Format, NW, 2>(p, plan[1], services.encode, done, stream);
@@ -233,9 +235,9 @@ cudaError_t launch_few_rows(FewRowsParams& p, int device, cudaStream_t stream)
 template <typename T, int NW>
 cudaError_t launch_int4(FewRowsParams& p, int device, cudaStream_t stream)
 {
-    if (p.group == 32) return launch_few_rows<T, Int4Format<T, 4>, NW>(p, device, stream);
-    if (p.group == 64) return launch_few_rows<T, Int4Format<T, 2>, NW>(p, device, stream);
-    return launch_few_rows<T, Int4Format<T, 1>, NW>(p, device, stream);
+    if (p.group == 32) return launch_few_rows<T, Int4Format<T, 4>, NW>(p, 1e299, device, stream);
+    if (p.group == 64) return launch_few_rows<T, Int4Format<T, 2>, NW>(p, 1e299, device, stream);
+    return launch_few_rows<T, Int4Format<T, 1>, NW>(p, 1e299, device, stream);
 }
 
 cudaError_t run_int4(const char* op, const void* x, const srtTensorDescriptor* xDesc, const srtInt4Matrix* w0, const srtInt4Matrix* w1, const void* bias0,
@@ -294,9 +296,9 @@ cudaError_t run_int4(const char* op, const void* x, const srtTensorDescriptor* x
 }
 
 template <typename T>
-cudaError_t launch_gated_rows(FewRowsParams& p, bool k_contiguous, int device, cudaStream_t stream)
+cudaError_t launch_gated_rows(FewRowsParams& p, bool k_contiguous, double limit, int device, cudaStream_t stream)
 {
-    return k_contiguous ? launch_few_rows<T, ColsFormat<T>, 2>(p, device, stream) : launch_few_rows<T, RowsFormat<T>, 2>(p, device, stream);
+    return k_contiguous ? launch_few_rows<T, ColsFormat<T>, 2>(p, limit, device, stream) : launch_few_rows<T, RowsFormat<T>, 2>(p, limit, device, stream);
 }
 
 }  // namespace
@@ -305,10 +307,10 @@ namespace srt {
 namespace host {
 
 // the gated product of a few rows with 16-bit weights (srtMatmulGated)
-cudaError_t gated_few_rows(srtDataType type, const FewRowsParams& params, bool k_contiguous, int device, cudaStream_t stream)
+cudaError_t gated_few_rows(srtDataType type, const FewRowsParams& params, bool k_contiguous, double limit, int device, cudaStream_t stream)
 {
     FewRowsParams p = params;
-    return type == real16F ? launch_gated_rows<__half>(p, k_contiguous, device, stream) : launch_gated_rows<__nv_bfloat16>(p, k_contiguous, device, stream);
+    return type == real16F ? launch_gated_rows<__half>(p, k_contiguous, limit, device, stream) : launch_gated_rows<__nv_bfloat16>(p, k_contiguous, limit, device, stream);
 }
 
 }  // namespace host

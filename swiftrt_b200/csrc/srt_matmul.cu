@@ -1728,14 +1728,18 @@ cudaError_t gated_fused(srtDataType type, const Matrix& x, const Matrix& wg, con
     return e;
 }
 
-// Up to this many rows the weights are streamed past them instead of through the tiles of the tensor cores' own memory.
-constexpr uint64_t kFewRows = 16;
+// Up to kFewRows rows the weights are streamed past them (few_rows.cuh); up to kSomeRows where that is estimated to be faster
+// than the tensor cores' tiles: a tile is 128 columns by 256 rows whatever M is, and takes 0.4 us for every 64 of K, 8 us around them
+// (17 .. 256 rows of 2048 x 2 x 2048 19 us, of 4096 x 2 x 16384 64 us, of 1024 x 2 x 4096 15 us; streamed, 16 rows of the same 11, 52 and
+// 17 us, 48 rows 20, - and 31 us).  The estimate of the streaming kernel is 1.3 times too low from 9 rows on.
+constexpr uint64_t kFewRows = 8, kSomeRows = 128;
 
-// the gated product of a few rows; any strides of x and the results, weights contiguous along K or along their columns
+// the gated product of a few rows; any strides of x and the results, weights contiguous along K or along their columns.
+// `if_faster`: only where the tiles are estimated to be slower
 cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, const Matrix& wu, const void* bg, long long bg_n, const void* bu, long long bu_n,
-                       uint32_t act, const Matrix* gate, const Matrix* up, const Matrix& out, int device, cudaStream_t stream)
+                       uint32_t act, const Matrix* gate, const Matrix* up, const Matrix& out, bool if_faster, int device, cudaStream_t stream)
 {
-    if (type == real32F || x.rows > kFewRows || x.cols == 0) return cudaErrorNotSupported;
+    if (type == real32F || x.rows > kSomeRows || x.cols == 0) return cudaErrorNotSupported;
     const bool by_rows = (wg.n == 1 || wg.cols == 1) && (wu.n == 1 || wu.cols == 1);
     const bool by_cols = (wg.m == 1 || wg.rows == 1) && (wu.m == 1 || wu.rows == 1);
     if (!by_rows && !by_cols) return cudaErrorNotSupported;
@@ -1761,7 +1765,13 @@ cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, cons
     p.out = const_cast<char*>(out.p); p.o_m = out.m; p.o_n = out.n;
     p.M = (uint32_t)x.rows; p.N = (uint32_t)wg.cols; p.K = (uint32_t)x.cols;
     p.act = act;
-    return gated_few_rows(type, p, !by_rows, device, stream);
+    double limit = 1e299;
+    if (if_faster && x.rows > kFewRows) {
+        if (!p.w[0].vec || !p.w[1].vec) return cudaErrorNotSupported;
+        const uint64_t tiles = (wg.cols + 127) / 128;
+        limit = ((double)((tiles + 73) / 74) * (double)((x.cols + 63) / 64) * 0.4 + 8.0) / 1.3;
+    }
+    return gated_few_rows(type, p, !by_rows, limit, device, stream);
 }
 
 // out = a1 . b1^T + a2 . b2^T (a [M x K], b [N x K]) in one launch
@@ -2611,9 +2621,14 @@ cudaError_t srtMatmulGated(const void* x, const srtTensorDescriptor* xDesc, cons
     if ((e = device_info(scope.device, info)) != cudaSuccess) return e;
     if (!info.sm100) return fail(cudaErrorNotSupported, "this library is built for sm_100a devices only");
     if (K > 0) {
-        e = gated_rows(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, scope.device, stream);
-        if (e != cudaErrorNotSupported) return e;
-        e = gated_fused(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, info, stream);
+        auto rows = [&](bool if_faster) {
+            return gated_rows(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, if_faster,
+                              scope.device, stream);
+        };
+        e = rows(true);
+        if (e == cudaErrorNotSupported)
+            e = gated_fused(type, mx, mg, mu, biasGate, bg_n, biasUp, bu_n, (uint32_t)activation, gate ? &kg : nullptr, gate ? &ku : nullptr, mo, info, stream);
+        if (e == cudaErrorNotSupported) e = rows(false);          // (views that the tiles do not take)
         if (e != cudaErrorNotSupported) return e;
     }
     // two products and an elementwise pass; the pre-activations need a place then

@@ -123,12 +123,12 @@ cudaError_t launch_spans_kernel(Kernel kernel, const Maps& maps, std::atomic<uin
     }
     const uint32_t blocks_d = (p.D + channels - 1) / channels, chunks = (p.T + kRecurrenceChunk - 1) / kRecurrenceChunk;
     const uint64_t blocks = (uint64_t)p.B * blocks_d;
-    // Spans of one item and channel block side by side until there are CTAs for most places: each CTA then goes through a
-    // longer part of its sequence, which hides its start, and exchanges with fewer.  Forward of 2048 steps, 4096
-    // channels, 1 / 2 / 4 / 8 CTAs a cluster: 4 items (256 blocks) 63 / 79 / 76 / 86 us; 8191 steps of one item (64 blocks) 172 /
-    // 127 / 84 / 95 us; 1024 channels of one item (16 blocks) 45 / 34 / 24 / 24 us.
+    // Spans of one item and channel block side by side while their CTAs find a place at once, three to an SM less what clusters
+    // leave free: a CTA alone on its SM waits for its own latencies.  Forward / backward in us of 2048 steps, bf16, with 1, 2, 4
+    // and 8 CTAs a cluster: 40 blocks 42/76 29/47 21/33 17/34; 55 blocks 41/78 29/47 21/37 23/39; 104 blocks 44/78 37/64 29/58
+    // 38/68; 130 blocks 43/80 39/64 39/70 45/79; 222 blocks 62/111 52/105 62/117 71/129; 256 blocks forward 63 79 76 86.
     uint32_t cluster = 1;
-    while (cluster < 8 && blocks * cluster < 192 && cluster < chunks) cluster *= 2;
+    while (cluster < 8 && cluster < chunks && blocks * cluster * 2 <= 148 * 3 - 28 * (cluster - 1)) cluster *= 2;
     if (blocks * cluster > 0x7fffffffull) return fail(cudaErrorInvalidValue, "too many channels for one call");
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);

@@ -367,6 +367,16 @@ struct StepWriter {
     }
 };
 
+// zeros in up to 8 steps from t0
+template <typename T, int VEC> __device__ __forceinline__ void write_zeros(const Strided3W& s, uint32_t b, uint32_t d, uint32_t t0, uint32_t there)
+{
+    using Raw = typename Lane<T, VEC>::Raw;
+    T* to = static_cast<T*>(s.p) + b * s.b + d * s.d + t0 * s.t;
+#pragma unroll
+    for (uint32_t k = 0; k < kSpanSteps; ++k)
+        if (k < there) *reinterpret_cast<Raw*>(to + k * s.t) = Raw{};
+}
+
 // a float2 (VEC = 2) or float per lane and quantity, in shared memory of any CTA of the cluster
 template <int VEC> struct Span { float a[VEC], h[VEC]; };
 
@@ -468,8 +478,8 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
 #pragma unroll
     for (int j = 0; j < VEC; ++j) state[j] = p.initial && on ? p.initial[b * p.initial_b + (d + j) * p.initial_d] : 0.0f;
 
-    uint32_t buf = 0;
-    for (uint32_t first = 0; first < chunks; first += cluster, buf ^= 1) {
+    uint32_t buf = 0, first = 0;
+    for (; first * kRecurrenceChunk < n; first += cluster, buf ^= 1) {
         const uint32_t chunk = first + rank, t0 = first_step(first), live = live_from(t0);
         const bool whole = live >= kSpanSteps;
         if constexpr (SRC == kFromWords) {
@@ -581,6 +591,14 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
             }
         }
     }
+    for (; first + rank < chunks; first += cluster) {             // nothing but padding
+        const uint32_t t0 = first_step(first);
+        if (on && t0 < p.T) write_zeros<T, VEC>(p.y, b, d, t0, p.T - t0);
+        if (p.states && warp == 0 && on) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) p.states[b * p.states_b + (first + rank) * p.states_c + (d + j) * p.states_d] = state[j];
+        }
+    }
     if constexpr (SRC == kFromTiles) {
         if (lane == 0) bulk_wait_group<0>();
     }
@@ -662,16 +680,28 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
     } else {
         __syncthreads();
     }
-    fetch(0, 0);
-    if constexpr (SRC == kFromTiles) fetch(cluster, 1);
-    fetch_state(0);
+    // the groups of spans behind the sequence
+    const uint32_t live_chunks = (n + kRecurrenceChunk - 1) / kRecurrenceChunk, dead = (chunks - live_chunks) / cluster * cluster;
+    fetch(dead, 0);
+    if constexpr (SRC == kFromTiles) fetch(dead + cluster, 1);
+    fetch_state(dead);
+    if (on) {
+        for (uint32_t done = 0; done < dead; done += cluster) {
+            const uint32_t t0 = chunk_start(done) + warp * kSpanSteps;
+            if (t0 >= p.T) continue;
+            write_zeros<T, VEC>(p.dx, b, d, t0, p.T - t0);
+            write_zeros<T, VEC>(p.df, b, d, t0, p.T - t0);
+            if constexpr (HAS_I) write_zeros<T, VEC>(p.di, b, d, t0, p.T - t0);
+            if constexpr (HAS_O) write_zeros<T, VEC>(p.dout, b, d, t0, p.T - t0);
+        }
+    }
 
     float carry[VEC];                                       // f_{t+1} dc_{t+1} behind what is left
 #pragma unroll
     for (int j = 0; j < VEC; ++j) carry[j] = p.dlast && on ? p.dlast[b * p.dlast_b + (d + j) * p.dlast_d] : 0.0f;
 
     uint32_t buf = 0;
-    for (uint32_t done = 0; done < chunks; done += cluster, buf ^= 1) {
+    for (uint32_t done = dead; done < chunks; done += cluster, buf ^= 1) {
         const uint32_t start = chunk_start(done), t0 = start + warp * kSpanSteps, live = live_from(t0);
         const bool whole = live >= kSpanSteps;
         const uint32_t stage = buf * kStageBytes;
@@ -729,7 +759,7 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
         __syncthreads();
         // everyone is done with the other stage: this one is read again below, so that its elements need no registers meanwhile
         if constexpr (SRC == kFromTiles) {
-            if (done > 0) fetch(done + cluster, buf ^ 1);
+            if (done > dead) fetch(done + cluster, buf ^ 1);
         }
         // this CTA's spans from the end: `whole_span` all of them, `behind` those after this warp's; and the state before this warp's
         Span<VEC> whole_span, behind;

@@ -733,7 +733,8 @@ struct Prepared {
 
 // Tensor map of an output view for the epilogue's bulk stores: boxes of 32 rows x 128 bytes,
 // 128-byte swizzle.  `base` is the view's first element (the caller's buffer, or the same view
-// in a peer's buffer).  False when the view is not TMA-addressable.
+// in a peer's buffer).  False when the view is not TMA-addressable, or when its rows end inside 16
+// bytes: a box is cut at whole 16 bytes, and what lies there behind the row would be overwritten.
 bool encode_out_map(CUtensorMap* map, const Problem& Q, long long ldo, void* base)
 {
     const CUtensorMapDataType dt = Q.type == real32F ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
@@ -743,7 +744,7 @@ bool encode_out_map(CUtensorMap* map, const Problem& Q, long long ldo, void* bas
     cuuint64_t gdim[3] = {Q.N, Q.M, one ? 1 : Q.batch};
     cuuint64_t gstride[2] = {(cuuint64_t)ldo * Q.elem, one ? (cuuint64_t)ldo * Q.elem * Q.M : (cuuint64_t)Q.o_b * Q.elem};
     cuuint32_t box[3] = {kRowBytes / Q.elem, 32, 1}, estr[3] = {1, 1, 1};
-    if (reinterpret_cast<uintptr_t>(base) % 16 != 0) return false;
+    if (reinterpret_cast<uintptr_t>(base) % 16 != 0 || (Q.N * Q.elem) % 16 != 0) return false;
     return gstride[1] % 16 == 0 && gstride[0] < (1ull << 40) && gstride[1] < (1ull << 40) &&
            g_encode(map, dt, 3, base, gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                     CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

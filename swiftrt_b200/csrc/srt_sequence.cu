@@ -169,13 +169,15 @@ template <> constexpr CUtensorMapDataType kMapType<__half> = CU_TENSOR_MAP_DATA_
 template <> constexpr CUtensorMapDataType kMapType<__nv_bfloat16> = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 
 // Tensor maps of every tensor of the call, boxes of 128 bytes of channels by 64 steps (inputs) or 8 steps (results); false when one
-// cannot have it: rows that do not start on 16 bytes, channels apart from each other, repeated or overlapping rows.
+// cannot have it: rows that do not start on 16 bytes, channels apart from each other, repeated or overlapping rows; or channels
+// that end inside 16 bytes, which the boxes of the results would write whole.
 template <typename T>
 bool encode_maps(const RecurrenceParams& p, EncodeTiledFn encode, RecurrenceMaps& maps)
 {
     auto one = [&](const void* ptr, long long b, long long t, long long d, uint32_t steps, CUtensorMap* map) {
         if (!ptr) return true;
         const long long elem = sizeof(T);
+        if (p.D * elem % 16 != 0) return false;
         if (p.T == 1) t = (long long)(p.D + 7) / 8 * 8;
         if (p.B == 1) b = t;
         if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0 || (d != 1 && p.D > 1) || t < (long long)p.D || b <= 0 || t * elem % 16 != 0 || b * elem % 16 != 0 ||

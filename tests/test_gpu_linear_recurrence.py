@@ -120,6 +120,38 @@ def test_column_blocks_other_strides_and_outputs_in_place_of_a_view(srt, dtype):
         ref.check(got, *want[name], name)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("gate_in", [False, True], ids=["fo", "fio"])
+@pytest.mark.parametrize("D", [66, 67, 68])
+def test_column_blocks_that_start_but_do_not_end_on_16_bytes(srt, dtype, gate_in, D):
+    """66 to 68 channels in blocks of 72: rows are aligned as for whole tiles, the last channel may have no partner, and
+    what lies between the blocks stays as it is."""
+    dt, B, T, pitch = TYPES[dtype], 3, 140, 72
+    tensors = _make(B, T, D, dt, gate_in, True)
+
+    def wide(fill):
+        return torch.full((B, T, 5 * pitch), fill, dtype=dt, device=DEV)
+
+    def blocks(w):
+        return [w[..., k * pitch:k * pitch + D] for k in range(5)]
+
+    source = wide(float("nan"))
+    inputs = []
+    for view, t in zip(blocks(source), tensors):
+        inputs.append(None if t is None else view.copy_(t))
+    lengths = torch.tensor([T, 70, 3], dtype=torch.int32, device=DEV)
+    fw, _, _, states = _check_forward(srt, tuple(inputs), _state(B, D), lengths)
+    dy = blocks(source)[4].copy_(torch.randn(B, T, D, generator=torch.Generator().manual_seed(4)).to(dt).to(DEV))
+    result = wide(7.0)
+    outs = [v if t is not None else None for v, t in zip(blocks(result), tensors)]
+    srt.gated_recurrence_backward(dy, *inputs, states, lengths, out=tuple(outs))
+    want = ref.backward(dy, fw, inputs[0], inputs[2], inputs[3])
+    for k, (name, got) in enumerate(zip(("update", "forget", "input", "output"), outs)):
+        if got is not None:
+            ref.check(got, *want[name], name)
+        assert bool((result[..., k * pitch + D:(k + 1) * pitch] == 7).all()), "written behind a block"
+
+
 @pytest.mark.parametrize("T", [1, 70, 300])
 def test_what_lies_behind_a_sequence_is_never_read(srt, T):
     """NaN and infinities behind the lengths, and lengths outside 0 .. T, which are taken as the nearest of them."""

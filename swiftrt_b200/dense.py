@@ -154,7 +154,10 @@ class GatedDense:
         def like(t, wanted=True):
             return torch.empty(t.shape, dtype=x.dtype, device=x.device) if wanted else None
 
-        dgate, dup, dx, dwg, dwu = like(gate), like(up), like(x), like(self.weight_gate), like(self.weight_up)
+        def two(t):                             # side by side: the weights' gradients are one batch of two
+            return torch.empty((2, *t.shape), dtype=x.dtype, device=x.device)
+
+        (dgate, dup), dx, (dwg, dwu) = two(gate), like(x), two(self.weight_gate)
         dbg = like(self.bias_gate) if self.bias_gate is not None else None
         dbu = like(self.bias_up) if self.bias_up is not None else None
 

@@ -282,3 +282,38 @@ def test_the_wait_limit_ends_the_fused_kernels_in_order(srt):
     assert torch.equal(layer(x), want) and srt.check_status() == 0
     for a, b in zip(grads, layer.backward(x, saved, dy)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("M,K,H", [(65, 96, 72), (520, 264, 300)])
+def test_weight_gradients_wherever_the_pairs_lie(srt, dtype, M, K, H):
+    """The second of dGate / dUp and of dWGate / dWUp before or behind the first one, apart or as column blocks of one
+    matrix.  Small integers and the identity: every sum is exact, the result has one right value."""
+    from swiftrt_b200._lib import lib
+    from swiftrt_b200.matmul import descriptor_args, enqueue
+    dt, g = TYPES[dtype], torch.Generator().manual_seed(M)
+    ints = lambda *s: torch.randint(-1, 2, s, generator=g).to(dt).to(DEV)  # noqa: E731
+    x, wg, wu, gate, up, dy = ints(M, K), ints(K, H), ints(K, H), ints(M, H), ints(M, H), ints(M, H)
+    dg, du = dy.double() * up.double(), dy.double() * gate.double()
+    want = [(x.double().t() @ d).to(dt) for d in (dg, du)]
+
+    def pair(rows, cols, how):
+        if how == "blocks":
+            pitch = (cols + 7) // 8 * 8
+            w = torch.full((rows, 2 * pitch), 7.0, dtype=dt, device=DEV)
+            return w[:, :cols], w[:, pitch:pitch + cols], w
+        w = torch.full((2, rows, cols), 7.0, dtype=dt, device=DEV)
+        return (w[0], w[1], w) if how == "behind" else (w[1], w[0], w)
+
+    for first in ("behind", "before", "blocks"):
+        for second in ("behind", "before", "blocks"):
+            dgate, dup, _ = pair(M, H, first)
+            dwg, dwu, wide = pair(K, H, second)
+            enqueue(lib.srtMatmulGatedBackward, x.device, *descriptor_args(dy, x, wg, wu, gate, up), int(srt.ActivationType.identity),
+                    *descriptor_args(dgate, dup, None, None, dwg, dwu, None, None))
+            srt.check_status(DEV)
+            assert torch.equal(dgate.double(), dg) and torch.equal(dup.double(), du)
+            assert torch.equal(dwg, want[0]) and torch.equal(dwu, want[1]), (first, second)
+            if second == "blocks":
+                pitch = wide.shape[1] // 2
+                assert bool((wide[:, H:pitch] == 7).all()) and bool((wide[:, pitch + H:] == 7).all())

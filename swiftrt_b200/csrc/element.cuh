@@ -108,6 +108,24 @@ template <typename T> __device__ __forceinline__ float gate_slope(uint32_t act, 
     }
 }
 
+// s(a), and s(a) with 1 - s(a), each to a relative error of a few 2^-23: with e = exp(-a) they are 1 / (1 + e) and
+// e / (1 + e), neither of which is the difference of 1 and its neighbour (a gate at 0.9999 keeps its decay 1 - f to full
+// precision).  The .ftz forms of the two approximations take one instruction each where the others rescale denormals
+// around them.  For the pair e is capped at 2^126, so that a closed gate is 2^-126 and not 0 times infinity.
+struct Gate { float on, off; };
+__device__ __forceinline__ float min_or_nan(float a, float b)
+{
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ Gate logistic_pair(float a)
+{
+    const float e = exp2_ftz(min_or_nan(-kLog2E * a, 126.0f));
+    const float on = reciprocal_ftz(1.0f + e);
+    return Gate{on, e * on};
+}
+
 // activation and slope of VEC values, what they share computed once; the selector is uniform, so the switch is taken once
 template <typename T, int VEC> __device__ __forceinline__ void gate_values(uint32_t act, const float (&z)[VEC], float (&a)[VEC], float (&slope)[VEC])
 {
@@ -115,9 +133,9 @@ template <typename T, int VEC> __device__ __forceinline__ void gate_values(uint3
         if (act == kActSilu) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float s = logistic(z[j]);
-                a[j] = z[j] * s;
-                slope[j] = fmaf(a[j], logistic(-z[j]), s);           // s + z s (1 - s), with 1 - s not as a difference
+                const Gate s = logistic_pair(z[j]);
+                a[j] = z[j] * s.on;
+                slope[j] = fmaf(a[j], s.off, s.on);                  // s + z s (1 - s), with 1 - s not as a difference
             }
             return;
         }

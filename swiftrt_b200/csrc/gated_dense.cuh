@@ -57,7 +57,7 @@ struct GateBackwardParams {
 // (grid y) walk the same columns at interleaved groups of 32 rows; the column sums of a cluster's CTAs are added in rank order
 // through distributed shared memory, so they need no scratch memory and no atomics.  The unrounded fp32 values are summed.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
 gate_backward_kernel(const __grid_constant__ GateBackwardParams p)
 {
     __shared__ float sums[2][8][8 * VEC];
@@ -90,18 +90,22 @@ gate_backward_kernel(const __grid_constant__ GateBackwardParams p)
                 const long long r = static_cast<long long>(r0) + k * static_cast<long long>(step);
                 if (r >= p.M) continue;
                 __align__(16) T dg[VEC], du[VEC];
-                float z[VEC], value[VEC], slope[VEC];
+                constexpr int kPart = VEC < 4 ? VEC : 4;                      // registers for four values at a time
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) z[j] = to_float<T>(g[k][j]);
-                gate_values<T, VEC>(p.act, z, value, slope);
+                for (int i = 0; i < VEC; i += kPart) {
+                    float z[kPart], value[kPart], slope[kPart];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float d = to_float<T>(dy[k][j]);
-                    const float vg = d * to_float<T>(u[k][j]) * slope[j], vu = d * value[j];
-                    dg[j] = from_float<T>(vg);
-                    du[j] = from_float<T>(vu);
-                    sg[j] += vg;
-                    su[j] += vu;
+                    for (int j = 0; j < kPart; ++j) z[j] = to_float<T>(g[k][i + j]);
+                    gate_values<T, kPart>(p.act, z, value, slope);
+#pragma unroll
+                    for (int j = 0; j < kPart; ++j) {
+                        const float d = to_float<T>(dy[k][i + j]);
+                        const float vg = d * to_float<T>(u[k][i + j]) * slope[j], vu = d * value[j];
+                        dg[i + j] = from_float<T>(vg);
+                        du[i + j] = from_float<T>(vu);
+                        sg[i + j] += vg;
+                        su[i + j] += vu;
+                    }
                 }
                 T* a = static_cast<T*>(p.dg.p) + r * p.dg.m + col * p.dg.n;
                 T* b = static_cast<T*>(p.du.p) + r * p.du.m + col * p.du.n;

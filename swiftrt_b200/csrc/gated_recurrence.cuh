@@ -41,24 +41,6 @@ struct RecurrenceParams {
     unsigned long long wait_cycles;
 };
 
-// s(a), and s(a) with 1 - s(a), each to a relative error of a few 2^-23: with e = exp(-a) they are 1 / (1 + e) and
-// e / (1 + e), neither of which is the difference of 1 and its neighbour (a gate at 0.9999 keeps its decay 1 - f to full
-// precision).  The .ftz forms of the two approximations take one instruction each where the others rescale denormals
-// around them.  For the pair e is capped at 2^126, so that a closed gate is 2^-126 and not 0 times infinity.
-struct Gate { float on, off; };
-__device__ __forceinline__ float min_or_nan(float a, float b)
-{
-    float y;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
-__device__ __forceinline__ Gate logistic_pair(float a)
-{
-    const float e = exp2_ftz(min_or_nan(-kLog2E * a, 126.0f));
-    const float on = reciprocal_ftz(1.0f + e);
-    return Gate{on, e * on};
-}
-
 // Two neighbouring channels at a time where VEC is 2 (one instruction for both products or sums)
 template <int VEC> __device__ __forceinline__ void mul_to(float (&d)[VEC], const float (&a)[VEC], const float (&b)[VEC])
 {

@@ -119,10 +119,11 @@ struct RowsPlan {
     uint32_t groups = 0, cluster = 0, stages = 0, k_per_part = 0, x_pitch = 0, x_bytes = 0;
 };
 
-// The choice of column tiles to a CTA and CTAs to a cluster by what it costs: rounds of CTAs (4 us and what they stream), x to bring in
-// before the first product, the exchange of a cluster, SMs without work or with one CTA's eight warps only.  One row, 4096 x 16384
-// in 4 bits, tiles x cluster: 8 x 4 17.0, 4 x 2 17.0, 2 x 1 16.4 us; 8 x 2 21.3, 8 x 8 22.5 us.  16 rows, 4096 x 2 x 16384 in bf16:
-// 8 x 4 56, 4 x 2 64, 2 x 1 76, 8 x 8 83 us.
+// The choice of column tiles to a CTA and CTAs to a cluster by what it costs: rounds of CTAs and what they stream, x to bring in before
+// the first product, the exchange of a cluster, SMs with one CTA's eight warps only, and the places that clusters of 4 and 8 leave
+// free.  The constants are fitted to the times of all choices at 9 shapes of 4-bit and 6 of 16-bit weights and 1 .. 48 rows; the choice is
+// on average 4 % slower than the best one.  One row, 4096 x 16384 in 4 bits, tiles x cluster: 8 x 4 17.0, 4 x 2 17.0, 2 x 1 16.4 us; 8 x 2
+// 21.3, 8 x 8 22.5 us.  17 rows, 8192 x 1024: 2 x 8 in rows of 8 13.3, in rows of 32 19.6 us.
 template <typename T, typename Format, int NW, int NT>
 cudaError_t plan_few_rows(const FewRowsParams& p, RowsPlan& best)
 {
@@ -154,11 +155,11 @@ cudaError_t plan_few_rows(const FewRowsParams& p, RowsPlan& best)
             if (stages > rounds) stages = rounds;
             if (stages == 0) continue;
             const uint32_t at_once = per_sm > 2 ? 2 : per_sm;
-            const double places = 148.0 * at_once, full = (double)((tiles + g - 1) / g) * row_blocks * c / places;
-            const double stream = rounds * stage_bytes * places / 5.5e6;                    // a round of CTAs at 5.5 TB/s
-            double cost = std::ceil(full) * (4.0 + stream * (at_once == 1 && Format::kGroups ? 1.6 : 1.0)) + x_bytes / 1024.0 * 0.06;
-            if (full < 0.5) cost -= stream * (0.5 - full);                                  // (few CTAs share the bandwidth)
-            if (c > 1) cost += 0.8 + 0.15 * c;
+            const double places = 148.0 * at_once * (c == 8 ? 0.45 : c == 4 ? 0.93 : 1.0), full = (double)((tiles + g - 1) / g) * row_blocks * c / places;
+            const double waves = std::ceil(full), stream = rounds * stage_bytes * places / 5.5e6 * (at_once == 1 && Format::kGroups ? 1.4 : 1.0);  // a round at 5.5 TB/s
+            double cost = waves * (7.3 + (Format::kGroups ? 0.6 * rounds : 0.0)) + stream * (0.15 * waves + 0.85 * (full > 0.25 ? full : 0.25)) + x_bytes / 1024.0 * 0.04 +
+                          0.1 * NW * NT;
+            if (c > 1) cost += 1.0 + 0.3 * c;
             if (cost < best.cost) {
                 best.cost = cost;
                 best.groups = g; best.cluster = c; best.stages = stages;

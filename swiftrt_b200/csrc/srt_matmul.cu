@@ -1732,9 +1732,9 @@ cudaError_t gated_fused(srtDataType type, const Matrix& x, const Matrix& wg, con
 }
 
 // Up to kFewRows rows the weights are streamed past them (few_rows.cuh); up to kSomeRows where that is estimated to be faster
-// than the tensor cores' tiles: a tile is 128 columns by 256 rows whatever M is, and takes 0.4 us for every 64 of K, 8 us around them
-// (17 .. 256 rows of 2048 x 2 x 2048 19 us, of 4096 x 2 x 16384 64 us, of 1024 x 2 x 4096 15 us; streamed, 16 rows of the same 11, 52 and
-// 17 us, 48 rows 20, - and 31 us).  The estimate of the streaming kernel is 1.3 times too low from 9 rows on.
+// than the tensor cores' tiles: a tile is 128 columns by 256 rows whatever M is, and takes 0.4 us for every 64 of K, 12 us around them
+// (17 .. 256 rows of 2048 x 2 x 2048 19 us, of 4096 x 2 x 16384 64 us, of 1024 x 2 x 4096 15 us; streamed, 16 rows of the same 11, 53 and
+// 11 us, 32 rows 15, - and 13 us).
 constexpr uint64_t kFewRows = 8, kSomeRows = 128;
 
 // the gated product of a few rows; any strides of x and the results, weights contiguous along K or along their columns.
@@ -1772,7 +1772,7 @@ cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, cons
     if (if_faster && x.rows > kFewRows) {
         if (!p.w[0].vec || !p.w[1].vec) return cudaErrorNotSupported;
         const uint64_t tiles = (wg.cols + 127) / 128;
-        limit = ((double)((tiles + 73) / 74) * (double)((x.cols + 63) / 64) * 0.4 + 8.0) / 1.3;
+        limit = (double)((tiles + 73) / 74) * (double)((x.cols + 63) / 64) * 0.4 + 12.0;
     }
     return gated_few_rows(type, p, !by_rows, limit, device, stream);
 }

@@ -60,6 +60,13 @@ void on_one_device(std::initializer_list<const at::Tensor*> tensors)
         }
 }
 
+bool truth(PyObject* o)
+{
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw PythonError{};
+    return v != 0;
+}
+
 srtDataType data_type(const at::Tensor& t)
 {
     switch (t.scalar_type()) {
@@ -177,7 +184,7 @@ PyObject* recurrence(PyObject*, PyObject* const* a, Py_ssize_t n)
         const at::Tensor& forget = tensor(a[1], "forget");
         const at::Tensor *input = tensor_or_null(a[2], "input"), *output = tensor_or_null(a[3], "output"), *initial = tensor_or_null(a[4], "initial"),
                          *lengths = tensor_or_null(a[5], "lengths"), *given = tensor_or_null(a[7], "last");
-        const bool keep = a[6] == Py_True;
+        const bool keep = truth(a[6]);
         on_one_device({&update, &forget, input, output, initial, lengths, given});
         sequence_rank(update);
         const int64_t batch = update.size(0), channels = update.size(-1), steps = update.dim() == 3 ? update.size(1) : 1;
@@ -239,7 +246,7 @@ PyObject* gated(PyObject*, PyObject* const* a, Py_ssize_t n)
         const at::Tensor& wu = tensor(a[2], "weight_up");
         const at::Tensor *bg = tensor_or_null(a[3], "bias_gate"), *bu = tensor_or_null(a[4], "bias_up");
         const auto act = static_cast<srtActivationType>(PyLong_AsLong(a[5]));
-        const bool keep = a[6] == Py_True;
+        const bool keep = truth(a[6]);
         on_one_device({&x, &wg, &wu, bg, bu});
         if (x.dim() != 2 || wg.dim() != 2) {
             PyErr_SetString(PyExc_ValueError, "matrices expected");

@@ -41,12 +41,17 @@ class Int4Weight:
         on_one_device(packed, scales, zeros)
         packed, scales = _on_rows_of(packed, 16), _on_rows_of(scales, 8)
         zeros = _on_rows_of(zeros, 4) if zeros is not None else None
-        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self._tensors = packed, scales, zeros
         self.shape, self.dtype, self.device = (self.rows, self.cols), scales.dtype, packed.device
         stride = lambda t: max(t.stride(0), self.cols)  # noqa: E731  (a single row may have any stride)
         self._struct = _lib.Int4Matrix(data_type(scales), self.group, self.rows, self.cols, packed.data_ptr(), stride(packed), scales.data_ptr(),
                                        stride(scales), zeros.data_ptr() if zeros is not None else None, stride(zeros) if zeros is not None else 0)
         self.address = ctypes.addressof(self._struct)
+
+    # (the library holds their addresses: their elements may change, the tensors may not)
+    packed = property(lambda self: self._tensors[0])
+    scales = property(lambda self: self._tensors[1])
+    zeros = property(lambda self: self._tensors[2])
 
     def dequantize(self) -> torch.Tensor:
         """The weight as a [rows, cols] tensor of its type, each element rounded once (srtDequantizeInt4)."""

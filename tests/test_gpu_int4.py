@@ -223,3 +223,16 @@ def test_streams_graphs_and_repeats_give_the_same_bits(srt):
         torch.cuda.synchronize()
         for a, b, c, d in zip(want, other, captured, again):
             assert torch.equal(a, b) and torch.equal(a, c) and torch.equal(a, d)
+
+
+def test_a_weight_keeps_its_tensors(srt):
+    """The library holds their addresses: elements may change in place, a tensor may not take another's place."""
+    K, N = 128, 64
+    w = _weight(srt, K, N, 64, torch.bfloat16, True)
+    for name in ("packed", "scales", "zeros"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, getattr(w, name).clone())
+    x = torch.randn(2, K, device=DEV).to(torch.bfloat16)
+    once = srt.matmul_int4(x, w)
+    w.scales.mul_(2)
+    assert torch.equal(srt.matmul_int4(x, w), once * 2)

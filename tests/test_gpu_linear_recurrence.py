@@ -202,6 +202,7 @@ def test_no_steps_no_items_and_one_step_forms(srt):
     grads = srt.gated_recurrence_backward(empty, empty, empty, None, None, states, last_grad=state)
     assert torch.equal(grads[-1], state)
     assert bool((srt.gated_recurrence(empty, empty)[1] == 0).all())
+    assert len(srt.gated_recurrence(empty, empty, keep=1)) == 3
     none = torch.empty(0, 4, D, device=DEV)
     assert srt.gated_recurrence(none, none)[0].shape == (0, 4, D)
     # rank 2 is one step; a state advances in place

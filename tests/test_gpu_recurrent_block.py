@@ -1,5 +1,10 @@
 """The language-model operators together: a residual block of a linear recurrence and a gated feed-forward layer, trained
 on a padded batch, then quantized to 4 bits and run token by token."""
+import os
+import subprocess
+import sys
+import threading
+
 import pytest
 import torch
 
@@ -109,3 +114,105 @@ def test_generation_with_4_bit_weights_follows_the_sequence(srt):
     # rounding of at most 2^-8 at each of the five tensors between the operators, and 2^-9 for the dequantized weights
     off = float((got - want).norm() / want.norm())
     assert off <= 6 * 2.0 ** -8, off
+
+
+FIRST_CALLS = """
+import sys, torch
+import swiftrt_b200 as srt
+DEV = "cuda:0"
+which = sys.argv[1]
+r = lambda *s: torch.randn(*s, device=DEV).to(torch.bfloat16)
+if which == "token":
+    args = [r(2, 96) for _ in range(4)]
+    call = lambda: srt.gated_recurrence(*args)
+elif which == "sequence":
+    args = [r(2, 200, 96) for _ in range(4)]
+    call = lambda: srt.gated_recurrence(*args, keep=True)
+elif which == "few":
+    x, wg, wu = r(3, 128), r(128, 256), r(128, 256)
+    call = lambda: (srt.GatedDense(wg, wu)(x),)
+elif which == "tiles":
+    x, wg, wu = r(300, 128), r(128, 256), r(128, 256)
+    call = lambda: srt.GatedDense(wg, wu).forward_keep(x)[1]
+elif which == "int4":
+    x = r(3, 128)
+    packed = torch.randint(-2 ** 31, 2 ** 31 - 1, (16, 96), device=DEV, dtype=torch.int64).to(torch.int32)
+    w = srt.Int4Weight(packed, torch.rand(1, 96, device=DEV).to(torch.bfloat16), None, 128, 128)
+    call = lambda: (srt.matmul_int4(x, w),)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = call()
+for t in captured:
+    t.zero_()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(captured, call()):
+    assert torch.equal(a, b)
+srt.check_status(DEV)
+print("right")
+"""
+
+
+@pytest.mark.parametrize("which", ["token", "sequence", "few", "tiles", "int4"])
+def test_the_first_call_of_a_process_may_be_captured(which):
+    """What a first call sets up (kernel attributes, the status word) is set up under a capture as well."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS, which], capture_output=True, text=True, timeout=300,
+                          env={**os.environ, "PYTHONPATH": root})
+    assert done.returncode == 0 and "right" in done.stdout, done.stdout + done.stderr
+
+
+def test_threads_and_graphs_at_once_give_the_same_bits(srt):
+    """Four threads on their own streams, then two captured copies of the same calls replayed on two streams at once."""
+    g = torch.Generator().manual_seed(6)
+    r = lambda *s, scale=1.0: (torch.randn(*s, generator=g) * scale).to(torch.bfloat16).to(DEV)  # noqa: E731
+    sequence, dy = [r(3, 300, 200) for _ in range(4)], r(3, 300, 200)
+    layer = srt.GatedDense(r(256, 512, scale=0.06), r(256, 512, scale=0.06))
+    rows, weight = [r(m, 256) for m in (1, 20, 100, 400)], srt.quantize_int4(r(256, 512))
+
+    def work():
+        kept = srt.gated_recurrence(*sequence, keep=True)
+        out = [*kept, *srt.gated_recurrence_backward(dy, *sequence, kept[2])]
+        for x in rows:
+            y, saved = layer.forward_keep(x)
+            out += [y, layer(x), srt.matmul_int4(x, weight), *(t for t in layer.backward(x, saved, y) if t is not None)]
+        return out
+
+    want = [t.clone() for t in work()]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def thread(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    got = work()
+                    stream.synchronize()
+                    wrong.extend((i, k) for k, (a, b) in enumerate(zip(want, got)) if not torch.equal(a, b))
+                stream.synchronize()
+        except Exception as e:  # noqa: BLE001  (shown by the assertion below)
+            wrong.append((i, repr(e)))
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:10]
+    graphs, captured = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured.append(work())
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    srt.check_status(DEV)
+    for got in captured:
+        assert [k for k, (a, b) in enumerate(zip(want, got)) if not torch.equal(a, b)] == []

@@ -15,6 +15,7 @@
 
 #include <initializer_list>
 #include <optional>
+#include <utility>
 
 #include "srt_matmul_api.h"
 
@@ -273,6 +274,48 @@ PyObject* gated(PyObject*, PyObject* const* a, Py_ssize_t n)
     });
 }
 
+// (x, outGrad, wGate, wUp, gate, up, biasGate, biasUp, activation) -> gradients of x, wGate, wUp, biasGate and biasUp (None where the
+// bias is None)
+PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 9, [&]() -> PyObject* {
+        const at::Tensor &x = tensor(a[0], "input"), &grad = tensor(a[1], "out_grad"), &wg = tensor(a[2], "weight_gate"), &wu = tensor(a[3], "weight_up"),
+                         &gate = tensor(a[4], "saved"), &up = tensor(a[5], "saved");
+        const at::Tensor *bg = tensor_or_null(a[6], "bias_gate"), *bu = tensor_or_null(a[7], "bias_up");
+        const auto act = static_cast<srtActivationType>(PyLong_AsLong(a[8]));
+        on_one_device({&x, &grad, &wg, &wu, &gate, &up, bg, bu});
+        if (x.dim() != 2 || wg.dim() != 2) {
+            PyErr_SetString(PyExc_ValueError, "matrices expected");
+            throw PythonError{};
+        }
+        Queue q(x);
+        const at::ScalarType type = x.scalar_type();
+        const int64_t rows = x.size(0), inner = x.size(1), cols = wg.size(1);
+        const at::Tensor dgate = empty({rows, cols}, type, x.device()), dup = empty({rows, cols}, type, x.device()), dx = empty({rows, inner}, type, x.device());
+        at::Tensor dwg = empty({inner, cols}, type, x.device()), dwu = empty({inner, cols}, type, x.device());
+        // both pairs in one direction: one batched product gives both
+        if ((dup.data_ptr() > dgate.data_ptr()) != (dwu.data_ptr() > dwg.data_ptr())) std::swap(dwg, dwu);
+        at::Tensor dbg, dbu, dx2;
+        if (bg) dbg = empty(bg->sizes(), type, x.device());
+        if (bu) dbu = empty(bu->sizes(), type, x.device());
+        auto opt = [](const at::Tensor& t) { return t.defined() ? &t : nullptr; };
+        const Arg ay(grad), ax(x), ag(wg), au(wu), kg(gate), ku(up), dg(dgate), du(dup), ox(dx), og(dwg), ou(dwu), sg(opt(dbg)), su(opt(dbu));
+        auto call = [&] {
+            const Arg ox2(opt(dx2));
+            return srtMatmulGatedBackward(ay.p, ay.desc, ax.p, ax.desc, ag.p, ag.desc, au.p, au.desc, kg.p, kg.desc, ku.p, ku.desc, act, dg.p, dg.desc, du.p, du.desc,
+                                          ox.p, ox.desc, ox2.p, ox2.desc, og.p, og.desc, ou.p, ou.desc, sg.p, sg.desc, su.p, su.desc, q.stream);
+        };
+        cudaError_t rc = cudaErrorNotSupported;
+        if (type != at::kFloat) rc = call();
+        if (rc == cudaErrorNotSupported) {                       // an input gradient in two products needs a place for the second
+            dx2 = empty({rows, inner}, type, x.device());
+            rc = call();
+        }
+        check(rc);
+        return pack({&dx, &dwg, &dwu, &dbg, &dbu});
+    });
+}
+
 // (x, address of the weight's srtInt4Matrix, address of a second one or 0, a tensor of the weights, columns, bias, second bias,
 // activation) -> y
 PyObject* int4(PyObject*, PyObject* const* a, Py_ssize_t n)
@@ -314,6 +357,7 @@ PyMethodDef kMethods[] = {
     {"recurrence", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(recurrence)), METH_FASTCALL, nullptr},
     {"recurrence_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(recurrence_backward)), METH_FASTCALL, nullptr},
     {"gated", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated)), METH_FASTCALL, nullptr},
+    {"gated_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gated_backward)), METH_FASTCALL, nullptr},
     {"int4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(int4)), METH_FASTCALL, nullptr},
     {"set_error_classes", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(set_error_classes)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -10,7 +10,7 @@ import torch
 from . import _lib
 from ._lib import lib
 from .int4 import Int4Weight, gated_matmul_int4, matmul_int4
-from .matmul import MatmulError, _descriptor, binding, descriptor_args, enqueue, matmul, on_one_device
+from .matmul import MatmulError, _descriptor, binding, matmul
 from .tensor import ActivationType, order_of
 
 
@@ -148,27 +148,7 @@ class GatedDense:
         """Gradients of (input, weightGate, weightUp, biasGate, biasUp); None for a bias that is None.  `saved` is the
         second value of forward_keep."""
         gate, up = saved
-        on_one_device(input, out_grad, gate, up, self.weight_gate, self.weight_up)
-        x, dy = input.reshape(-1, input.shape[-1]), out_grad.reshape(-1, out_grad.shape[-1])
-
-        def like(t, wanted=True):
-            return torch.empty(t.shape, dtype=x.dtype, device=x.device) if wanted else None
-
-        def two(t):                             # side by side: the weights' gradients are one batch of two
-            return torch.empty((2, *t.shape), dtype=x.dtype, device=x.device)
-
-        (dgate, dup), dx, (dwg, dwu) = two(gate), like(x), two(self.weight_gate)
-        dbg = like(self.bias_gate) if self.bias_gate is not None else None
-        dbu = like(self.bias_up) if self.bias_up is not None else None
-
-        def call(dx2):
-            enqueue(lib.srtMatmulGatedBackward, x.device, *descriptor_args(dy, x, self.weight_gate, self.weight_up, gate, up), int(self.activation),
-                    *descriptor_args(dgate, dup, dx, dx2, dwg, dwu, dbg, dbu))
-
-        try:
-            call(like(x, x.dtype == torch.float32))
-        except MatmulError as e:
-            if e.code != _lib.cudaErrorNotSupported:
-                raise
-            call(like(x))
+        flat = lambda t: t if t.dim() == 2 else t.reshape(-1, t.shape[-1])  # noqa: E731
+        dx, dwg, dwu, dbg, dbu = binding.gated_backward(flat(input), flat(out_grad), self.weight_gate, self.weight_up, gate, up, self.bias_gate,
+                                                        self.bias_up, int(self.activation))
         return dx.view(input.shape), dwg, dwu, dbg, dbu

@@ -440,9 +440,11 @@ cudaError_t srtGruCell(
  * strides (a transposed weight is its descriptor's strides).  gate and up [M x H] (both or neither) receive
  * x . wGate + biasGate and x . wUp + biasUp, rounded once each: what srtMatmulGatedBackward needs.  All activations
  * but clippedRelu and elu; K = 0 is a sum of no terms.  `out`, gate and up must not overlap anything.
- * Float16 / BFloat16 views with 16-byte aligned rows run as one launch in which neither product reaches memory.
- * Others (Float32 among them) run as two products and an elementwise pass over gate and up, which are rounded to the
- * element type in between; without gate and up that returns cudaErrorNotSupported. */
+ * Float16 / BFloat16 run as one launch in which neither product reaches memory: any number of rows where rows of all
+ * matrices start on 16 bytes (those of results being whole 16 bytes long), and up to 128 rows of any views of x and the results where the
+ * weights are contiguous along K or along H.  Others (Float32 among them) run as two products and an elementwise pass
+ * over gate and up, which are rounded to the element type in between; without gate and up that returns
+ * cudaErrorNotSupported. */
 cudaError_t srtMatmulGated(
     const void* x, const srtTensorDescriptor* xDesc,
     const void* wGate, const srtTensorDescriptor* wGateDesc,
@@ -461,8 +463,10 @@ cudaError_t srtMatmulGated(
  *     dBiasGate, dBiasUp = column sums of dGate and dUp (fp32 sums of the unrounded values)
  * dGate and dUp [M x H] are always written: the products read them, rounded as they are.  dX, dWGate, dWUp, dBiasGate and dBiasUp may be NULL
  * when not wanted.  dX2 [M x K] is scratch for one of dX's two products and may be NULL where dX is one launch
- * (Float16 / BFloat16 views with 16-byte aligned rows); where it is needed and NULL the call returns
- * cudaErrorNotSupported before it launches anything.  With it each of the two products is rounded before their sum is.  Results do not depend on timing.  M, K and H are at least 1.
+ * (Float16 / BFloat16 views whose rows start on 16 bytes, dX's being whole 16 bytes long); where it is needed and NULL
+ * the call returns cudaErrorNotSupported before it launches anything.  With it each of the two products is rounded
+ * before their sum is.  Results do not depend on timing.  M, K and H are at least 1.  Both weights' gradients are one batched product where
+ * dUp and dWUp lie in the same direction from dGate and dWGate, with equal strides.
  * The weight products may use the library's per-(device, stream) workspace, as srtMatmul does. */
 cudaError_t srtMatmulGatedBackward(
     const void* outGrad, const srtTensorDescriptor* outGradDesc,
@@ -508,8 +512,8 @@ typedef struct {
 /* out = activation(x . W + bias): what srtMatmulBiasActivation computes with the weight above.  x [M x rows], out [M x cols] and bias
  * [cols] (NULL: none) have the weight's `type`; x and out any strides, out must not overlap anything.  The products of x
  * and the integers q - z are summed in fp32 and scaled group by group, in fp32: no weight is rounded, and the result is
- * rounded once.  Any M; the weight is read once for every 32 rows, so that many rows are better served by srtDequantizeInt4 and
- * srtMatmul.  One launch, no workspace, and a result that does not depend on timing.  All activations but clippedRelu and elu. */
+ * rounded once.  Any M; the weight is read once for every 8, 16 or 32 rows (gated: 8 or 16; whichever is estimated to be
+ * fastest), so that many rows are better served by srtDequantizeInt4 and srtMatmul.  One launch, no workspace, and a result that does not depend on timing.  All activations but clippedRelu and elu. */
 cudaError_t srtMatmulInt4(
     const void* x, const srtTensorDescriptor* xDesc,
     const srtInt4Matrix* weight,
@@ -559,7 +563,8 @@ cudaError_t srtDequantizeInt4(const srtInt4Matrix* weight, void* out, const srtT
  * states (NULL: not wanted) is Float32 [batch x ceil(steps / 64) x channels] and receives the state before
  * steps 0, 64, 128, ...: what srtGatedRecurrenceBackward needs.
  * Outputs must not overlap each other or an input (but last, see above).  One launch on `stream`, no workspace; no
- * steps: last = initial.  A call without elements launches nothing. */
+ * steps: last = initial.  A call without elements launches nothing.  Waits inside the launches of the gated, 4-bit and
+ * recurrence calls are bounded as those of the products are (srtMatmulSetWaitLimit, srtMatmulCheckStatus). */
 #define SRT_GATED_RECURRENCE_CHUNK 64
 cudaError_t srtGatedRecurrence(
     const void* update, const srtTensorDescriptor* updateDesc,

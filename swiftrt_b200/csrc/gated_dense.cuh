@@ -56,6 +56,8 @@ struct GateBackwardParams {
 // A CTA owns 8 VEC columns: a warp's lanes are 8 column groups by 4 rows, its 8 warps 32 rows.  The CTAs of a cluster
 // (grid y) walk the same columns at interleaved groups of 32 rows; the column sums of a cluster's CTAs are added in rank order
 // through distributed shared memory, so they need no scratch memory and no atomics.  The unrounded fp32 values are summed.
+// Reading three and writing two values an element bounds it: 3999 x 8200 bf16 77 us (4.3 TB/s), without the sums 60 us (5.5 TB/s); the difference
+// is the clusters' end, where every CTA waits for its stores.  Gates of four values at a time and three CTAs an SM: 87 -> 77 us.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256, 3)
 gate_backward_kernel(const __grid_constant__ GateBackwardParams p)

@@ -200,9 +200,8 @@ recurrence_steps_backward_kernel(const __grid_constant__ RecurrenceParams p)
 //
 // How the elements travel (SRC):
 //   kFromTiles   TMA: one thread asks for a [64 steps x 128 bytes] box of every tensor, two spans ahead, and every warp stores its
-//                [8 x 128 bytes] of the results the same way (of up to three): no addresses, bounds or predicates per
-//                element.  Needs 16-byte aligned rows.
-//   kFromWords   cp.async of 4 or 8 bytes, by the thread that will use them (no barrier), one span ahead.
+//                [8 x 128 bytes] of the results the same way: no addresses, bounds or predicates per element.  Needs 16-byte aligned rows.
+//   kFromWords   cp.async of 4 bytes (a Float32, two 16-bit elements), by the thread that will use them (no barrier), one span ahead.
 //   kFromMemory  plain loads: 16-bit elements at odd offsets.
 //
 // HBM is the bound of what has to move (4 to 9 values an element), the kernels come within 0.74 (forward) and 0.67 (backward) of a
@@ -210,7 +209,7 @@ recurrence_steps_backward_kernel(const __grid_constant__ RecurrenceParams p)
 // the scheduler without a ready warp half of the time; the unit for exponentials is 55 % busy, issue slots 50 %.  One reciprocal shared by several gates
 // (the product of their denominators) took 7 of that unit's instructions instead of 12 and 17 % more time: the multiplications it costs
 // lie on the same chains.  A single sequence (8191 x 4096) 74 us; 1530 fp16 channels with all gates, whose rows start on 4 bytes and go
-// through the second path, 31 / 70 us at 5 x 777 steps (1024 channels in tiles, 2 x 1000 steps: 11 / 19 us).
+// through the second path, 33 / 70 us at 5 x 777 steps, 1536 in tiles 25 / 44 us.
 constexpr uint32_t kSpanWarps = 8, kSpanSteps = 8, kSpanThreads = 32 * kSpanWarps, kSpanStages = 2;
 static_assert(kSpanWarps * kSpanSteps == kRecurrenceChunk, "a CTA's span is what lies between two kept states");
 enum : int { kFromMemory = 0, kFromWords = 1, kFromTiles = 2 };
@@ -228,12 +227,6 @@ template <> struct Lane<float, 1> {
     static __device__ __forceinline__ void unpack(Raw r, float (&v)[1]) { v[0] = __uint_as_float(r); }
     static __device__ __forceinline__ Raw pack(const float (&v)[1]) { return __float_as_uint(v[0]); }
     static __device__ __forceinline__ Raw infinity() { return 0x7f800000u; }
-};
-template <> struct Lane<float, 2> {
-    using Raw = uint2;
-    static __device__ __forceinline__ void unpack(Raw r, float (&v)[2]) { v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); }
-    static __device__ __forceinline__ Raw pack(const float (&v)[2]) { return make_uint2(__float_as_uint(v[0]), __float_as_uint(v[1])); }
-    static __device__ __forceinline__ Raw infinity() { return make_uint2(0x7f800000u, 0x7f800000u); }
 };
 template <typename T> struct Lane<T, 1> {
     using Raw = unsigned short;
@@ -266,15 +259,13 @@ template <typename Raw> __device__ __forceinline__ Raw shared_word(uint32_t at)
 {
     Raw r;
     if constexpr (sizeof(Raw) == 2) asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(at) : "memory");
-    else if constexpr (sizeof(Raw) == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(at) : "memory");
-    else asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at) : "memory");
+    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(at) : "memory");
     return r;
 }
 template <typename Raw> __device__ __forceinline__ void store_shared_word(uint32_t at, Raw r)
 {
     if constexpr (sizeof(Raw) == 2) asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(r) : "memory");
-    else if constexpr (sizeof(Raw) == 4) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(r) : "memory");
-    else asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(r.x), "r"(r.y) : "memory");
+    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(r) : "memory");
 }
 
 template <typename T, int VEC> struct SpanTile {
@@ -334,8 +325,7 @@ template <typename T, int VEC, int SRC> __host__ __device__ constexpr uint32_t s
 }
 template <typename T, int VEC, int SRC> __host__ __device__ constexpr uint32_t span_smem_bytes(uint32_t tensors, uint32_t results)
 {
-    // four results do not fit next to the ring of five tensors while two CTAs share an SM: they are stored from registers
-    return kSpanStages * span_stage_bytes<T, VEC, SRC>(tensors) + (SRC == kFromTiles ? (results < 4 ? results : 0) * SpanTile<T, VEC>::kBytes + 128 : 0);
+    return kSpanStages * span_stage_bytes<T, VEC, SRC>(tensors) + (SRC == kFromTiles ? results * SpanTile<T, VEC>::kBytes + 128 : 0);
 }
 
 // Where a warp's results of 8 steps go.
@@ -610,13 +600,12 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
     using Raw = typename L::Raw;
     using Tile = SpanTile<T, VEC>;
     constexpr uint32_t kTensors = 3 + HAS_I + HAS_O, kStageBytes = span_stage_bytes<T, VEC, SRC>(kTensors);
-    constexpr bool kTileStores = SRC == kFromTiles && !(HAS_I && HAS_O);
+    constexpr bool kTileStores = SRC == kFromTiles;
     extern __shared__ __align__(128) uint8_t dynamic_smem[];
     __shared__ SpanBoth<VEC> in_cta[2][kSpanWarps][32];
     __shared__ alignas(16) Span<VEC> in_cluster[2][8][32];
     __shared__ alignas(8) uint64_t full[kSpanStages], arrived[2];
     const uint32_t ring = SRC == kFromTiles ? (smem_u32(dynamic_smem) + 127u) & ~127u : smem_u32(dynamic_smem);
-    const uint32_t staging = ring + kSpanStages * kStageBytes;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster > 1 ? cluster_ctarank() : 0;
     const uint32_t block = blockIdx.x / cluster;
@@ -746,6 +735,9 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
             mul_to<VEC>(mine.e, f[s], mine.e);
         }
         in_cta[buf][warp][lane] = mine;
+        if constexpr (kTileStores) {
+            if (lane == 0) bulk_wait_group_read<0>();             // the results of the last span have left the other stage
+        }
         __syncthreads();
         // everyone is done with the other stage: this one is read again below, so that its elements need no registers meanwhile
         if constexpr (SRC == kFromTiles) {
@@ -793,12 +785,10 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
         }
         fma_to<VEC>(e, behind.a, e, behind.h);
         const uint32_t there = on && t0 < p.T ? p.T - t0 : 0;
-        const StepWriter<T, VEC, kTileStores> out_x(p.dx, b, d, t0, staging, 0), out_f(p.df, b, d, t0, staging, 1), out_i(p.di, b, d, t0, staging, 2),
-            out_o(p.dout, b, d, t0, staging, 2 + HAS_I);
-        if constexpr (kTileStores) {
-            if (lane == 0) bulk_wait_group_read<0>();
-            __syncwarp();
-        }
+        // with tiles every gradient takes its operand's place in the stage, which this thread alone reads and for the last time before
+        const uint32_t tiles = ring + stage;
+        const StepWriter<T, VEC, kTileStores> out_f(p.df, b, d, t0, tiles, 0), out_x(p.dx, b, d, t0, tiles, 1), out_i(p.di, b, d, t0, tiles, 3),
+            out_o(p.dout, b, d, t0, tiles, 3 + HAS_I);
         // the states, and the output gate's gradient, which needs nothing else: its operands make room for the states
         float before[kSpanSteps][VEC];
 #pragma unroll
@@ -868,11 +858,11 @@ recurrence_span_backward_kernel(const __grid_constant__ RecurrenceParams p, cons
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && t0 < p.T) {
-                const uint32_t from = staging + warp * Tile::kWarpBytes;
-                tma_store_3d(&maps.dx, from, d0, t0, b);
-                tma_store_3d(&maps.df, from + Tile::kBytes, d0, t0, b);
-                if constexpr (HAS_I) tma_store_3d(&maps.di, from + 2 * Tile::kBytes, d0, t0, b);
-                if constexpr (HAS_O) tma_store_3d(&maps.dout, from + (2 + HAS_I) * Tile::kBytes, d0, t0, b);
+                const uint32_t from = tiles + warp * Tile::kWarpBytes;
+                tma_store_3d(&maps.df, from, d0, t0, b);
+                tma_store_3d(&maps.dx, from + Tile::kBytes, d0, t0, b);
+                if constexpr (HAS_I) tma_store_3d(&maps.di, from + 3 * Tile::kBytes, d0, t0, b);
+                if constexpr (HAS_O) tma_store_3d(&maps.dout, from + (3 + HAS_I) * Tile::kBytes, d0, t0, b);
                 bulk_commit_group();
             }
         }

@@ -152,7 +152,7 @@ cudaError_t launch_spans(const RecurrenceParams& p, const typename MapsOf<SRC>::
     static std::atomic<uint64_t> ready[2];
     constexpr uint32_t kInputs = 2 + HAS_I + HAS_O;
     return backward ? launch_spans_kernel(recurrence_span_backward_kernel<T, HAS_I, HAS_O, VEC, SRC>, maps, &ready[1],
-                                          span_smem_bytes<T, VEC, SRC>(kInputs + 1, kInputs), p, 32 * VEC, stream)
+                                          span_smem_bytes<T, VEC, SRC>(kInputs + 1, 0), p, 32 * VEC, stream)
                     : launch_spans_kernel(recurrence_span_kernel<T, HAS_I, HAS_O, VEC, SRC>, maps, &ready[0],
                                           span_smem_bytes<T, VEC, SRC>(kInputs, 1), p, 32 * VEC, stream);
 }
@@ -214,17 +214,20 @@ cudaError_t launch_recurrence(RecurrenceParams& p, bool backward, int device, cu
         p.wait_cycles = services.wait_cycles;
         RecurrenceMaps maps;
         memset(&maps, 0, sizeof maps);
-        // two channels per access where every tensor has them side by side and aligned
-        bool pairs = p.D % 2 == 0;
+        // two 16-bit channels per access where every tensor has them side by side and aligned (Float32 gains more from twice the CTAs: 3 x 1025 x
+        // 1002, all gates, 25 / 54 us one by one, 35 / 66 in pairs; 8 x 2048 x 2046 144 / 266 and 173 / 243)
+        bool pairs = sizeof(T) == 2 && p.D % 2 == 0;
         auto look = [&](const void* ptr, long long b, long long t, long long d) {
             pairs = pairs && (!ptr || (reinterpret_cast<uintptr_t>(ptr) % (2 * sizeof(T)) == 0 && d == 1 && b % 2 == 0 && t % 2 == 0));
         };
         for (const Strided3* s : {&p.x, &p.f, &p.i, &p.o, &p.dy}) look(s->p, s->b, s->t, s->d);
         for (const Strided3W* s : {&p.y, &p.dx, &p.df, &p.di, &p.dout}) look(s->p, s->b, s->t, s->d);
-        constexpr int kTileVec = sizeof(T) == 2 ? 2 : 1, kOddSource = sizeof(T) == 2 ? kFromMemory : kFromWords;
-        if (encode_maps<T>(p, services.encode, maps)) e = launch_spans_gates<T, kTileVec, kFromTiles>(p, maps, backward, stream);
-        else if (pairs) e = launch_spans_gates<T, 2, kFromWords>(p, NoMaps{}, backward, stream);
-        else e = launch_spans_gates<T, 1, kOddSource>(p, NoMaps{}, backward, stream);
+        constexpr int kPair = sizeof(T) == 2 ? 2 : 1;
+        if (encode_maps<T>(p, services.encode, maps)) e = launch_spans_gates<T, kPair, kFromTiles>(p, maps, backward, stream);
+        else if (pairs || sizeof(T) == 4) e = launch_spans_gates<T, kPair, kFromWords>(p, NoMaps{}, backward, stream);
+        else {
+            if constexpr (sizeof(T) == 2) e = launch_spans_gates<T, 1, kFromMemory>(p, NoMaps{}, backward, stream);
+        }
     }
     if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;

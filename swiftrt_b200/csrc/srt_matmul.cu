@@ -2723,6 +2723,10 @@ cudaError_t srtMatmulGatedBackward(const void* outGrad, const srtTensorDescripto
     gp.dg = View2W{dGate, dg.m, dg.n}; gp.du = View2W{dUp, du.m, du.n};
     gp.sum_g = dBiasGate; gp.sum_g_n = sg_n; gp.sum_u = dBiasUp; gp.sum_u_n = su_n;
     gp.M = (uint32_t)M; gp.N = (uint32_t)H; gp.act = (uint32_t)activation;
+    TileServices services;
+    if ((e = tile_services(scope.device, services)) != cudaSuccess) return e;
+    gp.status = services.status;
+    gp.wait_cycles = services.wait_cycles;
     auto vec_ok = [&](const Matrix& v) {
         return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && v.n == 1 && (v.m * (long long)elem) % 16 == 0;
     };

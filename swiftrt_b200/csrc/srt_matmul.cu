@@ -1252,7 +1252,7 @@ struct CallKey {
     int32_t force, tile_n, stages, max_ctas, split_k;
     int32_t device;
     uint32_t plan_epoch;
-    uint32_t no_alloc;              // 1: srtMatmulNoAlloc (split-K scratch = the static array)
+    uint32_t no_alloc;              // 1: srtMatmulNoAlloc (split-K scratch = the static array); 2: no split-K (16-bit products)
 };
 
 constexpr int kCallCacheSize = 64;
@@ -1522,11 +1522,11 @@ void multicast_destroy(MulticastBuffer* b)
 // ------------------------------------------------------------------ one product
 // Parses, plans (or finds the prepared launch of an identical earlier call) and enqueues.
 // `no_alloc`: split-K partial sums go to the static scratch array; products whose partial sums do
-// not fit there are refused before anything is launched.
+// not fit there are refused before anything is launched.  `no_split`: a 16-bit product uses no workspace.
 cudaError_t run_matmul(const void* a, const srtTensorDescriptor* aDesc, bool transA, const void* b,
                        const srtTensorDescriptor* bDesc, bool transB, const void* bias,
                        const srtTensorDescriptor* biasDesc, srtActivationType activation, void* out,
-                       const srtTensorDescriptor* oDesc, cudaStream_t stream, bool no_alloc)
+                       const srtTensorDescriptor* oDesc, cudaStream_t stream, bool no_alloc, bool no_split = false)
 {
     CallKey key;
     memset(&key, 0, sizeof key);                 // padding bytes are part of the hashed key
@@ -1543,7 +1543,8 @@ cudaError_t run_matmul(const void* a, const srtTensorDescriptor* aDesc, bool tra
     key.split_k = g_tuning.split_k.load(std::memory_order_relaxed);
     key.device = scope.device;
     key.plan_epoch = g_plan_epoch.load(std::memory_order_relaxed);
-    key.no_alloc = no_alloc ? 1u : 0u;
+    no_split = no_split && P.type != real32F;                // (longer Float32 reductions need it for their accuracy)
+    key.no_alloc = no_alloc ? 1u : no_split ? 2u : 0u;
     if (!t_cache) t_cache.reset(new CallCache());
     const int slot = (int)(hash_key(key) % kCallCacheSize);
     if (t_cache->valid[slot] && memcmp(&t_cache->key[slot], &key, sizeof key) == 0)
@@ -1552,6 +1553,18 @@ cudaError_t run_matmul(const void* a, const srtTensorDescriptor* aDesc, bool tra
     Plan plan;
     e = plan_for(P, plan);
     if (e != cudaSuccess) return e;
+    if (no_split && plan.splits > 1) {
+        DeviceInfo info;
+        if ((e = device_info(scope.device, info)) != cudaSuccess) return e;
+        make_plan_impl(P, info, plan, false);                // (the transposed plan of few rows is one of split-K)
+        if (plan.splits > 1) {
+            plan.kb_per_split = plan.kb_per_split * plan.splits;
+            plan.splits = 1;
+            plan.pub.splitK = 1;
+            plan.pub.workspaceBytes = 0;
+            plan.pub.ctas = plan.pub.tiles < info.sms ? plan.pub.tiles : info.sms;
+        }
+    }
     if (no_alloc && plan.pub.workspaceBytes > kNoAllocScratchBytes) {
         if (plan.splits > 1)
             return fail(cudaErrorInvalidValue,
@@ -1578,6 +1591,15 @@ cudaError_t run_matmul(const void* a, const srtTensorDescriptor* aDesc, bool tra
 }
 
 // ------------------------------------------------------------------ srtMatmulGated, srtMatmulGatedBackward: helpers
+// A captured call may be replayed beside others that were captured on the same stream, and would share the stream's workspace with
+// them: its products run without split-K.
+bool is_captured(cudaStream_t stream)
+{
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess) (void)cudaGetLastError();
+    return capture != cudaStreamCaptureStatusNone;
+}
+
 
 struct Matrix { const char* p; uint64_t rows, cols; long long m, n; };          // element strides
 
@@ -2640,9 +2662,10 @@ cudaError_t srtMatmulGated(const void* x, const srtTensorDescriptor* xDesc, cons
     // two products and an elementwise pass; the pre-activations need a place then
     if (!gate)
         return fail(cudaErrorNotSupported, "%s: these tensors (Float32, or views without 16-byte aligned rows) need gate and up to hold the two products", op);
-    e = srtMatmulBiasActivation(x, xDesc, false, wGate, wGateDesc, false, biasGate, biasGateDesc, srtActivationIdentity, gate, gateDesc, stream);
+    const bool captured = is_captured(stream);
+    e = run_matmul(x, xDesc, false, wGate, wGateDesc, false, biasGate, biasGateDesc, srtActivationIdentity, gate, gateDesc, stream, false, captured);
     if (e != cudaSuccess) return e;
-    e = srtMatmulBiasActivation(x, xDesc, false, wUp, wUpDesc, false, biasUp, biasUpDesc, srtActivationIdentity, up, upDesc, stream);
+    e = run_matmul(x, xDesc, false, wUp, wUpDesc, false, biasUp, biasUpDesc, srtActivationIdentity, up, upDesc, stream, false, captured);
     if (e != cudaSuccess) return e;
     GateForwardParams fp;
     fp.g = View2{kg.p, kg.m, kg.n}; fp.u = View2{ku.p, ku.m, ku.n};
@@ -2735,12 +2758,14 @@ cudaError_t srtMatmulGatedBackward(const void* outGrad, const srtTensorDescripto
         : type == real16F ? launch_gate_backward<__half>(gp, vec, stream) : launch_gate_backward<__nv_bfloat16>(gp, vec, stream);
     if (e != cudaSuccess) return e;
 
+    const bool captured = is_captured(stream);
     if (dX && one_launch) {
         if ((e = sum_fused(type, dg, wg, du, wu, dx, info, stream)) != cudaSuccess) return e;
     } else if (dX) {
         const LocalDescriptor d_out(dx, type), d_tmp(dx2, type), d_dg(dg, type), d_du(du, type), d_wg(mg, type), d_wu(mu, type);
-        if ((e = srtMatmul(dGate, &d_dg.d, false, wGate, &d_wg.d, true, dX, &d_out.d, stream)) != cudaSuccess) return e;
-        if ((e = srtMatmul(dUp, &d_du.d, false, wUp, &d_wu.d, true, dX2, &d_tmp.d, stream)) != cudaSuccess) return e;
+        if ((e = run_matmul(dGate, &d_dg.d, false, wGate, &d_wg.d, true, nullptr, nullptr, srtActivationIdentity, dX, &d_out.d, stream, false, captured)) != cudaSuccess ||
+            (e = run_matmul(dUp, &d_du.d, false, wUp, &d_wu.d, true, nullptr, nullptr, srtActivationIdentity, dX2, &d_tmp.d, stream, false, captured)) != cudaSuccess)
+            return e;
         GateForwardParams sp;
         sp.g = View2{dx.p, dx.m, dx.n}; sp.u = View2{dx2.p, dx2.m, dx2.n}; sp.y = View2W{dX, dx.m, dx.n};
         sp.M = (uint32_t)M; sp.N = (uint32_t)K; sp.act = kActIdentity;
@@ -2756,7 +2781,7 @@ cudaError_t srtMatmulGatedBackward(const void* outGrad, const srtTensorDescripto
     }
     const auto product = [&](const void* gradient, const Matrix& dv, void* out, const Matrix& ov, size_t batch, size_t apart, size_t out_apart) {
         const LocalDescriptor d_x(mx, type, batch), d_out(ov, type, batch, out_apart), d_g(dv, type, batch, apart);
-        return srtMatmul(x, &d_x.d, true, gradient, &d_g.d, false, out, &d_out.d, stream);
+        return run_matmul(x, &d_x.d, true, gradient, &d_g.d, false, nullptr, nullptr, srtActivationIdentity, out, &d_out.d, stream, false, captured);
     };
     // both weights' gradients as one batch of two where the second pair lies in the same direction from the first: fewer of the
     // tiles run in a last, partly empty wave.  Reduction 3999, 4096 x 8200 bf16: 2 x 247 -> 442 us; 1000, 1024 x 4096: 2 x 17 -> 26 us

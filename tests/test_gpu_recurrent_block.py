@@ -216,3 +216,33 @@ def test_threads_and_graphs_at_once_give_the_same_bits(srt):
     srt.check_status(DEV)
     for got in captured:
         assert [k for k, (a, b) in enumerate(zip(want, got)) if not torch.equal(a, b)] == []
+
+
+@pytest.mark.parametrize("M,K,H", [(4096, 128, 256), (2500, 72, 120)])
+def test_graphs_of_one_stream_share_no_workspace(srt, M, K, H):
+    """Weight gradients of few tiles and a long reduction, which split it over a workspace of the stream when they are not
+    captured: two captured copies over different inputs, replayed at once.  Small integers and the identity make every
+    sum exact."""
+    g = torch.Generator().manual_seed(8)
+    ints = lambda *s: torch.randint(-1, 2, s, generator=g).to(torch.bfloat16).to(DEV)  # noqa: E731
+    layer = srt.GatedDense(ints(K, H), ints(K, H), activation=srt.ActivationType.identity)
+    inputs = [(ints(M, K), (ints(M, H), ints(M, H)), ints(M, H)) for _ in range(2)]
+    want = [[t.clone() for t in layer.backward(*i)[:3]] for i in inputs]
+    graphs, captured = [], []
+    for i in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured.append(layer.backward(*i)[:3])
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    srt.check_status(DEV)
+    for x, (gate, up), dy in inputs[:1]:
+        assert torch.equal(want[0][1], (x.double().t() @ (dy * up).double()).to(torch.bfloat16))
+    for got, right in zip(captured, want):
+        for a, b in zip(got, right):
+            assert torch.equal(a, b)

@@ -1556,6 +1556,7 @@ cudaError_t run_matmul(const void* a, const srtTensorDescriptor* aDesc, bool tra
     if (no_split && plan.splits > 1) {
         DeviceInfo info;
         if ((e = device_info(scope.device, info)) != cudaSuccess) return e;
+        plan.splits = 1;
         make_plan_impl(P, info, plan, false);                // (the transposed plan of few rows is one of split-K)
         if (plan.splits > 1) {
             plan.kb_per_split = plan.kb_per_split * plan.splits;

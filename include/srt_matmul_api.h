@@ -467,8 +467,8 @@ cudaError_t srtMatmulGated(
  * the call returns cudaErrorNotSupported before it launches anything.  With it each of the two products is rounded
  * before their sum is.  Results do not depend on timing.  M, K and H are at least 1.  Both weights' gradients are one batched product where
  * dUp and dWUp lie in the same direction from dGate and dWGate, with equal strides.
- * Products that are launches of their own (the weights' gradients; see also srtMatmulGated) may use the library's
- * per-(device, stream) workspace, as srtMatmul does.  Those of Float16 and BFloat16 do not in a captured call, so that graphs
+ * The products (but those of srtMatmulGated that are one launch) may use the library's per-(device, stream) workspace, as
+ * srtMatmul does.  Those of Float16 and BFloat16 do not in a captured call, so that graphs
  * captured on one stream may run at once; their last bits may then differ from those of a call that is not captured. */
 cudaError_t srtMatmulGatedBackward(
     const void* outGrad, const srtTensorDescriptor* outGradDesc,

@@ -291,9 +291,11 @@ PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
         Queue q(x);
         const at::ScalarType type = x.scalar_type();
         const int64_t rows = x.size(0), inner = x.size(1), cols = wg.size(1);
-        const at::Tensor dgate = empty({rows, cols}, type, x.device()), dup = empty({rows, cols}, type, x.device()), dx = empty({rows, inner}, type, x.device());
+        at::Tensor dgate = empty({rows, cols}, type, x.device()), dup = empty({rows, cols}, type, x.device());
+        const at::Tensor dx = empty({rows, inner}, type, x.device());
         at::Tensor dwg = empty({inner, cols}, type, x.device()), dwu = empty({inner, cols}, type, x.device());
-        // both pairs in one direction: one batched product gives both
+        // all pairs in one direction: batched products
+        if ((dup.data_ptr() > dgate.data_ptr()) != (wu.data_ptr() > wg.data_ptr())) std::swap(dgate, dup);
         if ((dup.data_ptr() > dgate.data_ptr()) != (dwu.data_ptr() > dwg.data_ptr())) std::swap(dwg, dwu);
         at::Tensor dbg, dbu, dx2;
         if (bg) dbg = empty(bg->sizes(), type, x.device());

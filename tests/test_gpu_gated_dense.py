@@ -317,3 +317,31 @@ def test_weight_gradients_wherever_the_pairs_lie(srt, dtype, M, K, H):
             if second == "blocks":
                 pitch = wide.shape[1] // 2
                 assert bool((wide[:, H:pitch] == 7).all()) and bool((wide[:, pitch + H:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("M,K,H", [(1, 136, 4096), (2, 1000, 8000), (40, 72, 3304), (300, 264, 4096), (1030, 520, 5000)])
+def test_input_gradients_of_few_tiles_and_long_reductions(srt, dtype, M, K, H):
+    """dX where its reduction is split, with the weights in either order, into a view, and captured (not split).  Small
+    integers and the identity: the result has one right value."""
+    from swiftrt_b200._lib import lib
+    from swiftrt_b200.matmul import descriptor_args, enqueue
+    dt, g = TYPES[dtype], torch.Generator().manual_seed(M)
+    ints = lambda *s: torch.randint(-1, 2, s, generator=g).to(dt).to(DEV)  # noqa: E731
+    x, gate, up, dy, both = ints(M, K), ints(M, H), ints(M, H), ints(M, H), ints(2, K, H)
+    dg, du = dy.double() * up.double(), dy.double() * gate.double()
+    for wg, wu in ((both[0], both[1]), (both[1], both[0])):
+        want = (dg @ wg.double().t() + du @ wu.double().t()).to(dt)
+        layer = srt.GatedDense(wg, wu, activation=srt.ActivationType.identity)
+        assert torch.equal(layer.backward(x, (gate, up), dy)[0], want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = layer.backward(x, (gate, up), dy)[0]
+        graph.replay()
+        assert torch.equal(captured, want)
+        wide = torch.full((M, K + 8), 7.0, dtype=dt, device=DEV)
+        pair = torch.empty(2, M, H, dtype=dt, device=DEV)
+        enqueue(lib.srtMatmulGatedBackward, x.device, *descriptor_args(dy, x, wg, wu, gate, up), int(srt.ActivationType.identity),
+                *descriptor_args(pair[0], pair[1], wide[:, :K], None, None, None, None, None))
+        assert torch.equal(wide[:, :K], want) and bool((wide[:, K:] == 7).all())
+    srt.check_status(DEV)

@@ -27,6 +27,7 @@
 
 #include "element.cuh"
 #include "fast_div.cuh"
+#include "few_rows_plan.h"
 #include "ptx.cuh"
 
 namespace srt {
@@ -54,8 +55,6 @@ struct FewRowsParams {
     unsigned long long wait_cycles;
 };
 struct FewRowsMaps { CUtensorMap w[2]; };
-
-constexpr uint32_t kFewRowsWarps = 8;
 
 template <typename T> __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -98,8 +97,9 @@ __device__ __forceinline__ uint32_t lds_word(uint32_t at)
 // four t of a load take are two apart, so that the eight lanes of a quarter warp read eight different chunks: no bank conflicts.
 template <typename T, int GPB>            // GPB: scale groups in 128 rows (4, 2, or 1 for groups of 128 and more)
 struct Int4Format {
-    static constexpr uint32_t kCols = 32, kTiles = 2, kUnit = 32, kChunks = 1, kXWords = 4, kWarpRows = 128, kUnits = 4, kMaxColumnGroups = 8;
-    static constexpr bool kGroups = true;
+    static constexpr FewRowsFormat kFormat = kInt4Weights;
+    static constexpr uint32_t kCols = kFormat.cols, kTiles = 2, kUnit = 32, kChunks = 1, kXWords = 4, kWarpRows = kFormat.warp_rows, kUnits = 4;
+    static constexpr bool kGroups = kFormat.grouped;
     static __device__ __forceinline__ uint32_t column(uint32_t g, uint32_t tile, uint32_t half) { return 4 * g + 2 * tile + half; }
 
     struct Group { uint32_t scale[2], zero; };
@@ -236,8 +236,9 @@ struct NoGroup { uint32_t unused; };
 
 template <typename T>
 struct RowsFormat {
-    static constexpr uint32_t kCols = 64, kTiles = 4, kUnit = 16, kChunks = 4, kXWords = 2, kWarpRows = 16, kUnits = 1, kMaxColumnGroups = 8, kGroupUnits = 1;
-    static constexpr bool kGroups = false;
+    static constexpr FewRowsFormat kFormat = kRowWeights;
+    static constexpr uint32_t kCols = kFormat.cols, kTiles = 4, kUnit = 16, kChunks = 4, kXWords = 2, kWarpRows = kFormat.warp_rows, kUnits = 1, kGroupUnits = 1;
+    static constexpr bool kGroups = kFormat.grouped;
     static __device__ __forceinline__ uint32_t column(uint32_t g, uint32_t tile, uint32_t half) { return 8 * g + 2 * tile + half; }
     static __device__ __forceinline__ uint32_t row(uint32_t c, uint32_t t) { return 8 * (c >> 1) + 2 * t + (c & 1); }
     using Group = NoGroup;
@@ -288,8 +289,9 @@ struct RowsFormat {
 
 template <typename T>
 struct ColsFormat {
-    static constexpr uint32_t kCols = 32, kTiles = 2, kUnit = 32, kChunks = 4, kXWords = 4, kWarpRows = 32, kUnits = 1, kMaxColumnGroups = 2, kGroupUnits = 1;
-    static constexpr bool kGroups = false;
+    static constexpr FewRowsFormat kFormat = kColumnWeights;
+    static constexpr uint32_t kCols = kFormat.cols, kTiles = 2, kUnit = 32, kChunks = 4, kXWords = 4, kWarpRows = kFormat.warp_rows, kUnits = 1, kGroupUnits = 1;
+    static constexpr bool kGroups = kFormat.grouped;
     static __device__ __forceinline__ uint32_t column(uint32_t g, uint32_t tile, uint32_t half) { return 16 * tile + 8 * half + g; }
     using Group = NoGroup;
     using Offsets = NoGroup;
@@ -420,7 +422,6 @@ __device__ __forceinline__ void few_rows_finish(const FewRowsParams& p, float* r
         cluster_wait_acquire();
     }
 }
-template <typename Format, int NW, int NT> constexpr uint32_t few_rows_sum_bytes() { return NW * kFewRowsWarps * 8 * NT * (Format::kCols + 1) * 4; }
 
 // ------------------------------------------------------------------------------------------ any view
 // NW: weights (2: gated).  NT: tiles of 8 rows of x per CTA; grid z walks further rows.  Grid x: column tiles, grid y = the
@@ -468,8 +469,6 @@ few_rows_kernel(const __grid_constant__ FewRowsParams p)
 // Warps 0 .. 7 multiply: warp w takes column tile w mod CG and part w / CG (of KG = 8 / CG) of every stage's rows.  Warp 8 asks for the
 // stages: per weight 16 KB, CG tiles of 128-byte rows.  CG is 8 for wide weights (the rows of a stage are then a kilobyte of memory each)
 // and smaller where column tiles are few.
-constexpr uint32_t kFewRowsTileThreads = 32 * (kFewRowsWarps + 1), kFewRowsStageBytes = 16384, kFewRowsMaxStages = 6;
-
 template <typename T, typename Format, int NW, int NT>
 __global__ void __launch_bounds__(kFewRowsTileThreads)
 few_rows_tiles_kernel(const __grid_constant__ FewRowsParams p, const __grid_constant__ FewRowsMaps maps)

@@ -5,7 +5,6 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
-#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -92,7 +91,7 @@ cudaError_t launch_rows_kernel(Kernel kernel, std::atomic<uint64_t>& ready, dim3
     if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (!(ready.load(std::memory_order_acquire) & bit)) {            // once per kernel and device
-        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewRowsSharedLimit)) != cudaSuccess) return e;
         ready.fetch_or(bit, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg;
@@ -113,19 +112,8 @@ cudaError_t launch_rows_kernel(Kernel kernel, std::atomic<uint64_t>& ready, dim3
     return e;
 }
 
-// How few_rows_tiles_kernel would run a product, and an estimate of its time in microseconds.
-struct RowsPlan {
-    double cost = 1e300;
-    uint32_t groups = 0, cluster = 0, stages = 0, k_per_part = 0, x_pitch = 0, x_bytes = 0;
-};
-
-// The choice of column tiles to a CTA and CTAs to a cluster by what it costs: rounds of CTAs and what they stream, x to bring in before
-// the first product, the exchange of a cluster, SMs with one CTA's eight warps only, and the places that clusters of 4 and 8 leave
-// free.  The constants are fitted to the times of all choices at 9 shapes of 4-bit and 6 of 16-bit weights and 1 .. 48 rows; the choice is
-// on average 4 % slower than the best one.  One row, 4096 x 16384 in 4 bits, tiles x cluster: 8 x 4 17.0, 4 x 2 17.0, 2 x 1 16.4 us; 8 x 2
-// 21.3, 8 x 8 22.5 us.  17 rows, 8192 x 1024: 2 x 8 in rows of 8 13.3, in rows of 32 19.6 us.
 template <typename T, typename Format, int NW, int NT>
-cudaError_t plan_few_rows(const FewRowsParams& p, RowsPlan& best)
+cudaError_t plan_rows(const FewRowsParams& p, RowsPlan& plan)
 {
     static std::atomic<uint32_t> by_registers{0};                            // CTAs that an SM's registers hold
     uint32_t most = by_registers.load(std::memory_order_relaxed);
@@ -137,35 +125,7 @@ cudaError_t plan_few_rows(const FewRowsParams& p, RowsPlan& best)
         most = most > 3 ? 3 : most < 1 ? 1 : most;
         by_registers.store(most, std::memory_order_relaxed);
     }
-    const uint32_t row_blocks = (p.M + 8 * NT - 1) / (8 * NT), tiles = (p.N + Format::kCols - 1) / Format::kCols;
-    const uint32_t x_rows = p.M < 8 * NT ? p.M : 8 * NT, stage_bytes = NW * kFewRowsStageBytes;
-    for (uint32_t c = 1; c <= 8; c *= 2)
-        for (uint32_t g = Format::kMaxColumnGroups; g >= 1; g /= 2) {
-            const uint32_t stage_rows = 8 / g * Format::kWarpRows, rounds = ((p.K + stage_rows - 1) / stage_rows + c - 1) / c;
-            const uint32_t x_pitch = (rounds * stage_rows * 2 + 127) / 128 * 128 + 16;      // rows of x start four banks apart
-            const uint64_t x_bytes = (uint64_t)x_rows * x_pitch;
-            // as many CTAs to an SM as leave each three stages beside x
-            uint32_t per_sm = most, stages = 0;
-            for (; per_sm >= 1; --per_sm) {
-                const uint64_t room = (224u / per_sm - 2) * 1024u - 1024u;
-                stages = x_bytes < room ? (uint32_t)((room - x_bytes) / stage_bytes) : 0;
-                if (stages >= 3 || stages >= rounds || per_sm == 1) break;
-            }
-            if (stages > kFewRowsMaxStages) stages = kFewRowsMaxStages;
-            if (stages > rounds) stages = rounds;
-            if (stages == 0) continue;
-            const uint32_t at_once = per_sm > 2 ? 2 : per_sm;
-            const double places = 148.0 * at_once * (c == 8 ? 0.45 : c == 4 ? 0.93 : 1.0), full = (double)((tiles + g - 1) / g) * row_blocks * c / places;
-            const double waves = std::ceil(full), stream = rounds * stage_bytes * places / 5.5e6 * (at_once == 1 && Format::kGroups ? 1.4 : 1.0);  // a round at 5.5 TB/s
-            double cost = waves * (7.3 + (Format::kGroups ? 0.6 * rounds : 0.0)) + stream * (0.15 * waves + 0.85 * (full > 0.25 ? full : 0.25)) + x_bytes / 1024.0 * 0.04 +
-                          0.1 * NW * NT;
-            if (c > 1) cost += 1.0 + 0.3 * c;
-            if (cost < best.cost) {
-                best.cost = cost;
-                best.groups = g; best.cluster = c; best.stages = stages;
-                best.k_per_part = rounds * stage_rows; best.x_pitch = x_pitch; best.x_bytes = (uint32_t)x_bytes;
-            }
-        }
+    plan = plan_few_rows(Format::kFormat, NW, NT, p.M, p.N, p.K, most);
     return cudaSuccess;
 }
 
@@ -180,12 +140,9 @@ cudaError_t launch_tiles(FewRowsParams& p, const RowsPlan& plan, EncodeTiledFn e
     FewRowsMaps maps;
     done = row_blocks <= 65535 && encode_weight<T, Format>(encode, p, p.w[0], parts, &maps.w[0]) && encode_weight<T, Format>(encode, p, p.w[NW - 1], parts, &maps.w[1]);
     if (!done) return cudaSuccess;
-    // the sums take the ring's place
-    constexpr uint32_t kSums = (few_rows_sum_bytes<Format, NW, NT>() + 127) / 128 * 128;
-    const uint32_t ring = plan.stages * NW * kFewRowsStageBytes;
     static std::atomic<uint64_t> ready{0};
     return launch_rows_kernel(few_rows_tiles_kernel<T, Format, NW, NT>, ready, dim3((tiles + plan.groups - 1) / plan.groups, plan.cluster, row_blocks), kFewRowsTileThreads,
-                              1024 + (ring > kSums ? ring : kSums) + plan.x_bytes, stream, p, maps);
+                              plan.smem, stream, p, maps);
 }
 
 template <typename T, typename Format, int NW, int NT>
@@ -198,7 +155,7 @@ cudaError_t launch_any(FewRowsParams& p, cudaStream_t stream)
     while (cluster < 8 && (uint64_t)tiles * row_blocks * cluster * 2 <= 2 * 148 && kFewRowsWarps * cluster * 2 <= units) cluster *= 2;
     p.k_per_part = (units + kFewRowsWarps * cluster - 1) / (kFewRowsWarps * cluster) * Format::kUnit;
     static std::atomic<uint64_t> ready{0};
-    return launch_rows_kernel(few_rows_kernel<T, Format, NW, NT>, ready, dim3(tiles, cluster, row_blocks), 32 * kFewRowsWarps, few_rows_sum_bytes<Format, NW, NT>(), stream, p);
+    return launch_rows_kernel(few_rows_kernel<T, Format, NW, NT>, ready, dim3(tiles, cluster, row_blocks), 32 * kFewRowsWarps, few_rows_sum_bytes(Format::kFormat, NW, NT), stream, p);
 }
 
 // Eight, 16 or 32 rows of x to a CTA, whichever is estimated to be fastest: more rows read the weights fewer times, fewer rows have
@@ -214,10 +171,10 @@ cudaError_t launch_few_rows(FewRowsParams& p, double limit, int device, cudaStre
         p.status = services.status;
         p.wait_cycles = services.wait_cycles;
         RowsPlan plan[3];
-        if ((e = plan_few_rows<T, Format, NW, 1>(p, plan[0])) != cudaSuccess) return e;
-        if (p.M > 8 && (e = plan_few_rows<T, Format, NW, 2>(p, plan[1])) != cudaSuccess) return e;
+        if ((e = plan_rows<T, Format, NW, 1>(p, plan[0])) != cudaSuccess) return e;
+        if (p.M > 8 && (e = plan_rows<T, Format, NW, 2>(p, plan[1])) != cudaSuccess) return e;
         if constexpr (NW == 1)
-            if (p.M > 16 && (e = plan_few_rows<T, Format, NW, 4>(p, plan[2])) != cudaSuccess) return e;
+            if (p.M > 16 && (e = plan_rows<T, Format, NW, 4>(p, plan[2])) != cudaSuccess) return e;
         bool done = false;
         int which = plan[1].cost < plan[0].cost ? 1 : 0;
         if (plan[2].cost < plan[which].cost) which = 2;

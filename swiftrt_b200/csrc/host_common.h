@@ -28,6 +28,15 @@ inline cudaError_t fail(cudaError_t code, const char* fmt, ...)
     return code;
 }
 
+// What a launch returned, as the call's status.  A refused launch is also the runtime's last error, where the next kernel of anyone
+// who asks for that would find it: it is taken away and becomes the call's text.
+inline cudaError_t launch_status(cudaError_t e)
+{
+    if (e == cudaSuccess) return e;
+    (void)cudaGetLastError();
+    return fail(e, "a kernel could not be launched: %s", cudaGetErrorString(e));
+}
+
 // ------------------------------------------------------------------ the device of a call
 // Every entry point that takes a stream works on THAT stream's device, whatever device is current
 // on the calling thread: the reference's queues never select a device before they enqueue

@@ -107,7 +107,7 @@ cudaError_t launch_rows_kernel(Kernel kernel, std::atomic<uint64_t>& ready, dim3
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    e = launch_status(cudaLaunchKernelEx(&cfg, kernel, args...));
     if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;
 }

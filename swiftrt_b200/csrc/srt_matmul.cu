@@ -687,7 +687,7 @@ cudaError_t launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUte
         cluster_cache[dev & 63].store(max_clusters, std::memory_order_release);
     }
     if (ctas / 2 > (uint32_t)max_clusters) cfg.gridDim.x = 2u * (uint32_t)max_clusters;
-    return cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, gp, peers);
+    return launch_status(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mo, gp, peers));
 }
 
 template <typename T>
@@ -982,7 +982,7 @@ cudaError_t launch_x3_bn(const Prepared& pr, cudaStream_t stream)
         cluster_cache[dev & 63].store(max_clusters, std::memory_order_release);
     }
     if (pr.ctas / 2 > (uint32_t)max_clusters) cfg.gridDim.x = 2u * (uint32_t)max_clusters;
-    return cudaLaunchKernelEx(&cfg, kernel, pr.ma, pr.mb, pr.mbc, pr.mo, pr.xp);
+    return launch_status(cudaLaunchKernelEx(&cfg, kernel, pr.ma, pr.mb, pr.mbc, pr.mo, pr.xp));
 }
 
 cudaError_t launch_x3(const Prepared& pr, cudaStream_t stream)
@@ -1118,7 +1118,7 @@ cudaError_t launch_reduce_as_dependent(const ReduceParams& rp, unsigned blocks, 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, splitk_reduce_kernel<T, VEC>, rp);
+    return launch_status(cudaLaunchKernelEx(&cfg, splitk_reduce_kernel<T, VEC>, rp));
 }
 
 template <typename T>
@@ -1134,7 +1134,7 @@ cudaError_t launch_reduce_transposed(const ReduceParams& rp, cudaStream_t stream
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, splitk_reduce_transposed_kernel<T>, rp);
+    return launch_status(cudaLaunchKernelEx(&cfg, splitk_reduce_transposed_kernel<T>, rp));
 }
 
 cudaError_t launch_reduce(const Prepared& pr, cudaStream_t stream)
@@ -1901,7 +1901,7 @@ cudaError_t launch_gate_backward(const GateBackwardParams& gp, bool vec, cudaStr
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = vec ? cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, kVec>, gp) : cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, 1>, gp);
+    const cudaError_t e = launch_status(vec ? cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, kVec>, gp) : cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, 1>, gp));
     if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;
 }

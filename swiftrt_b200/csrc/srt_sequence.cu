@@ -143,7 +143,7 @@ cudaError_t launch_spans_kernel(Kernel kernel, const Maps& maps, std::atomic<uin
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p, maps, blocks_d, cluster);
+    return launch_status(cudaLaunchKernelEx(&cfg, kernel, p, maps, blocks_d, cluster));
 }
 
 template <typename T, bool HAS_I, bool HAS_O, int VEC, int SRC>

@@ -80,4 +80,16 @@ inline RowsPlan plan_few_rows(const FewRowsFormat& f, uint32_t nw, uint32_t nt, 
     return best;
 }
 
+// Which of the plans of 8, 16 and 32 rows to a CTA runs a product: the cheapest; kFewRowsElsewhere where the caller has another way that takes `limit`
+// microseconds and none is faster or fits; kFewRowsAnyView, the kernel without tiles, where none fits and there is no other way
+// (`limit` is infinite).
+enum : int { kFewRowsAnyView = -1, kFewRowsElsewhere = -2 };
+inline int choose_few_rows(const RowsPlan (&plan)[3], double limit)
+{
+    int which = plan[1].cost < plan[0].cost ? 1 : 0;
+    if (plan[2].cost < plan[which].cost) which = 2;
+    if (plan[which].groups == 0) return std::isinf(limit) ? kFewRowsAnyView : kFewRowsElsewhere;
+    return plan[which].cost > limit ? kFewRowsElsewhere : which;
+}
+
 }  // namespace srt

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 
@@ -160,7 +161,7 @@ cudaError_t launch_any(FewRowsParams& p, cudaStream_t stream)
 
 // Eight, 16 or 32 rows of x to a CTA, whichever is estimated to be fastest: more rows read the weights fewer times, fewer rows have
 // less of x to bring in and more CTAs to an SM (two weights' sums of 32 rows do not fit into registers).
-// cudaErrorNotSupported, without text, where the estimate is above `limit` microseconds.
+// cudaErrorNotSupported, without text, where the caller's other way, of `limit` microseconds, is to be taken (see choose_few_rows).
 template <typename T, typename Format, int NW>
 cudaError_t launch_few_rows(FewRowsParams& p, double limit, int device, cudaStream_t stream)
 {
@@ -176,16 +177,13 @@ cudaError_t launch_few_rows(FewRowsParams& p, double limit, int device, cudaStre
         if constexpr (NW == 1)
             if (p.M > 16 && (e = plan_rows<T, Format, NW, 4>(p, plan[2])) != cudaSuccess) return e;
         bool done = false;
-        int which = plan[1].cost < plan[0].cost ? 1 : 0;
-        if (plan[2].cost < plan[which].cost) which = 2;
-        if (plan[which].cost > limit) return cudaErrorNotSupported;
-        if (plan[which].cost < 1e300) {
-            if (which == 0) e = launch_tiles<T, Format, NW, 1>(p, plan[0], services.encode, done, stream);
-            else if (which == 1) e = launch_tiles<T, Format, NW, 2>(p, plan[1], services.encode, done, stream);
-            if constexpr (NW == 1)
-                if (which == 2) e = launch_tiles<T, Format, NW, 4>(p, plan[2], services.encode, done, stream);
-            if (done || e != cudaSuccess) return e;
-        }
+        const int which = choose_few_rows(plan, limit);
+        if (which == kFewRowsElsewhere) return cudaErrorNotSupported;
+        if (which == 0) e = launch_tiles<T, Format, NW, 1>(p, plan[0], services.encode, done, stream);
+        else if (which == 1) e = launch_tiles<T, Format, NW, 2>(p, plan[1], services.encode, done, stream);
+        if constexpr (NW == 1)
+            if (which == 2) e = launch_tiles<T, Format, NW, 4>(p, plan[2], services.encode, done, stream);
+        if (done || e != cudaSuccess) return e;
     }
     return p.M <= 8 ? launch_any<T, Format, NW, 1>(p, stream) : launch_any<T, Format, NW, 2>(p, stream);
 }
@@ -193,9 +191,9 @@ cudaError_t launch_few_rows(FewRowsParams& p, double limit, int device, cudaStre
 template <typename T, int NW>
 cudaError_t launch_int4(FewRowsParams& p, int device, cudaStream_t stream)
 {
-    if (p.group == 32) return launch_few_rows<T, Int4Format<T, 4>, NW>(p, 1e299, device, stream);
-    if (p.group == 64) return launch_few_rows<T, Int4Format<T, 2>, NW>(p, 1e299, device, stream);
-    return launch_few_rows<T, Int4Format<T, 1>, NW>(p, 1e299, device, stream);
+    if (p.group == 32) return launch_few_rows<T, Int4Format<T, 4>, NW>(p, HUGE_VAL, device, stream);
+    if (p.group == 64) return launch_few_rows<T, Int4Format<T, 2>, NW>(p, HUGE_VAL, device, stream);
+    return launch_few_rows<T, Int4Format<T, 1>, NW>(p, HUGE_VAL, device, stream);
 }
 
 cudaError_t run_int4(const char* op, const void* x, const srtTensorDescriptor* xDesc, const srtInt4Matrix* w0, const srtInt4Matrix* w1, const void* bias0,

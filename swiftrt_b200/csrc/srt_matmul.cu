@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -1761,7 +1762,7 @@ cudaError_t gated_fused(srtDataType type, const Matrix& x, const Matrix& wg, con
 constexpr uint64_t kFewRows = 8, kSomeRows = 128;
 
 // the gated product of a few rows; any strides of x and the results, weights contiguous along K or along their columns.
-// `if_faster`: only where the tiles are estimated to be slower
+// `if_faster`: only where the tiles are estimated to be slower, or the rows are few and x finds room
 cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, const Matrix& wu, const void* bg, long long bg_n, const void* bu, long long bu_n,
                        uint32_t act, const Matrix* gate, const Matrix* up, const Matrix& out, bool if_faster, int device, cudaStream_t stream)
 {
@@ -1791,7 +1792,7 @@ cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, cons
     p.out = const_cast<char*>(out.p); p.o_m = out.m; p.o_n = out.n;
     p.M = (uint32_t)x.rows; p.N = (uint32_t)wg.cols; p.K = (uint32_t)x.cols;
     p.act = act;
-    double limit = 1e299;
+    double limit = if_faster ? 1e299 : HUGE_VAL;
     if (if_faster && x.rows > kFewRows) {
         if (!p.w[0].vec || !p.w[1].vec) return cudaErrorNotSupported;
         const uint64_t tiles = (wg.cols + 127) / 128;

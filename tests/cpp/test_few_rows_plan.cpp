@@ -50,6 +50,19 @@ int main()
                         check(p.k_per_part % stage_rows == 0 && (uint64_t)p.k_per_part * p.cluster >= K, "K is not covered");
                     }
     }
+    // which of three plans runs: no plan leads to the kernel that takes any view unless the caller has another way
+    const auto chosen = [](double a, double b, double c, double limit) {
+        RowsPlan plan[3];
+        const double cost[3] = {a, b, c};
+        for (int i = 0; i < 3; ++i)
+            if (cost[i] > 0) plan[i].cost = cost[i], plan[i].groups = 1;
+        return choose_few_rows(plan, limit);
+    };
+    const bool choices = chosen(3, 0, 0, HUGE_VAL) == 0 && chosen(3, 2, 0, HUGE_VAL) == 1 && chosen(3, 2, 1, 1e299) == 2 && chosen(0, 0, 1, HUGE_VAL) == 2 &&
+                         chosen(3, 2, 4, 1.5) == kFewRowsElsewhere && chosen(0, 0, 0, 1.5) == kFewRowsElsewhere && chosen(0, 0, 0, 1e299) == kFewRowsElsewhere &&
+                         chosen(0, 0, 0, HUGE_VAL) == kFewRowsAnyView;
+    const RowsPlan none[3] = {plan_few_rows(kInt4Weights, 1, 1, 8, 4096, 131072, 3), plan_few_rows(kInt4Weights, 1, 2, 8, 4096, 131072, 3), RowsPlan{}};
+    if (!choices || choose_few_rows(none, HUGE_VAL) != kFewRowsAnyView) ++g_failures, printf("a wrong choice\n");
     printf("%ld plans, %ld failures\n", g_plans, g_failures);
     return g_failures != 0 || g_plans == 0;
 }

@@ -92,3 +92,41 @@ def test_gated_products_where_x_leaves_little_room(srt, M, K, N, by_columns):
     ea = 1.1 * eg + 2.0 ** -20 * a.abs()
     _check(got[:, columns], a * u, ea * (u.abs() + eu) + a.abs() * eu + 2.0 ** -23 * (a * u).abs())
     assert srt.check_status() == 0
+
+
+# x of these reductions fits beside no stage: the kernel that takes any view computes them
+@pytest.mark.parametrize("M,K,N,G,dtype,zeros", [(8, 131072, 4096, 128, "bf16", False), (8, 110000, 32, 64, "fp16", True), (33, 120000, 100, 32, "bf16", True)])
+def test_4_bit_products_without_room_for_x(srt, M, K, N, G, dtype, zeros):
+    _check_int4(srt, M, K, N, G, {"bf16": torch.bfloat16, "fp16": torch.float16}[dtype], zeros)
+
+
+@pytest.mark.parametrize("H", [60, 64])
+def test_gated_products_without_room_for_x(srt, H):
+    """Weights contiguous along K; results of 60 columns do not start on 16 bytes, which leaves the kernel without tiles."""
+    M, K = 8, 131072
+    x = _randn(M, K, seed=5)
+    weights = [_randn(H, K, seed=s, scale=K ** -0.5).t() for s in (1, 2)]
+    layer = srt.GatedDense(*weights)
+    before = srt.launch_count()
+    got = layer(x)
+    torch.cuda.synchronize()
+    assert srt.launch_count() == before + 1
+    # (up to 131072 / 16 adds into one accumulator: 8192 5.2 / sqrt(131072) 2^-23 S)
+    (g, eg), (u, eu) = ((x.double() @ w.double(), 2.0 ** -16 * (x.double().abs() @ w.double().abs())) for w in weights)
+    a = g * torch.sigmoid(g)
+    ea = 1.1 * eg + 2.0 ** -20 * a.abs()
+    _check(got, a * u, ea * (u.abs() + eu) + a.abs() * eu + 2.0 ** -23 * (a * u).abs())
+    assert srt.check_status() == 0
+
+
+def test_gated_4_bit_product_without_room_for_x(srt):
+    M, K, N = 8, 110000, 64
+    x = _randn(M, K, seed=7)
+    w = [_int4_weight(srt, K, N, 128, torch.bfloat16, True, seed=s) for s in (0, 1)]
+    got = srt.gated_matmul_int4(x, *w)
+    torch.cuda.synchronize()
+    (g, eg), (u, eu) = ((x.double() @ v, 2.0 ** -17.8 * (x.double().abs() @ v.abs())) for v in (_int4_columns(i, torch.arange(N, device=DEV)) for i in w))
+    a = g * torch.sigmoid(g)
+    ea = 1.1 * eg + 2.0 ** -20 * a.abs()
+    _check(got, a * u, ea * (u.abs() + eu) + a.abs() * eu + 2.0 ** -23 * (a * u).abs())
+    assert srt.check_status() == 0

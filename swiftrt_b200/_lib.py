@@ -161,7 +161,7 @@ lib.srtMulticastFree.restype = ctypes.c_int
 lib.srtMulticastFree.argtypes = [_P]
 lib.srtMatmulSetWaitLimit.restype = ctypes.c_int
 lib.srtMatmulSetWaitLimit.argtypes = [ctypes.c_uint64]
-# descriptors are passed by address (Descriptor.address): a call of a single token is bound by its marshalling
+# a Descriptor is passed as it is (its _as_parameter_ is the structure's address)
 lib.srtGatedRecurrence.restype = ctypes.c_int
 lib.srtGatedRecurrence.argtypes = [_P] * 18
 lib.srtGatedRecurrenceBackward.restype = ctypes.c_int

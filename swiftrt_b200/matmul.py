@@ -65,13 +65,14 @@ def _descriptor(t: torch.Tensor) -> Descriptor:
 
 
 def descriptor_args(*tensors) -> list:
-    """(data pointer, descriptor address) of every tensor, two nulls for None."""
+    """(data pointer, Descriptor) of every tensor, two nulls for None.  The descriptors live as long as the list: the cache
+    that they come from may be emptied at any time, by another thread while a call runs too."""
     out = []
     for t in tensors:
         if t is None:
             out += (None, None)
         else:
-            out += (t.data_ptr(), _descriptor(t).address)
+            out += (t.data_ptr(), _descriptor(t))
     return out
 
 

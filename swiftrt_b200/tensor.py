@@ -86,7 +86,7 @@ class Descriptor:
         span = 1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride())) if t.numel() else 0
         self.struct = TensorDescriptor(data_type(t), n, int(order_of(t)), t.numel(), span,
                                        self._shape, self._strides, self._strides)
-        self.address = ctypes.addressof(self.struct)
+        self._as_parameter_ = ctypes.addressof(self.struct)     # a Descriptor is itself the argument of a call, which keeps it alive
 
     def ref(self):
         return ctypes.byref(self.struct)

@@ -10,7 +10,7 @@ import torch
 from . import _lib
 from ._lib import lib
 from .int4 import Int4Weight, gated_matmul_int4, matmul_int4
-from .matmul import MatmulError, _descriptor, binding, matmul
+from .matmul import MatmulError, _descriptor, binding, matmul, rows_of
 from .tensor import ActivationType, order_of
 
 
@@ -133,22 +133,20 @@ class GatedDense:
     def __call__(self, input: torch.Tensor) -> torch.Tensor:
         if self.int4:
             return gated_matmul_int4(input, self.weight_gate, self.weight_up, self.bias_gate, self.bias_up, self.activation)
-        if input.dim() == 2:
-            return self._forward(input, False)
-        return self._forward(input.reshape(-1, input.shape[-1]), False).view(*input.shape[:-1], -1)
+        y = self._forward(rows_of(input), False)
+        return y if input.dim() == 2 else y.view(*input.shape[:-1], y.shape[-1])
 
     def forward_keep(self, input: torch.Tensor):
         """(output, saved) for training; `saved` is the pair of pre-activations that backward() needs."""
         if self.int4:
             raise ValueError("4-bit weights have no backward pass")
-        y, gate, up = self._forward(input.reshape(-1, input.shape[-1]), True)
-        return y.view(*input.shape[:-1], -1), (gate, up)
+        y, gate, up = self._forward(rows_of(input), True)
+        return y.view(*input.shape[:-1], y.shape[-1]), (gate, up)
 
     def backward(self, input: torch.Tensor, saved: tuple, out_grad: torch.Tensor):
         """Gradients of (input, weightGate, weightUp, biasGate, biasUp); None for a bias that is None.  `saved` is the
         second value of forward_keep."""
         gate, up = saved
-        flat = lambda t: t if t.dim() == 2 else t.reshape(-1, t.shape[-1])  # noqa: E731
-        dx, dwg, dwu, dbg, dbu = binding.gated_backward(flat(input), flat(out_grad), self.weight_gate, self.weight_up, gate, up, self.bias_gate,
+        dx, dwg, dwu, dbg, dbu = binding.gated_backward(rows_of(input), rows_of(out_grad), self.weight_gate, self.weight_up, gate, up, self.bias_gate,
                                                         self.bias_up, int(self.activation))
         return dx.view(input.shape), dwg, dwu, dbg, dbu

@@ -8,7 +8,7 @@ import torch
 
 from . import _lib
 from ._lib import lib
-from .matmul import binding, descriptor_args, enqueue, on_one_device
+from .matmul import binding, descriptor_args, enqueue, on_one_device, rows_of
 from .tensor import ActivationType, data_type
 
 
@@ -76,9 +76,8 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, zero_points: bool = Fa
 def matmul_int4(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None = None,
                 activation: ActivationType = ActivationType.identity) -> torch.Tensor:
     """activation(x . weight + bias) for an [..., rows] tensor x; asynchronous on torch's current stream."""
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    out = binding.int4(flat, weight.address, 0, weight.packed, weight.cols, bias, None, int(activation))
-    return out if x.dim() == 2 else out.view(*x.shape[:-1], -1)
+    out = binding.int4(rows_of(x), weight.address, 0, weight.packed, weight.cols, bias, None, int(activation))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], out.shape[-1])
 
 
 def gated_matmul_int4(x: torch.Tensor, weight_gate: Int4Weight, weight_up: Int4Weight, bias_gate: torch.Tensor | None = None,
@@ -86,6 +85,5 @@ def gated_matmul_int4(x: torch.Tensor, weight_gate: Int4Weight, weight_up: Int4W
     """activation(x . weight_gate + bias_gate) * (x . weight_up + bias_up) (srtMatmulGatedInt4)."""
     if weight_up.device != weight_gate.device:
         raise ValueError(f"tensors on different devices: {weight_gate.device} and {weight_up.device}")
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    out = binding.int4(flat, weight_gate.address, weight_up.address, weight_gate.packed, weight_gate.cols, bias_gate, bias_up, int(activation))
-    return out if x.dim() == 2 else out.view(*x.shape[:-1], -1)
+    out = binding.int4(rows_of(x), weight_gate.address, weight_up.address, weight_gate.packed, weight_gate.cols, bias_gate, bias_up, int(activation))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], out.shape[-1])

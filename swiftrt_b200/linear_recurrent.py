@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from .dense import bias_activation_backward
-from .matmul import binding, matmul
+from .matmul import binding, matmul, rows_of
 from .tensor import ActivationType
 
 STATE_CHUNK = 64            # steps between two kept states (SRT_GATED_RECURRENCE_CHUNK)
@@ -60,8 +60,8 @@ class LinearRecurrentCell:
 
     def _gates(self, input: torch.Tensor):
         """(fused, (update, forget, input gate or None, output)) of [batch, (steps,) inputSize]."""
-        fused = matmul(input.reshape(-1, input.shape[-1]), self.fused_weight, bias=self.fused_bias)
-        return fused, self._blocks(fused.view(*input.shape[:-1], -1))
+        fused = matmul(rows_of(input), self.fused_weight, bias=self.fused_bias)
+        return fused, self._blocks(fused.view(*input.shape[:-1], fused.shape[-1]))
 
     def _blocks(self, fused: torch.Tensor):
         h = self.hidden_size
@@ -87,13 +87,12 @@ class LinearRecurrentCell:
     def backward(self, input: torch.Tensor, saved: tuple, out_grad: torch.Tensor, last_grad: torch.Tensor | None = None):
         """(input gradient, weight gradient, bias gradient or None, initial state gradient)."""
         fused, states, lengths = saved
-        update, forget, gate, output = self._blocks(fused.view(*input.shape[:-1], -1))
+        update, forget, gate, output = self._blocks(fused.view(*input.shape[:-1], fused.shape[-1]))
         fused_grad = torch.empty_like(fused)
-        grads = self._blocks(fused_grad.view(*input.shape[:-1], -1))
+        grads = self._blocks(fused_grad.view(*input.shape[:-1], fused.shape[-1]))
         initial_grad = gated_recurrence_backward(out_grad, update, forget, gate, output, states, lengths, last_grad, out=grads)[-1]
-        x = input.reshape(-1, input.shape[-1])
         dx = matmul(fused_grad, self.fused_weight, False, True).view(input.shape)
-        dw = matmul(x, fused_grad, True, False)
+        dw = matmul(rows_of(input), fused_grad, True, False)
         db = None
         if self.fused_bias is not None:
             db = bias_activation_backward(fused_grad, None, ActivationType.identity, want_dz=False)[1]

@@ -10,6 +10,7 @@ Every call goes to the CUDA library; there is no other path.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -62,6 +63,11 @@ def _descriptor(t: torch.Tensor) -> Descriptor:
             _DESC_CACHE.clear()
         d = _DESC_CACHE[key] = Descriptor(t)
     return d
+
+
+def rows_of(t: torch.Tensor) -> torch.Tensor:
+    """`t` as a matrix, its leading dimensions as one (explicitly: no size can be inferred for a tensor without elements)."""
+    return t if t.dim() == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
 
 
 def descriptor_args(*tensors) -> list:

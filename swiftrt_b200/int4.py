@@ -13,9 +13,9 @@ from .tensor import ActivationType, data_type
 
 
 def _on_rows_of(t: torch.Tensor, nbytes: int) -> torch.Tensor:
-    """`t` itself where its rows start on multiples of `nbytes`, else a copy whose rows do."""
+    """`t` itself where its rows lie behind each other and start on multiples of `nbytes`, else a copy whose rows do."""
     width = nbytes // t.element_size()
-    if t.numel() == 0 or (t.data_ptr() % nbytes == 0 and (t.shape[0] == 1 or t.stride(0) % width == 0)):
+    if t.numel() == 0 or (t.data_ptr() % nbytes == 0 and (t.shape[0] == 1 or (t.stride(0) >= t.shape[1] and t.stride(0) % width == 0))):
         return t
     out = torch.empty((t.shape[0], -(-t.shape[1] // width) * width), dtype=t.dtype, device=t.device)[:, :t.shape[1]]
     return out.copy_(t)
@@ -27,7 +27,8 @@ class Int4Weight:
     Stands where a layer takes a weight (Dense, GatedDense) for its forward pass.
 
     The products read 16 bytes of a row at a time: tensors whose rows do not start on 16 bytes (8 for scales, 4 for
-    zeros), as those of 1001 contiguous columns, are copied once into ones whose rows do."""
+    zeros), as those of 1001 contiguous columns, are copied once into ones whose rows do; so are repeated rows (one
+    scale expanded over all groups)."""
 
     def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group: int, rows: int):
         self.rows, self.cols, self.group = int(rows), int(packed.shape[-1]), int(group)

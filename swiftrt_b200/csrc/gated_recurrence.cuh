@@ -582,6 +582,11 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
     if constexpr (SRC == kFromTiles) {
         if (lane == 0) bulk_wait_group<0>();
     }
+    if (cluster > 1 && p.last && p.last == p.initial) {                   // a state advanced in place: the other CTAs have read it
+        __syncwarp();
+        cluster_arrive_release();
+        cluster_wait_acquire();
+    }
     if (p.last && rank == 0 && warp == 0 && on) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) p.last[b * p.last_b + (d + j) * p.last_d] = state[j];

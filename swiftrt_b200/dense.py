@@ -102,6 +102,8 @@ class Dense:
 
         dz and db come from one fused pass; dx = dz . W^T and dW = x^T . dz are the two transposed
         products that matmulGradients composes (MathDerivatives.swift:460-482, case (false, false))."""
+        if self.int4:
+            raise ValueError("a 4-bit weight has no backward pass")
         dz, db = bias_activation_backward(out_grad, output, self.activation)
         dx = matmul(dz, self.weight, False, True)
         dw = matmul(input, dz, True, False)
@@ -146,6 +148,8 @@ class GatedDense:
     def backward(self, input: torch.Tensor, saved: tuple, out_grad: torch.Tensor):
         """Gradients of (input, weightGate, weightUp, biasGate, biasUp); None for a bias that is None.  `saved` is the
         second value of forward_keep."""
+        if self.int4:
+            raise ValueError("4-bit weights have no backward pass")
         gate, up = saved
         dx, dwg, dwu, dbg, dbu = binding.gated_backward(rows_of(input), rows_of(out_grad), self.weight_gate, self.weight_up, gate, up, self.bias_gate,
                                                         self.bias_up, int(self.activation))

@@ -656,7 +656,9 @@ int4_quantize_kernel(const __grid_constant__ Int4QuantizeParams p)
         lo = fminf(lo, v);
         hi = fmaxf(hi, v);
     }
-    const T stored = from_float<T>(finite ? (p.zeros ? __fdiv_rn(hi - lo, 15.0f) : __fdiv_rn(fmaxf(hi, -lo), 7.0f)) : __int_as_float(0x7fffffff));
+    // (the range of finite BFloat16 values may exceed fp32's: the halves are subtracted then)
+    const float range = hi - lo <= 3.402823466e38f ? __fdiv_rn(hi - lo, 15.0f) : __fdiv_rn(0.5f * hi - 0.5f * lo, 7.5f);
+    const T stored = from_float<T>(finite ? (p.zeros ? range : __fdiv_rn(fmaxf(hi, -lo), 7.0f)) : __int_as_float(0x7fffffff));
     const float s = to_float<T>(stored);
     const bool some = s > 0.0f;
     float z = 8.0f;

@@ -112,8 +112,11 @@ __device__ __forceinline__ uint32_t live_steps(const RecurrenceParams& p, uint32
     return n < 0 ? 0u : min(static_cast<uint32_t>(n), p.T);
 }
 
-// One thread per channel of one batch item, step after step: up to 8 steps, where a launch is all that a call costs (16 tokens of
+// Up to this many steps one thread walks a channel of one batch item, step after step: a launch is all that such a call costs (16 tokens of
 // 2048 channels 5.3 us a call, most of it on the host).
+constexpr uint32_t kFewSteps = 8;
+static_assert(kFewSteps <= kRecurrenceChunk, "the state before the first step is the only one kept");
+
 template <typename T>
 __global__ void __launch_bounds__(128)
 recurrence_steps_kernel(const __grid_constant__ RecurrenceParams p)
@@ -123,8 +126,8 @@ recurrence_steps_kernel(const __grid_constant__ RecurrenceParams p)
     const uint32_t b = static_cast<uint32_t>(id / p.D), d = static_cast<uint32_t>(id % p.D);
     const uint32_t n = live_steps(p, b);
     float c = p.initial ? p.initial[b * p.initial_b + d * p.initial_d] : 0.0f;
+    if (p.states && p.T > 0) p.states[b * p.states_b + d * p.states_d] = c;
     for (uint32_t t = 0; t < p.T; ++t) {
-        if (p.states && t % kRecurrenceChunk == 0) p.states[b * p.states_b + (t / kRecurrenceChunk) * p.states_c + d * p.states_d] = c;
         float y = 0.0f;
         if (t < n) {
             const Gate f = logistic_pair(load3<T>(p.f, b, t, d));
@@ -137,7 +140,7 @@ recurrence_steps_kernel(const __grid_constant__ RecurrenceParams p)
     if (p.last) p.last[b * p.last_b + d * p.last_d] = c;
 }
 
-// The same for the backward pass: chunk after chunk from the end, the states of a chunk recomputed from its kept one.
+// The same for the backward pass: the states are recomputed from the kept one, then the steps are walked from the last.
 template <typename T>
 __global__ void __launch_bounds__(128)
 recurrence_steps_backward_kernel(const __grid_constant__ RecurrenceParams p)
@@ -145,7 +148,7 @@ recurrence_steps_backward_kernel(const __grid_constant__ RecurrenceParams p)
     const unsigned long long id = blockIdx.x * 128ull + threadIdx.x;
     if (id >= static_cast<unsigned long long>(p.B) * p.D) return;
     const uint32_t b = static_cast<uint32_t>(id / p.D), d = static_cast<uint32_t>(id % p.D);
-    const uint32_t n = live_steps(p, b);
+    const uint32_t n = min(live_steps(p, b), kFewSteps);
     float carry = p.dlast ? p.dlast[b * p.dlast_b + d * p.dlast_d] : 0.0f;         // f_{t+1} dc_{t+1}
     for (uint32_t t = p.T; t-- > n;) {
         store3<T>(p.dx, b, t, d, 0.0f);
@@ -153,39 +156,36 @@ recurrence_steps_backward_kernel(const __grid_constant__ RecurrenceParams p)
         if (p.i.p) store3<T>(p.di, b, t, d, 0.0f);
         if (p.o.p) store3<T>(p.dout, b, t, d, 0.0f);
     }
-    for (uint32_t chunk = (n + kRecurrenceChunk - 1) / kRecurrenceChunk; chunk-- > 0;) {
-        const uint32_t t0 = chunk * kRecurrenceChunk, t1 = min(n, t0 + kRecurrenceChunk);
-        float before[kRecurrenceChunk];
-        float c = p.states[b * p.states_b + chunk * p.states_c + d * p.states_d];
-        for (uint32_t t = t0; t < t1; ++t) {
-            before[t - t0] = c;
-            const Gate f = logistic_pair(load3<T>(p.f, b, t, d));
-            const float x = load3<T>(p.x, b, t, d);
-            c = fmaf(f.on, c, (p.i.p ? logistic(load3<T>(p.i, b, t, d)) : f.off) * x);
+    float before[kFewSteps];
+    float c = n > 0 ? p.states[b * p.states_b + d * p.states_d] : 0.0f;
+    for (uint32_t t = 0; t < n; ++t) {
+        before[t] = c;
+        const Gate f = logistic_pair(load3<T>(p.f, b, t, d));
+        const float x = load3<T>(p.x, b, t, d);
+        c = fmaf(f.on, c, (p.i.p ? logistic(load3<T>(p.i, b, t, d)) : f.off) * x);
+    }
+    for (uint32_t t = n; t-- > 0;) {
+        const Gate f = logistic_pair(load3<T>(p.f, b, t, d));
+        const float x = load3<T>(p.x, b, t, d), dy = load3<T>(p.dy, b, t, d), prev = before[t];
+        float dc = carry;
+        if (p.o.p) {
+            const Gate o = logistic_pair(load3<T>(p.o, b, t, d));
+            store3<T>(p.dout, b, t, d, dy * c * o.on * o.off);
+            dc = fmaf(dy, o.on, dc);
+        } else {
+            dc += dy;
         }
-        for (uint32_t t = t1; t-- > t0;) {
-            const Gate f = logistic_pair(load3<T>(p.f, b, t, d));
-            const float x = load3<T>(p.x, b, t, d), dy = load3<T>(p.dy, b, t, d), prev = before[t - t0];
-            float dc = carry;
-            if (p.o.p) {
-                const Gate o = logistic_pair(load3<T>(p.o, b, t, d));
-                store3<T>(p.dout, b, t, d, dy * c * o.on * o.off);
-                dc = fmaf(dy, o.on, dc);
-            } else {
-                dc += dy;
-            }
-            if (p.i.p) {
-                const Gate i = logistic_pair(load3<T>(p.i, b, t, d));
-                store3<T>(p.dx, b, t, d, dc * i.on);
-                store3<T>(p.di, b, t, d, dc * x * i.on * i.off);
-                store3<T>(p.df, b, t, d, dc * prev * f.on * f.off);
-            } else {
-                store3<T>(p.dx, b, t, d, dc * f.off);
-                store3<T>(p.df, b, t, d, dc * (prev - x) * f.on * f.off);
-            }
-            carry = dc * f.on;
-            c = prev;
+        if (p.i.p) {
+            const Gate i = logistic_pair(load3<T>(p.i, b, t, d));
+            store3<T>(p.dx, b, t, d, dc * i.on);
+            store3<T>(p.di, b, t, d, dc * x * i.on * i.off);
+            store3<T>(p.df, b, t, d, dc * prev * f.on * f.off);
+        } else {
+            store3<T>(p.dx, b, t, d, dc * f.off);
+            store3<T>(p.df, b, t, d, dc * (prev - x) * f.on * f.off);
         }
+        carry = dc * f.on;
+        c = prev;
     }
     if (p.dinitial) p.dinitial[b * p.dinitial_b + d * p.dinitial_d] = carry;
 }

@@ -194,9 +194,6 @@ bool encode_maps(const RecurrenceParams& p, EncodeTiledFn encode, RecurrenceMaps
            out(p.df, &maps.df) && out(p.di, &maps.di) && out(p.dout, &maps.dout);
 }
 
-// up to this many steps one thread walks a channel
-constexpr uint32_t kFewSteps = 8;
-
 template <typename T>
 cudaError_t launch_recurrence(RecurrenceParams& p, bool backward, int device, cudaStream_t stream)
 {

@@ -48,8 +48,10 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
     return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// The logistic function to a relative error of a few 2^-23.  The .ftz forms of the two approximations take one instruction each
-// where the others rescale denormals around them: what is below 2^-126 is zero.
+// The logistic function to a relative error of (6 + 0.61 |a|) 2^-23: the argument -log2(e) a of the power of two is rounded to fp32, which
+// counts with its size (4 units at -10, 16 at -40; an exact argument would take four more instructions a gate, and 16-bit results do not
+// show it).  The .ftz forms of the two approximations take one instruction each where the others rescale denormals around them: what is
+// below 2^-126 is zero.
 __device__ __forceinline__ float exp2_ftz(float x)
 {
     float y;
@@ -108,10 +110,9 @@ template <typename T> __device__ __forceinline__ float gate_slope(uint32_t act, 
     }
 }
 
-// s(a), and s(a) with 1 - s(a), each to a relative error of a few 2^-23: with e = exp(-a) they are 1 / (1 + e) and
+// s(a) with 1 - s(a), each to the relative error of logistic(): with e = exp(-a) they are 1 / (1 + e) and
 // e / (1 + e), neither of which is the difference of 1 and its neighbour (a gate at 0.9999 keeps its decay 1 - f to full
-// precision).  The .ftz forms of the two approximations take one instruction each where the others rescale denormals
-// around them.  For the pair e is capped at 2^126, so that a closed gate is 2^-126 and not 0 times infinity.
+// precision).  For the pair e is capped at 2^126, so that a closed gate is 2^-126 and not 0 times infinity.
 struct Gate { float on, off; };
 __device__ __forceinline__ float min_or_nan(float a, float b)
 {

@@ -466,10 +466,12 @@ cudaError_t srtMatmulGated(
  * (Float16 / BFloat16 views whose rows start on 16 bytes, dX's being whole 16 bytes long); where it is needed and NULL
  * the call returns cudaErrorNotSupported before it launches anything.  With it each of the two products is rounded
  * before their sum is.  Results do not depend on timing.  M, K and H are at least 1.  Both weights' gradients are one batched product where
- * dUp and dWUp lie in the same direction from dGate and dWGate, with equal strides.
+ * dUp follows dGate, and dWUp follows dWGate, as the second matrix of a dense [2 x rows x cols] tensor follows the first.
  * The products (but those of srtMatmulGated that are one launch) may use the library's per-(device, stream) workspace, as
  * srtMatmul does.  Those of Float16 and BFloat16 do not in a captured call, so that graphs
- * captured on one stream may run at once; their last bits may then differ from those of a call that is not captured. */
+ * captured on one stream may run at once; their last bits may then differ from those of a call that is not captured, and a
+ * backward pass of few rows, whose long reductions are not split then, takes longer (2 rows of 4096 x 2 x 8192 114 instead of
+ * 84 us, 50 rows of 512 x 2 x 8192 82 instead of 51). */
 cudaError_t srtMatmulGatedBackward(
     const void* outGrad, const srtTensorDescriptor* outGradDesc,
     const void* x, const srtTensorDescriptor* xDesc,

@@ -105,6 +105,21 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Device& d
     return at::detail::empty_cuda(sizes, type, device, std::nullopt);
 }
 
+// two matrices in one allocation, both starting on 16 bytes: a dense [2 x rows x cols] tensor where that is one
+std::pair<at::Tensor, at::Tensor> empty_pair(int64_t rows, int64_t cols, at::ScalarType type, const at::Device& device)
+{
+    const int64_t unit = 16 / static_cast<int64_t>(c10::elementSize(type)), apart = (rows * cols + unit - 1) / unit * unit;
+    const at::Tensor whole = empty({apart + rows * cols}, type, device);
+    const auto part = [&](int64_t offset) {
+        auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+        impl->set_storage_offset(offset);
+        const int64_t sizes[2] = {rows, cols};
+        impl->set_sizes_contiguous(sizes);
+        return at::Tensor(std::move(impl));
+    };
+    return {part(0), part(apart)};
+}
+
 // the device made current where it is not, and torch's current stream there
 struct Queue {
     c10::cuda::OptionalCUDAGuard guard;
@@ -291,12 +306,10 @@ PyObject* gated_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
         Queue q(x);
         const at::ScalarType type = x.scalar_type();
         const int64_t rows = x.size(0), inner = x.size(1), cols = wg.size(1);
-        at::Tensor dgate = empty({rows, cols}, type, x.device()), dup = empty({rows, cols}, type, x.device());
+        // the matrices of a pair lie behind each other: batched products
+        const auto [dgate, dup] = empty_pair(rows, cols, type, x.device());
+        const auto [dwg, dwu] = empty_pair(inner, cols, type, x.device());
         const at::Tensor dx = empty({rows, inner}, type, x.device());
-        at::Tensor dwg = empty({inner, cols}, type, x.device()), dwu = empty({inner, cols}, type, x.device());
-        // all pairs in one direction: batched products
-        if ((dup.data_ptr() > dgate.data_ptr()) != (wu.data_ptr() > wg.data_ptr())) std::swap(dgate, dup);
-        if ((dup.data_ptr() > dgate.data_ptr()) != (dwu.data_ptr() > dwg.data_ptr())) std::swap(dwg, dwu);
         at::Tensor dbg, dbu, dx2;
         if (bg) dbg = empty(bg->sizes(), type, x.device());
         if (bu) dbu = empty(bu->sizes(), type, x.device());

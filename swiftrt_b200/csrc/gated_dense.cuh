@@ -51,44 +51,22 @@ struct GateBackwardParams {
     void* sum_g; long long sum_g_n;          // bias gradients, may be null
     void* sum_u; long long sum_u_n;
     uint32_t M, N, act;
-    uint32_t* status;                        // of the device, and the limit of a wait in SM cycles
-    unsigned long long wait_cycles;
 };
 
-// `v` to the same place in the shared memory of CTA `rank`, counted there on its barrier
-__device__ __forceinline__ void send_to_cta(uint32_t at, uint32_t bar, uint32_t rank, float v)
-{
-    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];"
-                 ::"r"(map_to_cta(at, rank)), "r"(__float_as_uint(v)), "r"(map_to_cta(bar, rank)) : "memory");
-}
-
-// A CTA owns 8 VEC columns: a warp's lanes are 8 column groups by 4 rows, its 8 warps 32 rows.  The CTAs of a cluster
-// (grid y) walk the same columns at interleaved groups of 32 rows; the column sums of a cluster's CTAs are added in rank order
-// in the first CTA's shared memory, where each CTA sends its own counted by a barrier: no scratch memory, no atomics, and no CTA waits for its
-// stores as at a barrier of the cluster.  The unrounded fp32 values are summed.
-// Reading three and writing two values an element bounds it: 3999 x 8200 bf16 70 us (4.7 TB/s), without the sums 60 us (5.5 TB/s).  Gates of four
-// values at a time and three CTAs an SM took it from 87 to 77 us, sums sent instead of read behind a barrier of the cluster to 70.
-template <typename T, int VEC>
+// A CTA owns 8 VEC columns: a warp's lanes are 8 column groups by 4 rows, its 8 warps 32 rows.  With CLUSTER the CTAs of a cluster
+// (grid y, 2 .. 8 of them) walk the same columns at interleaved groups of 32 rows; each leaves its column sums in its shared memory, and
+// behind a barrier of the cluster the first CTA adds them in rank order: no scratch memory, no atomics.  Up to 32 rows are one CTA's,
+// which needs no cluster.  The unrounded fp32 values are summed.
+// Reading three and writing two values an element bounds it: 3999 x 8200 bf16 82 us (4.0 TB/s) from a cold cache, without the sums 64 us (5.2 TB/s).
+// Gates of four values at a time and three CTAs an SM took a tenth off.  Sums sent with st.async instead saved another tenth; that is not
+// used here since a launch with clusters of one CTA, which sent to itself, is under suspicion of an illegal access.
+template <typename T, int VEC, bool CLUSTER>
 __global__ void __launch_bounds__(256, 3)
 gate_backward_kernel(const __grid_constant__ GateBackwardParams p)
 {
     constexpr uint32_t kCols = 8 * VEC;
     __shared__ float sums[2][8][kCols];
-    __shared__ alignas(16) float gathered[8][2][kCols];                 // of the cluster's CTAs, in rank 0
-    __shared__ alignas(8) uint64_t arrived;
-    __shared__ volatile uint32_t never_set;
-    const bool with_sums = p.sum_g != nullptr || p.sum_u != nullptr;    // uniform over the grid
-    const uint32_t rank = with_sums ? cluster_ctarank() : 0;
-    if (with_sums) {
-        if (threadIdx.x == 0) {
-            never_set = 0;
-            mbar_init(smem_u32(&arrived), 1);
-            fence_mbar_init();
-            if (rank == 0) mbar_arrive_expect_tx(smem_u32(&arrived), gridDim.y * static_cast<uint32_t>(sizeof gathered[0]));
-        }
-        __syncwarp();
-        cluster_arrive_release();
-    }
+    __shared__ float total[2][kCols];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t col = (blockIdx.x * 8 + (lane & 7)) * VEC;
     float sg[VEC], su[VEC];
@@ -146,7 +124,7 @@ gate_backward_kernel(const __grid_constant__ GateBackwardParams p)
             }
         }
     }
-    if (!with_sums) return;
+    if (p.sum_g == nullptr && p.sum_u == nullptr) return;               // uniform over the grid
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         sg[j] += __shfl_xor_sync(0xffffffffu, sg[j], 8);
@@ -160,25 +138,31 @@ gate_backward_kernel(const __grid_constant__ GateBackwardParams p)
     }
     __syncthreads();
     const uint32_t which = threadIdx.x / kCols, c = threadIdx.x % kCols;
-    cluster_wait_acquire();                                             // rank 0's barrier is set up
+    float s = 0.0f;
     if (which < 2) {
-        float s = sums[which][0][c];
+        s = sums[which][0][c];
 #pragma unroll
         for (int w = 1; w < 8; ++w) s += sums[which][w][c];
-        send_to_cta(smem_u32(&gathered[rank][which][c]), smem_u32(&arrived), 0, s);
     }
-    if (rank == 0 && which < 2) {
-        if (!mbar_wait(smem_u32(&arrived), 0, &never_set, p.wait_cycles)) {
-            atomicOr(p.status, 1u);                                     // (the result is invalid; what is on its way has to land)
-            mbar_wait(smem_u32(&arrived), 0, &never_set, 4000000000ull);
-        }
-        float s = 0.0f;
-        for (uint32_t r = 0; r < gridDim.y; ++r) s += gathered[r][which][c];
-        const uint32_t n = blockIdx.x * kCols + c;
-        if (n < p.N) {
-            if (which == 0 && p.sum_g) static_cast<T*>(p.sum_g)[n * p.sum_g_n] = from_float<T>(s);
-            if (which == 1 && p.sum_u) static_cast<T*>(p.sum_u)[n * p.sum_u_n] = from_float<T>(s);
-        }
+    uint32_t rank = 0;
+    if constexpr (CLUSTER) {
+        rank = cluster_ctarank();
+        if (which < 2) total[which][c] = s;
+        __syncwarp();
+        cluster_arrive_release();
+        cluster_wait_acquire();
+        if (rank == 0 && which < 2)
+            for (uint32_t r = 1; r < gridDim.y; ++r) s += __uint_as_float(ld_shared_remote_u32(smem_u32(&total[which][c]), r));
+    }
+    const uint32_t n = blockIdx.x * kCols + c;
+    if (rank == 0 && which < 2 && n < p.N) {
+        if (which == 0 && p.sum_g) static_cast<T*>(p.sum_g)[n * p.sum_g_n] = from_float<T>(s);
+        if (which == 1 && p.sum_u) static_cast<T*>(p.sum_u)[n * p.sum_u_n] = from_float<T>(s);
+    }
+    if constexpr (CLUSTER) {                                             // a CTA's sums are read until here
+        __syncwarp();
+        cluster_arrive_release();
+        cluster_wait_acquire();
     }
 }
 

@@ -1801,6 +1801,16 @@ cudaError_t gated_rows(srtDataType type, const Matrix& x, const Matrix& wg, cons
     return gated_few_rows(type, p, !by_rows, limit, device, stream);
 }
 
+// the partial sums of a split-K product of 16-bit operands, into the workspace that it is bound to
+cudaError_t launch_first_pass(Prepared& pr, cudaStream_t stream)
+{
+    pr.gp.wait_cycles = g_wait_limit_ns.load(std::memory_order_relaxed) * 2;
+    const cudaError_t e = pr.type == real16F ? launch_tc_bn<__half, float>(pr.bn, pr.ma, pr.mb, pr.mo, pr.gp, pr.ctas, pr.smem, stream)
+                                             : launch_tc_bn<__nv_bfloat16, float>(pr.bn, pr.ma, pr.mb, pr.mo, pr.gp, pr.ctas, pr.smem, stream);
+    if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return e;
+}
+
 // out = a1 . b1^T + a2 . b2^T (a [M x K], b [N x K]) in one launch
 cudaError_t sum_fused(srtDataType type, const Matrix& a1, const Matrix& b1, const Matrix& a2, const Matrix& b2, const Matrix& out, const DeviceInfo& dev,
                       cudaStream_t stream)
@@ -1835,24 +1845,22 @@ cudaError_t sum_fused(srtDataType type, const Matrix& a1, const Matrix& b1, cons
     return e;
 }
 
-// The same where its tiles are few and the reduction long: a batch of the two products whose fp32 partial sums, cut along K too,
-// are all added by one reduce pass.  The two pairs of operands have to lie in one direction from each other.  Backward pass of 2 rows, 4096 x 2 x
-// 8192: 121 -> 80 us; 50 rows, 512 x 2 x 8192: 77 -> 35 us; 1001 rows, 504 x 2 x 8192: 110 -> 86 us.  cudaErrorNotSupported: not such a product.
+// The same where its tiles are few and the reduction long: both products cut along K, their fp32 partial sums side by side in the workspace
+// and all added by one reduce pass.  Backward pass (without, with) of 2 rows, 4096 x 2 x 8192: 114, 84 us; 50 rows, 512 x 2 x 8192: 82, 51 us;
+// 1001 rows, 504 x 2 x 8192: 108, 88 us.  (Two launches, not a batch of two: a tensor map over both weights would span separate
+// allocations, with a stride that is no multiple of a row's.)  cudaErrorNotSupported: not such a product.
 cudaError_t sum_split(srtDataType type, const Matrix& a1, const Matrix& b1, const Matrix& a2, const Matrix& b2, const Matrix& out, const DeviceInfo& dev,
-                      cudaStream_t stream)
+                      int dev_ordinal, cudaStream_t stream)
 {
     const uint64_t tiles = ((out.rows + 255) / 256) * ((out.cols + 255) / 256), k_blocks = (a1.cols + 63) / 64;
     if (type == real32F || tiles > (uint64_t)dev.sms / 4 || k_blocks < 50) return cudaErrorNotSupported;
-    long long a_apart = (long long)(reinterpret_cast<intptr_t>(a2.p) - reinterpret_cast<intptr_t>(a1.p));
-    long long b_apart = (long long)(reinterpret_cast<intptr_t>(b2.p) - reinterpret_cast<intptr_t>(b1.p));
-    const bool ahead = a_apart > 0 && b_apart > 0, behind = a_apart < 0 && b_apart < 0;
-    if (!(ahead || behind) || a1.m != a2.m || a1.n != a2.n || b1.m != b2.m || b1.n != b2.n || a_apart % 2 != 0 || b_apart % 2 != 0) return cudaErrorNotSupported;
+    if (a1.m != a2.m || a1.n != a2.n || b1.m != b2.m || b1.n != b2.n) return cudaErrorNotSupported;
     Problem P;
     memset(&P, 0, sizeof P);
-    P.type = type; P.elem = 2; P.batch = 2;
+    P.type = type; P.elem = 2; P.batch = 1;
     P.M = out.rows; P.N = out.cols; P.K = a1.cols;
-    P.a = (ahead ? a1 : a2).p; P.a_b = (ahead ? a_apart : -a_apart) / 2; P.a_m = a1.m; P.a_k = a1.n;
-    P.b = (ahead ? b1 : b2).p; P.b_b = (ahead ? b_apart : -b_apart) / 2; P.b_n = b1.m; P.b_k = b1.n;
+    P.a = a1.p; P.a_m = a1.m; P.a_k = a1.n;
+    P.b = b1.p; P.b_n = b1.m; P.b_k = b1.n;
     P.out = const_cast<char*>(out.p); P.o_m = out.m; P.o_n = out.n;
     P.act = kActIdentity;
     Plan plan;
@@ -1862,19 +1870,24 @@ cudaError_t sum_split(srtDataType type, const Matrix& a1, const Matrix& b1, cons
         plan.splits = 2;
         plan.kb_per_split = (uint32_t)((k_blocks + 1) / 2);
         plan.pub.splitK = 2;
-        plan.pub.workspaceBytes = (size_t)2 * P.batch * P.M * P.N * 4;
+        plan.pub.workspaceBytes = (size_t)2 * P.M * P.N * 4;
         plan.pub.ctas = 2 * plan.pub.tiles < dev.sms ? 2 * plan.pub.tiles : dev.sms;
     }
-    std::unique_ptr<Prepared> pr(new Prepared());
-    cudaError_t e = prepare_tc(plan, *pr);
+    std::unique_ptr<Prepared> first(new Prepared()), second(new Prepared());
+    cudaError_t e = prepare_tc(plan, *first);
     if (e != cudaSuccess) return e;
-    ReduceParams& rp = pr->rp;                               // [split][product][M][N]: as many parts of one result
+    Problem& Q = plan.Q;                                     // the second pair of operands, where the first one's are
+    (plan.swapped ? Q.b : Q.a) = a2.p;
+    (plan.swapped ? Q.a : Q.b) = b2.p;
+    if ((e = prepare_tc(plan, *second)) != cudaSuccess) return e;
+    void* ws = nullptr;
+    if ((e = workspace_for(dev_ordinal, stream, 2 * plan.pub.workspaceBytes, &ws)) != cudaSuccess) return e;
+    if ((e = bind_workspace(*first, ws)) != cudaSuccess || (e = bind_workspace(*second, static_cast<char*>(ws) + plan.pub.workspaceBytes)) != cudaSuccess) return e;
+    if ((e = launch_first_pass(*first, stream)) != cudaSuccess || (e = launch_first_pass(*second, stream)) != cudaSuccess) return e;
+    ReduceParams& rp = first->rp;                            // [product][split][M][N]: as many parts of one result
     rp.splits = 2 * plan.splits;
-    rp.slice = (unsigned long long)rp.M * rp.N;
-    rp.batch = 1;
-    const unsigned long long blocks = (rp.slice / pr->reduce_vec + 255) / 256;
-    pr->reduce_blocks = (uint32_t)(blocks < 148ull * 16 ? blocks : 148ull * 16);
-    return launch_prepared(*pr, stream);
+    if ((e = launch_reduce(*first, stream)) == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
+    return e;
 }
 
 template <typename T>
@@ -1890,19 +1903,27 @@ cudaError_t launch_gate_backward(const GateBackwardParams& gp, bool vec, cudaStr
         rows = (148u * 8 + col_blocks - 1) / col_blocks;
         if (rows > row_groups) rows = row_groups;
     }
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof cfg);
-    cfg.gridDim = dim3(col_blocks, rows, 1);
-    cfg.blockDim = dim3(256, 1, 1);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = sums ? rows : 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = launch_status(vec ? cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, kVec>, gp) : cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, 1>, gp));
+    const dim3 grid(col_blocks, rows, 1);
+    cudaError_t e;
+    if (sums && rows > 1) {
+        cudaLaunchConfig_t cfg;
+        memset(&cfg, 0, sizeof cfg);
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(256, 1, 1);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 1;
+        attr[0].val.clusterDim.y = rows;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = launch_status(vec ? cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, kVec, true>, gp) : cudaLaunchKernelEx(&cfg, gate_backward_kernel<T, 1, true>, gp));
+    } else {
+        if (vec) gate_backward_kernel<T, kVec, false><<<grid, 256, 0, stream>>>(gp);
+        else     gate_backward_kernel<T, 1, false><<<grid, 256, 0, stream>>>(gp);
+        e = cudaGetLastError();
+    }
     if (e == cudaSuccess) g_launches.fetch_add(1, std::memory_order_relaxed);
     return e;
 }
@@ -2790,10 +2811,6 @@ cudaError_t srtMatmulGatedBackward(const void* outGrad, const srtTensorDescripto
     gp.dg = View2W{dGate, dg.m, dg.n}; gp.du = View2W{dUp, du.m, du.n};
     gp.sum_g = dBiasGate; gp.sum_g_n = sg_n; gp.sum_u = dBiasUp; gp.sum_u_n = su_n;
     gp.M = (uint32_t)M; gp.N = (uint32_t)H; gp.act = (uint32_t)activation;
-    TileServices services;
-    if ((e = tile_services(scope.device, services)) != cudaSuccess) return e;
-    gp.status = services.status;
-    gp.wait_cycles = services.wait_cycles;
     auto vec_ok = [&](const Matrix& v) {
         return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && v.n == 1 && (v.m * (long long)elem) % 16 == 0;
     };
@@ -2804,7 +2821,7 @@ cudaError_t srtMatmulGatedBackward(const void* outGrad, const srtTensorDescripto
 
     const bool captured = is_captured(stream);
     if (dX && one_launch) {
-        e = captured ? cudaErrorNotSupported : sum_split(type, dg, wg, du, wu, dx, info, stream);
+        e = captured ? cudaErrorNotSupported : sum_split(type, dg, wg, du, wu, dx, info, scope.device, stream);
         if (e == cudaErrorNotSupported) e = sum_fused(type, dg, wg, du, wu, dx, info, stream);
         if (e != cudaSuccess) return e;
     } else if (dX) {
@@ -2829,16 +2846,14 @@ cudaError_t srtMatmulGatedBackward(const void* outGrad, const srtTensorDescripto
         const LocalDescriptor d_x(mx, type, batch), d_out(ov, type, batch, out_apart), d_g(dv, type, batch, apart);
         return run_matmul(x, &d_x.d, true, gradient, &d_g.d, false, nullptr, nullptr, srtActivationIdentity, out, &d_out.d, stream, false, captured);
     };
-    // both weights' gradients as one batch of two where the second pair lies in the same direction from the first: fewer of the
-    // tiles run in a last, partly empty wave.  Reduction 3999, 4096 x 8200 bf16: 2 x 247 -> 442 us; 1000, 1024 x 4096: 2 x 17 -> 26 us
-    if (dWGate && dWUp) {
-        const long long from = (long long)(reinterpret_cast<intptr_t>(dUp) - reinterpret_cast<intptr_t>(dGate));
-        const long long to = (long long)(reinterpret_cast<intptr_t>(dWUp) - reinterpret_cast<intptr_t>(dWGate));
-        const bool ahead = from > 0 && to > 0, behind = from < 0 && to < 0;
-        const long long apart = ahead ? from : -from, out_apart = ahead ? to : -to;
-        if ((ahead || behind) && dg.m == du.m && dg.n == du.n && dwg.m == dwu.m && dwg.n == dwu.n && apart % elem == 0 && out_apart % elem == 0)
-            return product(ahead ? dGate : dUp, dg, ahead ? dWGate : dWUp, dwg, 2, (size_t)(apart / elem), (size_t)(out_apart / elem));
-    }
+    // both weights' gradients as one batch of two where the second of either pair follows the first as the second matrix of a dense
+    // tensor does: fewer of the tiles run in a last, partly empty wave.  Reduction 3999, 4096 x 8200 bf16: 2 x 247 -> 442 us; 1000,
+    // 1024 x 4096: 2 x 17 -> 26 us
+    const auto follows = [&](const Matrix& first, const Matrix& second) {
+        return first.n == 1 && second.n == 1 && first.m == second.m && first.m >= (long long)first.cols && second.p == first.p + first.rows * first.m * (long long)elem;
+    };
+    if (dWGate && dWUp && follows(dg, du) && follows(dwg, dwu))
+        return product(dGate, dg, dWGate, dwg, 2, (size_t)(dg.rows * dg.m), (size_t)(dwg.rows * dwg.m));
     if (dWGate && (e = product(dGate, dg, dWGate, dwg, 0, 0, 0)) != cudaSuccess) return e;
     if (dWUp && (e = product(dUp, du, dWUp, dwu, 0, 0, 0)) != cudaSuccess) return e;
     return cudaSuccess;

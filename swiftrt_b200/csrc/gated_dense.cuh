@@ -148,7 +148,6 @@ gate_backward_kernel(const __grid_constant__ GateBackwardParams p)
     if constexpr (CLUSTER) {
         rank = cluster_ctarank();
         if (which < 2) total[which][c] = s;
-        __syncwarp();
         cluster_arrive_release();
         cluster_wait_acquire();
         if (rank == 0 && which < 2)
@@ -160,7 +159,6 @@ gate_backward_kernel(const __grid_constant__ GateBackwardParams p)
         if (which == 1 && p.sum_u) static_cast<T*>(p.sum_u)[n * p.sum_u_n] = from_float<T>(s);
     }
     if constexpr (CLUSTER) {                                             // a CTA's sums are read until here
-        __syncwarp();
         cluster_arrive_release();
         cluster_wait_acquire();
     }

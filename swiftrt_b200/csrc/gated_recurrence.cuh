@@ -583,7 +583,6 @@ recurrence_span_kernel(const __grid_constant__ RecurrenceParams p, const __grid_
         if (lane == 0) bulk_wait_group<0>();
     }
     if (cluster > 1 && p.last && p.last == p.initial) {                   // a state advanced in place: the other CTAs have read it
-        __syncwarp();
         cluster_arrive_release();
         cluster_wait_acquire();
     }

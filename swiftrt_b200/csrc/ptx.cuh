@@ -429,10 +429,12 @@ __device__ __forceinline__ uint32_t cluster_ctarank()
 }
 __device__ __forceinline__ void cluster_arrive_release()
 {
+    __syncwarp();                        // .aligned: all lanes arrive as one
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait_acquire()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 

@@ -516,7 +516,7 @@ typedef struct {
 /* out = activation(x . W + bias): what srtMatmulBiasActivation computes with the weight above.  x [M x rows], out [M x cols] and bias
  * [cols] (NULL: none) have the weight's `type`; x and out any strides, out must not overlap anything.  The products of x
  * and the integers q - z are summed in fp32 and scaled group by group, in fp32: no weight is rounded, and the result is
- * rounded once.  Any M; the weight is read once for every 8, 16 or 32 rows (gated: 8 or 16; whichever is estimated to be
+ * rounded once.  M up to 1 048 560; the weight is read once for every 8, 16 or 32 rows (gated: 8 or 16; whichever is estimated to be
  * fastest), so that many rows are better served by srtDequantizeInt4 and srtMatmul.  One launch, no workspace, and a result that does not depend on timing.  All activations but clippedRelu and elu. */
 cudaError_t srtMatmulInt4(
     const void* x, const srtTensorDescriptor* xDesc,

@@ -6,7 +6,7 @@
 //
 //   Int4   word (j, n) of the packed weight: rows 8 j .. 8 j + 7 of column n.  Lane (g, t) of a warp takes 4 columns (16 bytes)
 //          of one word row: 32 columns x 32 rows per step.  Two nibbles at a time become the 16-bit floats 128 + q (bf16) or
-//          1024 + q (fp16) by one AND-OR; subtracting 128 + z (1024 + z) is exact, so the MMA multiplies the integers
+//          1024 + q (fp16) by one AND-OR (as published by Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't Run", 2022); subtracting 128 + z (1024 + z) is exact, so the MMA multiplies the integers
 //          q - z and the group's scale is applied to its fp32 sum, once per group: no weight is ever rounded.
 //   Rows   16-bit elements, columns contiguous ([K x N] as Dense keeps it): lane (g, t) takes 8 columns of four rows;
 //          neighbouring rows are paired by byte permutes.

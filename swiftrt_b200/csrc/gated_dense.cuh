@@ -59,7 +59,7 @@ struct GateBackwardParams {
 // which needs no cluster.  The unrounded fp32 values are summed.
 // Reading three and writing two values an element bounds it: 3999 x 8200 bf16 82 us (4.0 TB/s) from a cold cache, without the sums 64 us (5.2 TB/s).
 // Gates of four values at a time and three CTAs an SM took a tenth off.  Sums sent with st.async instead saved another tenth; that is not
-// used here since a launch with clusters of one CTA, which sent to itself, is under suspicion of an illegal access.
+// done: launches with clusters of one CTA, which sent to itself, are among the suspects of an illegal access.
 template <typename T, int VEC, bool CLUSTER>
 __global__ void __launch_bounds__(256, 3)
 gate_backward_kernel(const __grid_constant__ GateBackwardParams p)

@@ -147,7 +147,7 @@ class GatedDense:
 
     def backward(self, input: torch.Tensor, saved: tuple, out_grad: torch.Tensor):
         """Gradients of (input, weightGate, weightUp, biasGate, biasUp); None for a bias that is None.  `saved` is the
-        second value of forward_keep."""
+        second value of forward_keep.  Both weights' gradients are parts of one allocation."""
         if self.int4:
             raise ValueError("4-bit weights have no backward pass")
         gate, up = saved

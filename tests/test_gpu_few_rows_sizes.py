@@ -130,3 +130,12 @@ def test_gated_4_bit_product_without_room_for_x(srt):
     ea = 1.1 * eg + 2.0 ** -20 * a.abs()
     _check(got, a * u, ea * (u.abs() + eu) + a.abs() * eu + 2.0 ** -23 * (a * u).abs())
     assert srt.check_status() == 0
+
+
+def test_more_rows_than_a_launch_has_room_for_are_refused(srt):
+    w = _int4_weight(srt, 1, 4, 32, torch.bfloat16, False)
+    x = torch.ones(1, 1, dtype=torch.bfloat16, device=DEV)
+    most = 1048560
+    assert torch.equal(srt.matmul_int4(x.expand(most, 1), w)[::4099], srt.matmul_int4(x, w).expand(256, 4))
+    with pytest.raises(srt.MatmulError, match="too many rows"):
+        srt.matmul_int4(x.expand(2200000, 1), w)

@@ -29,7 +29,7 @@ int main()
         for (uint32_t M : {1, 2, 7, 8, 9, 12, 13, 15, 16, 17, 24, 25, 31, 32, 33, 40, 48, 63, 64, 70, 100, 128, 200, 256, 509, 512})
             for (uint32_t K : {64, 100, 129, 256, 500, 1024, 1111, 2048, 2500, 3200, 4096, 5000, 6144, 6400, 7168, 8192, 8200, 10240, 11008, 12288, 14336, 16384, 20000, 24576,
                                24816, 28672, 32768, 50000, 65536, 100000, 110000, 131072})
-                for (uint32_t N : {64, 100, 512, 1001, 2048, 4096, 5000, 8192, 12288, 14336, 16384, 24576, 28672, 30720, 40408, 65536, 128256, 262144})
+                for (uint32_t N : {64, 100, 512, 1001, 2048, 4096, 5000, 8192, 12288, 14336, 16384, 24576, 28672, 30976, 40408, 65536, 128256, 262144})
                     for (uint32_t most = 1; most <= 3; ++most) {
                         const RowsPlan p = plan_few_rows(k.f, k.nw, k.nt, M, N, K, most);
                         const auto check = [&](bool ok, const char* what) { expect(ok, what, k.name, k.nw, k.nt, M, K, N, most, p); };
